@@ -245,6 +245,108 @@ IRT_API int irt_codec_decode_ragged(irt_codec* c, const float* latent, int32_t b
 IRT_API int irt_codec_decode_noalloc(irt_codec* c, const float* latent, int32_t batch, int32_t frames, float* wav,
                                      void* stream);
 
+/* ---- attention over context states --------------------------------------- */
+
+/*
+ * Operators of the joint attention (src/model/attention.rs:403-418, :619-664)
+ * for programs that attend to encoder states outside the engine: attention of
+ * packed queries over the states of an encoder, and over a context cache held
+ * in 4 bits.  They differ from the engine's calls in three ways: every pointer
+ * is device memory of GPU `device`; the work is queued on `stream` (a
+ * cudaStream_t, NULL = that GPU's legacy default stream) and the call returns
+ * without waiting for it, so it can be captured into a CUDA graph; and no
+ * state is kept, so calls from several threads and streams are independent.
+ * The current device of the calling thread is left as it was.
+ *
+ * Rows of heads: element (row, head, d) of a tensor is at
+ * data[row * row_stride + head * head_stride + d], strides in elements.
+ * Types: irt_precision (IRT_PREC_BF16: bf16, IRT_PREC_F32: float) for every
+ * tensor of a call; scores, softmax and sums are f32 in both.  Query head h
+ * reads KV head h / (heads / kv_heads).  head_dim is a multiple of 8, 8..256.
+ */
+typedef struct irt_rows {
+  void* data;
+  int64_t row_stride, head_stride;
+} irt_rows;
+
+/* One sequence: queries [q_start, q_start + q_len) attend to the context rows
+ * [k_start, k_start + k_len).  Context ranges may overlap (guidance variants
+ * of one utterance read sub-ranges of the same rows); query ranges must not. */
+typedef struct irt_attn_seq {
+  int32_t q_start, q_len, k_start, k_len;
+} irt_attn_seq;
+
+typedef struct irt_attn_args {
+  int32_t device;
+  int32_t dtype;               /* irt_precision of q, k, v, gate and out */
+  int32_t heads, kv_heads, head_dim;
+  int32_t num_seqs;
+  int32_t max_q_len, max_k_len; /* upper bounds of the table's q_len, k_len */
+  float scale;                 /* of the scores; 1 / sqrt(head_dim) in the model */
+  int64_t q_rows;              /* rows of q, gate and out */
+  /* [num_seqs] in device memory.  An entry outside q_rows, the context rows or
+   * the two bounds above is skipped: its output rows are left as they were,
+   * like the rows that no entry covers.  NULL: sequence i has max_q_len rows
+   * from i * max_q_len and max_k_len context rows from i * max_k_len. */
+  const irt_attn_seq* seqs;
+  irt_rows q;                  /* [q_rows, heads, head_dim] */
+  irt_rows gate;               /* as q, multiplied into the output; data NULL: none */
+  irt_rows out;                /* as q; must not overlap any input */
+  const uint8_t* key_mask;     /* [context rows], non-zero = attend; NULL: all.  A masked row is
+                                * not read for its values: it may hold anything, NaN included */
+  float* lse;                  /* [q_rows, heads] log of the softmax's sum, or NULL */
+} irt_attn_args;
+
+/* Cross attention to an encoder's states k, v [k_rows, kv_heads, head_dim].
+ * A query without any key gives 0 and lse = -inf (the model's safe softmax,
+ * src/model/attention.rs:675-724). */
+IRT_API int irt_cross_attention(const irt_attn_args* a, const irt_rows* k, const irt_rows* v, int64_t k_rows,
+                                void* stream);
+
+/*
+ * Context cache in 4 bits: the K and V rows of an encoder's states, 4.5 bits a
+ * value.  Each row of a KV head is cut into groups of 32 values (the last one
+ * may be shorter).  A group has one scale s, the smallest number of 5
+ * significant bits with 7 s >= max|x| (at most 1.125 * 2^125); its values are
+ * c s with c = x / s rounded to the nearest of -7..7 (halves away from zero).
+ * A group with max|x| < 2^-100 holds zeros, one with an infinity or NaN reads
+ * as NaN.  c s has at most 8 significant bits, so it is a bf16 number and the
+ * tensor cores multiply it without a further rounding.
+ * Codes c + 8 are packed two a byte, the even index in the low half; scales
+ * are bf16.  Each KV head's rows are contiguous.  The buffers are the
+ * caller's, aligned to 16 bytes.
+ */
+typedef struct irt_kv4_cache {
+  int64_t rows;
+  int32_t kv_heads, head_dim;
+  uint8_t* k_codes;            /* [kv_heads, rows, head_dim / 2] */
+  uint16_t* k_scales;          /* [kv_heads, rows, ceil(head_dim / 32)] bf16 */
+  uint8_t* v_codes;
+  uint16_t* v_scales;
+} irt_kv4_cache;
+
+/* Cache rows [row_start, row_start + n) = the source rows src_index[0..n)
+ * (int32 device memory; NULL: rows 0..n) of k, v [src_rows, kv_heads,
+ * head_dim].  A source index outside [0, src_rows) leaves its cache row as it
+ * was; several cache rows may take the same source row. */
+IRT_API int irt_kv4_append(int device, int dtype, const irt_kv4_cache* cache, int64_t row_start, int64_t n,
+                           const irt_rows* k, const irt_rows* v, int64_t src_rows, const int32_t* src_index,
+                           void* stream);
+/* The values that cache rows [row_start, row_start + n) hold, into rows 0..n
+ * of k and v.  Exact in bf16 and f32. */
+IRT_API int irt_kv4_read(int device, int dtype, const irt_kv4_cache* cache, int64_t row_start, int64_t n,
+                         const irt_rows* k, const irt_rows* v, void* stream);
+/* Attention over [own rows | context rows of the cache].  k_self, v_self
+ * [q_rows, kv_heads, head_dim]: a sequence's queries also attend to the rows
+ * of its own query range, unmasked, as in the model's joint attention; NULL:
+ * the cache alone. */
+IRT_API int irt_kv4_attention(const irt_attn_args* a, const irt_kv4_cache* cache, const irt_rows* k_self,
+                              const irt_rows* v_self, void* stream);
+/* Waits for GPU `device` and reports whether a bounded wait inside one of the
+ * attention operators' kernels has expired since the last check (IRT_E_CUDA:
+ * outputs since then are invalid). */
+IRT_API int irt_attention_check(int device);
+
 #ifdef __cplusplus
 }
 #endif

@@ -611,8 +611,14 @@ def load_codec(path: str, device: int = 0, precision: str = "f32") -> DacVaeCode
     return DacVaeCodec(h, device)
 
 
+from .ops import (SIGNATURES as _OP_SIGNATURES, Kv4Cache, attention_check, attention_table, cross_attention,  # noqa: E402
+                  kv4_append, kv4_attention, kv4_read)
+
+_SIGNATURES.update(_OP_SIGNATURES)
+
 __all__ = [
     "InferenceBuilder", "LoadedBuilder", "ReadyBuilder", "InferenceEngine", "SamplerParams", "GuidanceConfig",
     "TemporalRescaleConfig", "SpeakerKvConfig", "SamplingRequest", "DacVaeCodec", "load_codec", "IrodoriError",
-    "ConfigError", "StateError", "lib", "version", "LIB_PATH",
+    "ConfigError", "StateError", "lib", "version", "LIB_PATH", "Kv4Cache", "attention_check", "attention_table",
+    "cross_attention", "kv4_append", "kv4_attention", "kv4_read",
 ]

@@ -7,6 +7,7 @@
 
 #include "codec.hpp"
 #include "config.hpp"
+#include "ctx_attn.hpp"
 #include "engine.hpp"
 
 struct irt_engine {
@@ -231,6 +232,62 @@ int irt_codec_decode_noalloc(irt_codec* c, const float* latent, int32_t batch, i
     need(latent, "latent");
     need(wav, "wav");
     irt::codec_decode_noalloc(*c->c, latent, batch, frames, wav, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int irt_cross_attention(const irt_attn_args* a, const irt_rows* k, const irt_rows* v, int64_t k_rows, void* stream) {
+  return guard([&] {
+    need(a, "args");
+    need(k, "k");
+    need(v, "v");
+    const irt::CtxAttnParams p = irt::ctx_attn_params(*a, nullptr, k, v, k_rows, nullptr, nullptr);
+    irt::DeviceGuard dg(a->device);
+    irt::ctx_attention(p, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int irt_kv4_attention(const irt_attn_args* a, const irt_kv4_cache* cache, const irt_rows* k_self,
+                      const irt_rows* v_self, void* stream) {
+  return guard([&] {
+    need(a, "args");
+    need(cache, "cache");
+    const irt::CtxAttnParams p = irt::ctx_attn_params(*a, cache, nullptr, nullptr, cache->rows, k_self, v_self);
+    irt::DeviceGuard dg(a->device);
+    irt::ctx_attention(p, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int irt_kv4_append(int device, int dtype, const irt_kv4_cache* cache, int64_t row_start, int64_t n, const irt_rows* k,
+                   const irt_rows* v, int64_t src_rows, const int32_t* src_index, void* stream) {
+  return guard([&] {
+    need(cache, "cache");
+    need(k, "k");
+    need(v, "v");
+    irt::kv4_check_rows(*cache, dtype, row_start, n, *k, *v, src_rows, false);
+    if (!src_index && n > src_rows)
+      throw irt::shape_error("n " + std::to_string(n) + " exceeds the source's " + std::to_string(src_rows) + " rows");
+    irt::DeviceGuard dg(device);
+    irt::kv4_append(*cache, dtype == IRT_PREC_BF16, row_start, n, *k, *v, src_rows, src_index,
+                    reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int irt_kv4_read(int device, int dtype, const irt_kv4_cache* cache, int64_t row_start, int64_t n, const irt_rows* k,
+                 const irt_rows* v, void* stream) {
+  return guard([&] {
+    need(cache, "cache");
+    need(k, "k");
+    need(v, "v");
+    irt::kv4_check_rows(*cache, dtype, row_start, n, *k, *v, n, true);
+    irt::DeviceGuard dg(device);
+    irt::kv4_read(*cache, dtype == IRT_PREC_BF16, row_start, n, *k, *v, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+
+int irt_attention_check(int device) {
+  return guard([&] {
+    irt::DeviceGuard dg(device);
+    IRT_CUDA(cudaDeviceSynchronize());
   });
 }
 

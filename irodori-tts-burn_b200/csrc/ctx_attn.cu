@@ -1,0 +1,420 @@
+// Attention over context states: argument checks, choice of kernel, and the
+// row kernel that handles every type, head dimension, stride and alignment.
+//
+//   out_i = gate_i * sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i.k_j - m_i)
+//
+// over a sequence's own rows (if given) and its allowed context rows, native
+// or 4-bit.  One pass over the keys with a running maximum and sum; keys are
+// split over lanes, warps and the CTAs of a cluster, whose partial
+// (maximum, sum, output) triples are merged in a fixed order: results do not
+// depend on timing, and no workspace is needed.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "ctx_attn.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace irt {
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+constexpr int ROW_WARPS = 8;
+
+struct RowArgs {
+  CtxAttnParams p;
+  int lanes;  // lanes that share a key: a power of two >= head_dim / 8
+  int split;  // CTAs of a cluster over the keys of one row block
+  int q_vec, k_vec, v_vec, ks_vec, vs_vec;
+};
+
+// R packed query rows (query x grouped head) of one KV head per CTA.  A key is
+// held by `lanes` lanes, eight values each; a warp works on 32 / lanes keys at
+// a time, U of them in flight per lane group, each group with its own running
+// maximum.
+template <bool BF, bool CTX4, int R, int U>
+__global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __grid_constant__ RowArgs a) {
+  const CtxAttnParams& p = a.p;
+  irt_attn_seq sd;
+  if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
+  const int split = a.split, rank = blockIdx.x % split;
+  const int hk = blockIdx.y, G = p.G, hd = p.hd;
+  const int row0 = (blockIdx.x / split) * R;
+  if (row0 >= sd.q_len * G) return;  // the whole cluster
+  extern __shared__ float sm[];
+  // [warp][R][hd] partial outputs, [warp][R] maxima and sums; then the CTA's own
+  float* part = sm;
+  float* pm = part + ROW_WARPS * R * hd;
+  float* pl = pm + ROW_WARPS * R;
+  float* cpart = pl + ROW_WARPS * R;
+  float* cm = cpart + R * hd;
+  float* cl = cm + R;
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int LK = a.lanes, sub = lane / LK, o = lane % LK, per = 32 / LK;
+  const bool on = 8 * o < hd;
+  const float qscale = p.scale * LOG2E;
+  float q[R][8], acc[R][8], m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int pr = row0 + r;
+    const bool ok = on && pr < sd.q_len * G;
+    if (ok)
+      load8<BF>(p.q.data, (sd.q_start + pr / G) * p.q.row_stride + (hk * G + pr % G) * p.q.head_stride + 8 * o, a.q_vec,
+                q[r]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (!ok) q[r][j] = 0.f;
+      acc[r][j] = 0.f;
+    }
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+  }
+  const int n_self = p.ks.data ? sd.q_len : 0;
+  const int nk = n_self + sd.k_len;
+  const int chunk = per * U;
+  for (int c0 = (rank * ROW_WARPS + warp) * chunk; c0 < nk; c0 += split * ROW_WARPS * chunk) {
+    float k[U][8], v[U][8];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = c0 + u * per + sub;
+      const long row = j < n_self ? (long)sd.q_start + j : (long)sd.k_start + (j - n_self);
+      ok[u] = j < nk && (j < n_self || !p.mask || p.mask[row]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) k[u][i] = v[u][i] = 0.f;
+      if (ok[u] && on) {
+        if (j < n_self) {
+          load8<BF>(p.ks.data, row * p.ks.row_stride + hk * p.ks.head_stride + 8 * o, a.ks_vec, k[u]);
+          load8<BF>(p.vs.data, row * p.vs.row_stride + hk * p.vs.head_stride + 8 * o, a.vs_vec, v[u]);
+        } else if (CTX4) {
+          const long cr = (long)hk * p.k_rows + row;
+          const int g = kv4_groups(hd);
+          kv4_unpack8(*reinterpret_cast<const uint32_t*>(p.kc + cr * (hd / 2) + 4 * o),
+                      __bfloat162float(p.kscale[cr * g + o / 4]), k[u]);
+          kv4_unpack8(*reinterpret_cast<const uint32_t*>(p.vc + cr * (hd / 2) + 4 * o),
+                      __bfloat162float(p.vscale[cr * g + o / 4]), v[u]);
+        } else {
+          load8<BF>(p.k.data, row * p.k.row_stride + hk * p.k.head_stride + 8 * o, a.k_vec, k[u]);
+          load8<BF>(p.v.data, row * p.v.row_stride + hk * p.v.head_stride + 8 * o, a.v_vec, v[u]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float s[U];
+      float mx = m[r];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d = fmaf(q[r][i], k[u][i], d);
+        for (int w = LK / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+        s[u] = ok[u] ? d * qscale : -INFINITY;
+        mx = fmaxf(mx, s[u]);
+      }
+      const float base = mx == -INFINITY ? 0.f : mx;  // NaN scores stay NaN in p and the sum
+      const float corr = exp2f(m[r] - base);
+      m[r] = mx;
+      l[r] *= corr;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[r][i] *= corr;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e = exp2f(s[u] - base);
+        l[r] += e;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(e, v[u][i], acc[r][i]);
+      }
+    }
+  }
+
+  // lane groups of the warp
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float mw = m[r];
+    for (int w = LK; w < 32; w <<= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, w));
+    const float f = exp2f(m[r] - (mw == -INFINITY ? 0.f : mw));
+    float lw = l[r] * f;
+    for (int w = LK; w < 32; w <<= 1) lw += __shfl_xor_sync(0xffffffffu, lw, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x = acc[r][i] * f;
+      for (int w = LK; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+      if (sub == 0 && on) part[(warp * R + r) * hd + 8 * o + i] = x;
+    }
+    if (lane == 0) {
+      pm[warp * R + r] = mw;
+      pl[warp * R + r] = lw;
+    }
+  }
+  __syncthreads();
+  // warps of the CTA
+  for (int e = threadIdx.x; e < R * hd; e += 32 * ROW_WARPS) {
+    const int r = e / hd, d = e % hd;
+    float mc = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < ROW_WARPS; ++w) mc = fmaxf(mc, pm[w * R + r]);
+    const float base = mc == -INFINITY ? 0.f : mc;
+    float lc = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < ROW_WARPS; ++w) {
+      const float f = exp2f(pm[w * R + r] - base);
+      lc = fmaf(pl[w * R + r], f, lc);
+      x = fmaf(part[(w * R + r) * hd + d], f, x);
+    }
+    cpart[e] = x;
+    if (d == 0) {
+      cm[r] = mc;
+      cl[r] = lc;
+    }
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (split > 1) cluster.sync();
+  else __syncthreads();
+  // CTAs of the cluster: each finishes a share of the block's values
+  for (int e = rank * 32 * ROW_WARPS + threadIdx.x; e < R * hd; e += split * 32 * ROW_WARPS) {
+    const int r = e / hd, d = e % hd, pr = row0 + r;
+    if (pr >= sd.q_len * G) continue;
+    float mt = -INFINITY;
+    for (int c = 0; c < split; ++c) mt = fmaxf(mt, split > 1 ? cluster.map_shared_rank(cm, c)[r] : cm[r]);
+    const float base = mt == -INFINITY ? 0.f : mt;
+    float lt = 0.f, x = 0.f;
+    for (int c = 0; c < split; ++c) {
+      const float* om = split > 1 ? cluster.map_shared_rank(cm, c) : cm;
+      const float* ol = split > 1 ? cluster.map_shared_rank(cl, c) : cl;
+      const float* op = split > 1 ? cluster.map_shared_rank(cpart, c) : cpart;
+      const float f = exp2f(om[r] - base);
+      lt = fmaf(ol[r], f, lt);
+      x = fmaf(op[e], f, x);
+    }
+    x *= lt == 0.f ? 0.f : 1.f / lt;
+    const long row = sd.q_start + pr / G;
+    const int head = hk * G + pr % G;
+    if (p.gate.data) {
+      const long off = row * p.gate.row_stride + head * p.gate.head_stride + d;
+      x *= BF ? __bfloat162float(static_cast<const bf16*>(p.gate.data)[off]) : static_cast<const float*>(p.gate.data)[off];
+    }
+    const long off = row * p.out.row_stride + head * p.out.head_stride + d;
+    if (BF) static_cast<bf16*>(p.out.data)[off] = __float2bfloat16_rn(x);
+    else static_cast<float*>(p.out.data)[off] = x;
+    if (p.lse && d == 0) p.lse[row * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
+  }
+  if (split > 1) cluster.sync();  // the others may still read this CTA's part
+}
+
+int device_sms() {
+  int dev = 0, n = 0;
+  IRT_CUDA(cudaGetDevice(&dev));
+  IRT_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  return n;
+}
+
+template <bool BF, bool CTX4, int R, int U>
+void launch_rows(const CtxAttnParams& p, cudaStream_t s) {
+  RowArgs a{};
+  a.p = p;
+  a.lanes = 1;
+  while (a.lanes < p.hd / 8) a.lanes *= 2;
+  a.q_vec = rows_vec(p.q, BF);
+  a.k_vec = rows_vec(p.k, BF);
+  a.v_vec = rows_vec(p.v, BF);
+  a.ks_vec = rows_vec(p.ks, BF);
+  a.vs_vec = rows_vec(p.vs, BF);
+  const long blocks = ((long)p.max_q * p.G + R - 1) / R;
+  const long ctas = blocks * p.Hkv * p.nseq;
+  const long keys = (long)p.max_k + (p.ks.data ? p.max_q : 0);
+  // Keys are split over a cluster while there are fewer than two CTAs per SM
+  // and every CTA keeps at least two chunks per warp.
+  const int sms = device_sms();
+  const long least = 2L * ROW_WARPS * U * (32 / a.lanes);
+  a.split = 1;
+  while (a.split < 8 && ctas * a.split * 2 <= 2L * sms && keys >= 2L * a.split * least) a.split *= 2;
+  const size_t smem = ((size_t)(ROW_WARPS + 1) * R * p.hd + 2 * (ROW_WARPS + 1) * R) * sizeof(float);
+  auto kernel = ctx_attn_rows_kernel<BF, CTX4, R, U>;  // smem <= 37.2 KB (R = 4, head_dim 256)
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
+  cfg.blockDim = dim3(32 * ROW_WARPS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)a.split, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IRT_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  IRT_CHECK_LAUNCH();
+}
+
+template <bool BF>
+void rows_path(const CtxAttnParams& p, cudaStream_t s) {
+  const bool one = (long)p.max_q * p.G == 1;
+  if (p.kc) {
+    if (one) launch_rows<BF, true, 1, 4>(p, s);
+    else launch_rows<BF, true, 4, 2>(p, s);
+  } else {
+    if (one) launch_rows<BF, false, 1, 4>(p, s);
+    else launch_rows<BF, false, 4, 2>(p, s);
+  }
+}
+
+// ---- argument checks -------------------------------------------------------
+
+// Rows of a tensor: a sequence's own and context rows together stay below 2^31.
+constexpr long MAX_ROWS = (1L << 30) - 1;
+
+Error arg_error(const std::string& m) { return Error(IRT_E_INVALID_ARG, m); }
+
+// First and one-past-last byte of a tensor of rows (strides are not negative).
+struct Span {
+  uintptr_t lo, hi;
+};
+Span span_of(const irt_rows& r, long rows, int heads, int hd, int esz) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(r.data);
+  if (!r.data || rows <= 0) return {lo, lo};
+  return {lo, lo + (uintptr_t)((rows - 1) * r.row_stride + (heads - 1) * r.head_stride + hd) * esz};
+}
+bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+void check_rows(const char* name, const irt_rows& r, long rows, int heads, int esz) {
+  if (!r.data && rows > 0) throw arg_error(std::string(name) + " is NULL");
+  if (reinterpret_cast<uintptr_t>(r.data) % esz) throw arg_error(std::string(name) + " is not aligned to its type");
+  if (r.row_stride < 0 || r.head_stride < 0) throw shape_error(std::string(name) + " has a negative stride");
+  // a tensor of more than 2^48 elements is a mistake, and keeps 64-bit offsets from overflowing
+  const long lim = 1L << 48;
+  if (r.row_stride > lim || r.head_stride > lim || (rows > 0 && r.row_stride > lim / rows) ||
+      (heads > 0 && r.head_stride > lim / heads))
+    throw shape_error(std::string(name) + " has a stride beyond 2^48 elements");
+}
+
+// A tensor that is written must not overlap itself.
+void check_own(const char* name, const irt_rows& r, long rows, int heads, int hd) {
+  const bool row_major = (heads == 1 || r.head_stride >= hd) &&
+                         (rows <= 1 || r.row_stride >= (heads - 1) * r.head_stride + hd);
+  const bool head_major = (rows <= 1 || r.row_stride >= hd) &&
+                          (heads == 1 || r.head_stride >= (rows - 1) * r.row_stride + hd);
+  if (!row_major && !head_major) throw shape_error(std::string(name) + "'s rows overlap one another");
+}
+
+void check_heads(int heads, int kv_heads, int hd) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    throw shape_error("heads " + std::to_string(heads) + " must be a positive multiple of kv_heads " +
+                      std::to_string(kv_heads));
+  if (kv_heads > 65535) throw shape_error("at most 65535 KV heads");
+  if (hd < 8 || hd > 256 || hd % 8)
+    throw shape_error("head_dim " + std::to_string(hd) + " must be a multiple of 8 in 8..256");
+}
+
+}  // namespace
+
+void kv4_check_cache(const irt_kv4_cache& c) {
+  check_heads(c.kv_heads, c.kv_heads, c.head_dim);
+  if (c.rows < 0 || c.rows > MAX_ROWS) throw shape_error("cache rows " + std::to_string(c.rows) + " out of range");
+  const void* const ps[4] = {c.k_codes, c.k_scales, c.v_codes, c.v_scales};
+  for (const void* q : ps) {
+    if (!q && c.rows > 0) throw arg_error("a cache buffer is NULL");
+    if (reinterpret_cast<uintptr_t>(q) & 15) throw arg_error("cache buffers must be aligned to 16 bytes");
+  }
+}
+
+void kv4_check_rows(const irt_kv4_cache& c, int dtype, long row_start, long n, const irt_rows& k, const irt_rows& v,
+                    long ext_rows, bool written) {
+  if (dtype != IRT_PREC_BF16 && dtype != IRT_PREC_F32) throw arg_error("dtype must be an irt_precision");
+  kv4_check_cache(c);
+  if (row_start < 0 || n < 0 || row_start > c.rows || n > c.rows - row_start)
+    throw shape_error("rows [" + std::to_string(row_start) + ", " + std::to_string(row_start) + " + " +
+                      std::to_string(n) + ") are outside the cache's " + std::to_string(c.rows));
+  if (ext_rows < 0 || ext_rows > MAX_ROWS) throw shape_error("source rows must be in 0..2^30 - 1");
+  const int esz = dtype == IRT_PREC_BF16 ? 2 : 4;
+  check_rows("k", k, ext_rows, c.kv_heads, esz);
+  check_rows("v", v, ext_rows, c.kv_heads, esz);
+  if (written) {
+    check_own("k", k, ext_rows, c.kv_heads, c.head_dim);
+    check_own("v", v, ext_rows, c.kv_heads, c.head_dim);
+  }
+}
+
+CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache, const irt_rows* k,
+                              const irt_rows* v, long k_rows, const irt_rows* k_self, const irt_rows* v_self) {
+  if (a.dtype != IRT_PREC_BF16 && a.dtype != IRT_PREC_F32) throw arg_error("dtype must be an irt_precision");
+  check_heads(a.heads, a.kv_heads, a.head_dim);
+  if (a.num_seqs < 0 || a.num_seqs > 65535) throw shape_error("num_seqs must be in 0..65535");
+  if (a.max_q_len < 0 || a.max_k_len < 0) throw shape_error("max_q_len and max_k_len must not be negative");
+  if (a.q_rows < 0 || k_rows < 0 || a.q_rows > MAX_ROWS || k_rows > MAX_ROWS)
+    throw shape_error("q_rows and the context rows must be in 0..2^30 - 1");
+  if ((long)a.max_q_len * (a.heads / a.kv_heads) > (1L << 26)) throw shape_error("max_q_len is too large");
+  if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) throw arg_error("scale must be finite");
+  if (!a.seqs && ((long)a.num_seqs * a.max_q_len > a.q_rows || (long)a.num_seqs * a.max_k_len > k_rows))
+    throw shape_error("without a sequence table q needs num_seqs * max_q_len rows and the context num_seqs * max_k_len");
+  const bool bf = a.dtype == IRT_PREC_BF16;
+  const int esz = bf ? 2 : 4;
+  CtxAttnParams p{};
+  p.bf16_io = bf;
+  p.H = a.heads;
+  p.Hkv = a.kv_heads;
+  p.hd = a.head_dim;
+  p.G = a.heads / a.kv_heads;
+  p.nseq = a.num_seqs;
+  p.max_q = a.max_q_len;
+  p.max_k = a.max_k_len;
+  p.scale = a.scale;
+  p.q_rows = a.q_rows;
+  p.k_rows = k_rows;
+  p.seqs = a.seqs;
+  p.q = a.q;
+  p.gate = a.gate;
+  p.out = a.out;
+  p.mask = a.key_mask;
+  p.lse = a.lse;
+  check_rows("q", a.q, a.q_rows, a.heads, esz);
+  check_rows("out", a.out, a.q_rows, a.heads, esz);
+  check_own("out", a.out, a.q_rows, a.heads, a.head_dim);
+  if (a.gate.data) check_rows("gate", a.gate, a.q_rows, a.heads, esz);
+  const Span so = span_of(a.out, a.q_rows, a.heads, a.head_dim, esz);
+  auto apart = [&](const char* name, const irt_rows& r, long rows, int heads) {
+    if (overlap(so, span_of(r, rows, heads, a.head_dim, esz))) throw arg_error("out overlaps " + std::string(name));
+  };
+  apart("q", a.q, a.q_rows, a.heads);
+  apart("gate", a.gate, a.q_rows, a.heads);
+  if (cache) {
+    kv4_check_cache(*cache);
+    if (cache->kv_heads != a.kv_heads || cache->head_dim != a.head_dim)
+      throw shape_error("the cache holds " + std::to_string(cache->kv_heads) + " heads of " +
+                        std::to_string(cache->head_dim) + ", the call has " + std::to_string(a.kv_heads) + " of " +
+                        std::to_string(a.head_dim));
+    p.kc = cache->k_codes;
+    p.vc = cache->v_codes;
+    p.kscale = reinterpret_cast<const bf16*>(cache->k_scales);
+    p.vscale = reinterpret_cast<const bf16*>(cache->v_scales);
+  } else {
+    check_rows("k", *k, k_rows, a.kv_heads, esz);
+    check_rows("v", *v, k_rows, a.kv_heads, esz);
+    apart("k", *k, k_rows, a.kv_heads);
+    apart("v", *v, k_rows, a.kv_heads);
+    p.k = *k;
+    p.v = *v;
+  }
+  const bool s0 = k_self && k_self->data, s1 = v_self && v_self->data;
+  if (s0 != s1) throw missing_input("k_self and v_self go together");
+  if (s0) {
+    check_rows("k_self", *k_self, a.q_rows, a.kv_heads, esz);
+    check_rows("v_self", *v_self, a.q_rows, a.kv_heads, esz);
+    apart("k_self", *k_self, a.q_rows, a.kv_heads);
+    apart("v_self", *v_self, a.q_rows, a.kv_heads);
+    p.ks = *k_self;
+    p.vs = *v_self;
+  }
+  return p;
+}
+
+void ctx_attention(const CtxAttnParams& p, cudaStream_t s) {
+  if (p.nseq == 0 || p.max_q == 0 || p.q_rows == 0) return;
+  if (p.bf16_io) rows_path<true>(p, s);
+  else rows_path<false>(p, s);
+}
+
+}  // namespace irt

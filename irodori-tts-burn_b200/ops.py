@@ -1,0 +1,326 @@
+"""Attention over context states as operators on torch CUDA tensors: cross
+attention to an encoder's states, and the context cache held in 4 bits.
+
+The engine's joint attention (src/model/attention.rs:403-418, :619-664) reads
+its latent frames and its text / speaker rows in one pass; these calls offer
+the same attention to programs that keep queries and context rows themselves.
+
+    table = attention_table(q_lens, k_lens, device=0)           # once per batch
+    out = cross_attention(q, k, v, table, max(q_lens), max(k_lens))
+
+    cache = Kv4Cache(rows, kv_heads=16, head_dim=128, device=0)  # 4.5 bits a value
+    kv4_append(cache, k, v)
+    out = kv4_attention(q, cache, table, max(q_lens), max(k_lens), k_self=ks, v_self=vs)
+
+Unlike ``InferenceEngine.sample`` the calls queue their work and return: with
+``stream=None`` on torch's current stream of the tensors' GPU (whichever GPU is
+current), so they order like torch's own operators and can be captured into a
+CUDA graph.  They are forward only; a tensor that requires a gradient is
+refused while gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+from . import IrodoriError, PREC, _check, lib
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class _AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("device", ctypes.c_int32), ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("num_seqs", ctypes.c_int32), ("max_q_len", ctypes.c_int32),
+        ("max_k_len", ctypes.c_int32), ("scale", ctypes.c_float), ("q_rows", ctypes.c_int64),
+        ("seqs", ctypes.c_void_p), ("q", _Rows), ("gate", _Rows), ("out", _Rows), ("key_mask", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p)]
+
+
+SIGNATURES = {
+    "irt_cross_attention": (ctypes.c_int, [ctypes.POINTER(_AttnArgs), ctypes.POINTER(_Rows), ctypes.POINTER(_Rows),
+                                           ctypes.c_int64, ctypes.c_void_p]),
+    "irt_kv4_append": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.POINTER(_Cache), ctypes.c_int64,
+                                      ctypes.c_int64, ctypes.POINTER(_Rows), ctypes.POINTER(_Rows), ctypes.c_int64,
+                                      ctypes.c_void_p, ctypes.c_void_p]),
+    "irt_kv4_read": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.POINTER(_Cache), ctypes.c_int64, ctypes.c_int64,
+                                    ctypes.POINTER(_Rows), ctypes.POINTER(_Rows), ctypes.c_void_p]),
+    "irt_kv4_attention": (ctypes.c_int, [ctypes.POINTER(_AttnArgs), ctypes.POINTER(_Cache), ctypes.POINTER(_Rows),
+                                         ctypes.POINTER(_Rows), ctypes.c_void_p]),
+    "irt_attention_check": (ctypes.c_int, [ctypes.c_int]),
+}
+
+GROUP = 32  # values that share a scale in the 4-bit cache
+
+_torch = None
+_dtype_code = None
+
+
+def _t():
+    """torch, imported at the first call (the package itself does not need it)."""
+    global _torch, _dtype_code
+    if _torch is None:
+        import torch
+        _torch = torch
+        _dtype_code = {torch.bfloat16: PREC["bf16"], torch.float32: PREC["f32"]}
+    return _torch
+
+
+def _heads(name, t, device, dtype, shape):
+    """Rows of heads of a [rows, heads, head_dim] tensor (any strides, the last one 1)."""
+    if t.dtype is not dtype:
+        raise IrodoriError(9, f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
+    if t.device != device:
+        raise IrodoriError(22, f"{name} must be on {device}, got {t.device}")
+    if t.requires_grad and _torch.is_grad_enabled():
+        raise IrodoriError(4, f"Unsupported mode: {name} requires a gradient; the operators are forward only "
+                              "(call them under torch.no_grad())")
+    st = t.stride()
+    if st[2] != 1 and shape[2] != 1 and t.numel():
+        raise IrodoriError(22, f"{name}: the values of a head must be contiguous")
+    return _Rows(t.data_ptr(), st[0], st[1])
+
+
+def _first(name, t):
+    torch = _t()
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise IrodoriError(22, f"{name} must be a torch CUDA tensor")
+    if t.dim() != 3:
+        raise IrodoriError(2, f"Shape mismatch: {name} must be [rows, heads, head_dim], got {list(t.shape)}")
+    if t.dtype not in _dtype_code:
+        raise IrodoriError(9, f"{name} must be bfloat16 or float32, got {t.dtype}")
+    return torch
+
+
+def _plain(name, t, device, dtypes, shape):
+    """A contiguous helper tensor (table, mask, index, cache buffer)."""
+    if not isinstance(t, _torch.Tensor) or t.device != device:
+        raise IrodoriError(22, f"{name} must be a tensor on {device}")
+    if t.dtype not in dtypes:
+        raise IrodoriError(9, f"{name} must be {dtypes[0]}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
+    if not t.is_contiguous():
+        raise IrodoriError(22, f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+class _Queue:
+    """The stream of one call.  Without an explicit stream: torch's current one on the tensors' GPU."""
+
+    def __init__(self, stream, device):
+        self.torch_stream = None
+        if stream is None:
+            self.handle = _torch.cuda.current_stream(device).cuda_stream
+        else:
+            self.torch_stream = (_torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int)
+                                 else stream)
+            self.handle = self.torch_stream.cuda_stream
+
+    def empty(self, shape, dtype, device):
+        if self.torch_stream is None:
+            return _torch.empty(shape, dtype=dtype, device=device)
+        with _torch.cuda.stream(self.torch_stream):
+            return _torch.empty(shape, dtype=dtype, device=device)
+
+    def uses(self, *tensors):
+        """Keeps the allocator from handing out these tensors' memory before an explicit stream is done with them."""
+        if self.torch_stream is not None:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(self.torch_stream)
+
+
+def attention_table(q_lens, k_lens, k_starts=None, device=0):
+    """The sequence table of ``cross_attention`` / ``kv4_attention``: int32
+    [n, 4] rows (q_start, q_len, k_start, k_len) on the GPU.  Queries are
+    packed in order; context rows too, unless ``k_starts`` places them (ranges
+    may overlap)."""
+    torch = _t()
+    q_lens, k_lens = [int(x) for x in q_lens], [int(x) for x in k_lens]
+    if len(q_lens) != len(k_lens) or (k_starts is not None and len(k_starts) != len(k_lens)):
+        raise IrodoriError(2, "Shape mismatch: q_lens, k_lens and k_starts must have one entry per sequence")
+    if any(x < 0 for x in q_lens + k_lens):
+        raise IrodoriError(2, "Shape mismatch: lengths must not be negative")
+    rows, q, k = [], 0, 0
+    for i, (a, b) in enumerate(zip(q_lens, k_lens)):
+        rows.append([q, a, k if k_starts is None else int(k_starts[i]), b])
+        q, k = q + a, k + b
+    if not rows:
+        return torch.zeros((0, 4), dtype=torch.int32, device=torch.device("cuda", device))
+    return torch.tensor(rows, dtype=torch.int32, device=torch.device("cuda", device))
+
+
+class Kv4Cache:
+    """Context cache in 4 bits (``irt_kv4_cache``): K and V rows as codes of 4
+    bits with one bf16 scale per 32 values of a head's row.  Holds values of a
+    relative error of about 0.1 (normal data) in 0.28 of a bf16 cache's bytes;
+    every value it holds is a bf16 number.  Rows start as zeros."""
+
+    def __init__(self, rows: int, kv_heads: int, head_dim: int, device=0):
+        torch = _t()
+        dev = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if rows < 0 or kv_heads <= 0 or head_dim < 8 or head_dim > 256 or head_dim % 8:
+            raise IrodoriError(2, "Shape mismatch: a 4-bit cache has rows >= 0, kv_heads > 0 and a head_dim that is a "
+                                  f"multiple of 8 in 8..256, got {rows}, {kv_heads}, {head_dim}")
+        g = -(-head_dim // GROUP)
+        self._set(torch.zeros((kv_heads, rows, head_dim // 2), dtype=torch.uint8, device=dev),
+                  torch.zeros((kv_heads, rows, g), dtype=torch.bfloat16, device=dev),
+                  torch.zeros((kv_heads, rows, head_dim // 2), dtype=torch.uint8, device=dev),
+                  torch.zeros((kv_heads, rows, g), dtype=torch.bfloat16, device=dev))
+
+    @classmethod
+    def from_buffers(cls, k_codes, k_scales, v_codes, v_scales) -> "Kv4Cache":
+        """A cache over tensors of the caller: codes uint8 [kv_heads, rows,
+        head_dim / 2], scales bfloat16 [kv_heads, rows, ceil(head_dim / 32)]."""
+        self = cls.__new__(cls)
+        self._set(k_codes, k_scales, v_codes, v_scales)
+        return self
+
+    def _set(self, k_codes, k_scales, v_codes, v_scales):
+        torch = _t()
+        if not isinstance(k_codes, torch.Tensor) or not k_codes.is_cuda or k_codes.dim() != 3:
+            raise IrodoriError(22, "k_codes must be a CUDA tensor [kv_heads, rows, head_dim / 2]")
+        h, n, half = k_codes.shape
+        shape, scale_shape, dev = (h, n, half), (h, n, -(-2 * half // GROUP)), k_codes.device
+        u8, b16 = (torch.uint8,), (torch.bfloat16,)
+        self.buffers = (k_codes, k_scales, v_codes, v_scales)
+        self.rows, self.kv_heads, self.head_dim, self.device = n, h, 2 * half, dev
+        self._c = _Cache(n, h, 2 * half, _plain("k_codes", k_codes, dev, u8, shape),
+                         _plain("k_scales", k_scales, dev, b16, scale_shape),
+                         _plain("v_codes", v_codes, dev, u8, shape),
+                         _plain("v_scales", v_scales, dev, b16, scale_shape))
+
+
+def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=None) -> None:
+    """Writes rows of ``k``, ``v`` [rows, kv_heads, head_dim] into ``cache``
+    from ``row_start`` on (``irt_kv4_append``): all of them, or rows
+    ``src_rows`` (int32 tensor; an index outside the source leaves its cache
+    row as it was)."""
+    torch = _first("k", k)
+    n_src = k.shape[0]
+    shape = (n_src, cache.kv_heads, cache.head_dim)
+    kr = _heads("k", k, cache.device, k.dtype, shape)
+    vr = _heads("v", v, cache.device, k.dtype, shape)
+    n, idx = n_src, None
+    if src_rows is not None:
+        n = src_rows.shape[0] if isinstance(src_rows, torch.Tensor) and src_rows.dim() == 1 else -1
+        idx = _plain("src_rows", src_rows, cache.device, (torch.int32,), (n,))
+    q = _Queue(stream, cache.device)
+    _check(lib().irt_kv4_append(cache.device.index, _dtype_code[k.dtype], ctypes.byref(cache._c), row_start, n,
+                                ctypes.byref(kr), ctypes.byref(vr), n_src, idx, q.handle))
+    q.uses(k, v, src_rows, *cache.buffers)
+
+
+def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=None):
+    """The values that cache rows [row_start, row_start + rows) hold, as
+    (k, v) [rows, kv_heads, head_dim] of ``dtype`` (bfloat16, the default, or
+    float32; exact in both)."""
+    torch = _t()
+    dtype = torch.bfloat16 if dtype is None else dtype
+    if dtype not in _dtype_code:
+        raise IrodoriError(9, f"dtype must be bfloat16 or float32, got {dtype}")
+    n = cache.rows - row_start if rows is None else rows
+    if n < 0:
+        raise IrodoriError(2, f"Shape mismatch: {n} rows from {row_start} of a cache of {cache.rows}")
+    q = _Queue(stream, cache.device)
+    shape = (n, cache.kv_heads, cache.head_dim)
+    k, v = q.empty(shape, dtype, cache.device), q.empty(shape, dtype, cache.device)
+    kr, vr = (_Rows(t.data_ptr(), t.stride(0), t.stride(1)) for t in (k, v))
+    _check(lib().irt_kv4_read(cache.device.index, _dtype_code[dtype], ctypes.byref(cache._c), row_start, n,
+                              ctypes.byref(kr), ctypes.byref(vr), q.handle))
+    q.uses(*cache.buffers)
+    return k, v
+
+
+def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, gate, scale, out, return_lse, stream,
+               context, keep):
+    torch = _torch
+    n, h, d = shape = q.shape
+    dev, dtype = q.device, q.dtype
+    st = _Queue(stream, dev)
+    if out is None:
+        out = st.empty(shape, dtype, dev)
+    lse = st.empty((n, h), torch.float32, dev) if return_lse else None
+    if seqs is None:
+        nseq, tab = (n // max_q_len if max_q_len > 0 else 0), None
+        if nseq * max_q_len != n or nseq * max_k_len != k_rows:
+            raise IrodoriError(2, f"Shape mismatch: without a table {n} query rows and {k_rows} context rows must be "
+                                  f"the same number of sequences of {max_q_len} and {max_k_len}")
+    else:
+        nseq = seqs.shape[0] if isinstance(seqs, torch.Tensor) and seqs.dim() == 2 else -1
+        tab = _plain("seqs", seqs, dev, (torch.int32,), (nseq, 4))
+    mask = None
+    if key_mask is not None:
+        mask = _plain("key_mask", key_mask, dev, (torch.uint8, torch.bool), (k_rows,))
+    a = _AttnArgs(dev.index, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
+                  1.0 / math.sqrt(d) if scale is None else scale, n, tab, _heads("q", q, dev, dtype, shape),
+                  _Rows() if gate is None else _heads("gate", gate, dev, dtype, shape),
+                  _heads("out", out, dev, dtype, shape), mask, None if lse is None else lse.data_ptr())
+    _check(call(ctypes.byref(a), *context, st.handle))
+    st.uses(q, seqs, key_mask, gate, out, *keep)
+    return (out, lse) if return_lse else out
+
+
+def cross_attention(q, k, v, seqs, max_q_len: int, max_k_len: int, key_mask=None, gate=None, scale=None, out=None,
+                    return_lse: bool = False, stream=None):
+    """Attention of packed queries ``q`` [q_rows, heads, head_dim] to an
+    encoder's states ``k``, ``v`` [k_rows, kv_heads, head_dim]
+    (``irt_cross_attention``); bfloat16 or float32, any row and head strides.
+
+    ``seqs`` is an ``attention_table`` (or None: equal sequences of
+    ``max_q_len`` query and ``max_k_len`` context rows, in order); ``max_q_len``
+    and ``max_k_len`` bound its lengths.  Query head h reads KV head
+    h // (heads // kv_heads).  ``key_mask`` uint8 / bool [k_rows]: non-zero =
+    attend.  ``gate``, shaped like ``q``, is multiplied into the output.
+    ``scale`` defaults to 1 / sqrt(head_dim).
+
+    Returns [q_rows, heads, head_dim], with ``return_lse`` also the float32
+    [q_rows, heads] log of the softmax's sum.  A query without any key gives 0
+    and -inf; rows that no sequence covers (and sequences that reach outside
+    the tensors or the bounds) are left as they were: pass ``out`` where that
+    matters."""
+    _first("q", q)
+    _first("k", k)
+    n = k.shape[0]
+    shape = (n, k.shape[1], q.shape[2])
+    kr = _heads("k", k, q.device, q.dtype, shape)
+    vr = _heads("v", v, q.device, q.dtype, shape)
+    return _attention(lib().irt_cross_attention, q, shape[1], n, seqs, max_q_len, max_k_len, key_mask, gate, scale,
+                      out, return_lse, stream, (ctypes.byref(kr), ctypes.byref(vr), n), (k, v))
+
+
+def kv4_attention(q, cache: Kv4Cache, seqs, max_q_len: int, max_k_len: int, k_self=None, v_self=None, key_mask=None,
+                  gate=None, scale=None, out=None, return_lse: bool = False, stream=None):
+    """Attention of packed queries over a 4-bit context cache
+    (``irt_kv4_attention``).  With ``k_self``, ``v_self`` [q_rows, kv_heads,
+    head_dim] a sequence's queries attend to the rows of their own range too,
+    as in the model's joint attention.  The other arguments and the result are
+    those of ``cross_attention``, the cache's rows in the place of ``k``, ``v``."""
+    _first("q", q)
+    if cache.device != q.device:
+        raise IrodoriError(22, f"the cache must be on {q.device}, got {cache.device}")
+    shape = (q.shape[0], cache.kv_heads, q.shape[2])
+    kr = None if k_self is None else ctypes.byref(_heads("k_self", k_self, q.device, q.dtype, shape))
+    vr = None if v_self is None else ctypes.byref(_heads("v_self", v_self, q.device, q.dtype, shape))
+    return _attention(lib().irt_kv4_attention, q, cache.kv_heads, cache.rows, seqs, max_q_len, max_k_len, key_mask,
+                      gate, scale, out, return_lse, stream, (ctypes.byref(cache._c), kr, vr),
+                      (k_self, v_self, *cache.buffers))
+
+
+def attention_check(device: int = 0) -> None:
+    """Waits for the GPU and raises if a bounded wait inside an attention
+    operator's kernel has expired since the last check."""
+    _check(lib().irt_attention_check(device))
