@@ -288,6 +288,8 @@ int irt_attention_check(int device) {
   return guard([&] {
     irt::DeviceGuard dg(device);
     IRT_CUDA(cudaDeviceSynchronize());
+    if (irt::read_and_clear_ctx_attn_error())
+      throw irt::Error(IRT_E_CUDA, "a bounded wait inside an attention operator expired: its outputs are invalid");
   });
 }
 

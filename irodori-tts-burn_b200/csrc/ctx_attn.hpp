@@ -47,6 +47,12 @@ __device__ __forceinline__ bool ctx_attn_seq(const CtxAttnParams& p, int n, irt_
 // Queues the attention on s (checks of arguments are done by the caller).
 void ctx_attention(const CtxAttnParams& p, cudaStream_t s);
 
+// The same on tcgen05 (ctx_attn_tc.cu): bf16, head_dim <= 128, 16-byte rows.
+// Returns false, with nothing queued, where the call is outside what it handles.
+bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s);
+// Bounded-wait flag of its kernels on the current device (0 = ok).
+int read_and_clear_ctx_attn_error();
+
 // cache rows [row_start, row_start + n) from source rows idx[i] (or i); see
 // irt_kv4_append / irt_kv4_read.
 void kv4_append(const irt_kv4_cache& c, int bf16_io, long row_start, long n, const irt_rows& k, const irt_rows& v,

@@ -1,0 +1,628 @@
+// Attention over context states on tcgen05 (bf16, head_dim <= 128).
+//
+// One CTA = one (sequence, head group, tile of 128 packed query rows); with
+// grouped heads the rows of a tile are query x head of the group (row r =
+// query r / Gp, head r % Gp), so the group's K and V are read once.  Two CTAs
+// share an SM.  Key tiles of 64: a sequence's own rows first, then its context
+// rows.  Warps:
+//   0..3  softmax: thread = query row.  Per tile: scores from TMEM, masked
+//         keys to -inf, P = exp2(s - m) as packed bf16 over the first half of
+//         the score buffer (the A operand of P V).  m is raised, and O rescaled,
+//         only when a row's maximum grows by more than 2^8.  Warps without a
+//         query row take no part.
+//   4     TMA: Q once, K and V of native tiles (2-stage rings, K two tiles
+//         ahead of V).
+//   5     tcgen05.mma issue: S_j = Q K_j^T, O += P_j V_j.
+//   6, 7  (4-bit context) codes -> bf16 K and V tiles in the same swizzled
+//         layout.  A value c s has at most 8 significant bits, so the bf16 tile
+//         is exact and the products are those of the cache's values.
+// Keys that do not count (past the sequence, masked) must not meet the P V
+// product even with weight 0, since 0 * NaN is NaN: their V rows are zeroed in
+// shared memory before the product (native tiles: by the softmax warps, only
+// in tiles that have such keys).
+//
+// Few query tiles: the key tiles of one query tile are shared by a cluster of
+// 2, 4 or 8 CTAs, which merge their (m, l, O) through distributed shared
+// memory in rank order.  No workspace, no atomics.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "ctx_attn.cuh"
+#include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace irt {
+
+namespace {
+
+using namespace tcx;
+
+constexpr int QT = 128, KT = 64, NKV = 2;
+constexpr float RESCALE_LOG2 = 8.f;
+constexpr float LN2 = 0.6931471805599453f;
+
+template <int HDT, bool CTX4>
+struct Cfg {
+  static constexpr int THREADS = CTX4 ? 256 : 192;
+  static constexpr uint32_t Q_HALF = QT * 128, Q_BYTES = Q_HALF * (HDT / 64);  // 64-column halves
+  static constexpr uint32_t HALF = KT * 128, TILE = HALF * (HDT / 64);
+  static constexpr uint32_t OFF_K = Q_BYTES, OFF_V = OFF_K + NKV * TILE, OFF_BAR = OFF_V + NKV * TILE;
+  static constexpr size_t SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t IDESC_S = idesc_bf16(128, KT, false), IDESC_O = idesc_bf16(128, HDT, true);
+  static constexpr uint32_t TM_S = 0, TM_O = 2 * KT, TM_COLS = 256;
+  // arrivals that fill a K or V stage: the TMA thread and both code warps
+  static constexpr uint32_t FULL_COUNT = CTX4 ? 3 : 1;
+  // cluster merge: f32 O rows (padded against bank conflicts), m and l
+  static constexpr int OLD = HDT + 4;
+  static_assert((uint32_t)QT * OLD * 4 + 2 * QT * 4 <= OFF_BAR, "merge buffers fit the tiles");
+};
+
+struct TcArgs {
+  CtxAttnParams p;
+  float scale_log2;
+  int Gp;     // heads packed into a query tile
+  int split;  // CTAs of the cluster
+};
+
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc));
+}
+
+// Box of a (d, head, row) tensor.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Eight codes -> eight bf16 values c s, in order.  (128 + code) is a bf16
+// number with the code in its low mantissa bits; minus 136 and times s are
+// exact.
+__device__ __forceinline__ uint4 kv4_bf16x8(uint32_t w, __nv_bfloat162 s2) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6 / 1 3 5 7
+  const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);  // 0 1 2 3 / 4 5 6 7
+  uint32_t r[4] = {__byte_perm(a, 0x43434343u, 0x4140), __byte_perm(a, 0x43434343u, 0x4342),
+                   __byte_perm(b, 0x43434343u, 0x4140), __byte_perm(b, 0x43434343u, 0x4342)};
+  const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __nv_bfloat162 v = *reinterpret_cast<__nv_bfloat162*>(&r[i]);
+    v = __hmul2(__hsub2(v, off), s2);
+    r[i] = *reinterpret_cast<uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void st_shared8_zero(uint32_t addr) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(addr), "r"(0) : "memory");
+}
+
+template <int HDT, bool CTX4>
+__global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
+    ctx_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKS,
+                       const __grid_constant__ CUtensorMap tmVS, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcArgs a) {
+  using C = Cfg<HDT, CTX4>;
+  pdl_wait();
+  pdl_trigger();
+  const CtxAttnParams& p = a.p;
+  irt_attn_seq sd;
+  if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
+  const int split = a.split, rank = blockIdx.x % split, Gp = a.Gp;
+  const int q0 = (blockIdx.x / split) * (QT / Gp);  // first query of the tile
+  if (q0 >= sd.q_len) return;                       // the whole cluster
+  const int head0 = blockIdx.y * Gp, hk = head0 / p.G;
+  const int rows = min(QT, (sd.q_len - q0) * Gp);  // packed query rows of the tile
+  const int n_self = p.ks.data ? (sd.q_len + KT - 1) / KT : 0;
+  const int n_all = n_self + (sd.k_len + KT - 1) / KT;
+  const int t0 = (int)((long)n_all * rank / split), nt = (int)((long)n_all * (rank + 1) / split) - t0;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::OFF_BAR);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  const uint32_t Q_FULL = bar(0), O_DONE = bar(1), O_FINAL = bar(2);
+  auto K_FULL = [&](int s) { return bar(3 + s); };
+  auto K_EMPTY = [&](int s) { return bar(3 + NKV + s); };
+  auto V_FULL = [&](int s) { return bar(3 + 2 * NKV + s); };
+  auto V_EMPTY = [&](int s) { return bar(3 + 3 * NKV + s); };
+  auto S_FULL = [&](int b) { return bar(3 + 4 * NKV + b); };
+  auto P_FULL = [&](int b) { return bar(5 + 4 * NKV + b); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7 + 4 * NKV);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int sm_warps = (rows + 31) / 32;  // softmax warps that have a query row
+  if (threadIdx.x == 0) {
+    mbar_init(Q_FULL, 1);
+    mbar_init(O_DONE, 1);
+    mbar_init(O_FINAL, 1);
+    for (int r = 0; r < NKV; ++r) {
+      mbar_init(K_FULL(r), C::FULL_COUNT);
+      mbar_init(K_EMPTY(r), 1);
+      mbar_init(V_FULL(r), C::FULL_COUNT);
+      mbar_init(V_EMPTY(r), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(S_FULL(b), 1);
+      mbar_init(P_FULL(b), sm_warps);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 5) tmem_alloc(smem_u32(tmem_slot), C::TM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t sQ = smem_u32(sm);
+  auto sK = [&](int s) { return smem_u32(sm + C::OFF_K + s * C::TILE); };
+  auto sV = [&](int s) { return smem_u32(sm + C::OFF_V + s * C::TILE); };
+  // first row and valid keys of local tile j
+  auto row_of = [&](int j) {
+    const int t = t0 + j;
+    return t < n_self ? sd.q_start + t * KT : sd.k_start + (t - n_self) * KT;
+  };
+  auto keys_of = [&](int j) {
+    const int t = t0 + j;
+    return min(KT, t < n_self ? sd.q_len - t * KT : sd.k_len - (t - n_self) * KT);
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  if (nt > 0) {
+    if (warp == 4) {
+      // ---------------- TMA ----------------
+      if (lane == 0) {
+        mbar_expect_tx(Q_FULL, C::Q_BYTES);
+#pragma unroll
+        for (int h = 0; h < HDT / 64; ++h) tma_load_3d(sQ + h * C::Q_HALF, &tmQ, Q_FULL, 64 * h, head0, sd.q_start + q0);
+        auto load = [&](int j, uint32_t full, uint32_t empty, uint32_t dst, const CUtensorMap* self, const CUtensorMap* ctx) {
+          mbar_wait(empty, ((j / NKV) & 1) ^ 1);
+          const bool own = t0 + j < n_self;
+          if (CTX4 && !own) {  // the code warps fill this one
+            mbar_arrive(full);
+            return;
+          }
+          mbar_expect_tx(full, C::TILE);
+          const CUtensorMap* m = own ? self : ctx;
+#pragma unroll
+          for (int h = 0; h < HDT / 64; ++h) tma_load_3d(dst + h * C::HALF, m, full, 64 * h, hk, row_of(j));
+        };
+        auto load_k = [&](int j) { load(j, K_FULL(j % NKV), K_EMPTY(j % NKV), sK(j % NKV), &tmKS, &tmK); };
+        auto load_v = [&](int j) { load(j, V_FULL(j % NKV), V_EMPTY(j % NKV), sV(j % NKV), &tmVS, &tmV); };
+        load_k(0);
+        if (nt > 1) load_k(1);
+        for (int j = 0; j < nt; ++j) {
+          load_v(j);
+          if (j + 2 < nt) load_k(j + 2);
+        }
+      }
+    } else if (warp == 5) {
+      // ---------------- MMA ----------------
+      if (lane == 0) {
+        mbar_wait(Q_FULL, 0);
+        tc_fence_after();
+        auto issue_s = [&](int j) {
+          const int r = j % NKV, b = j & 1;
+          mbar_wait(K_FULL(r), (j / NKV) & 1);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < HDT / 16; ++kk) {
+            const uint64_t da = sdesc_kmajor(sQ + (kk >> 2) * C::Q_HALF + (kk & 3) * 32);
+            const uint64_t db = sdesc_kmajor(sK(r) + (kk >> 2) * C::HALF + (kk & 3) * 32);
+            umma_f16(tmem + C::TM_S + b * KT, da, db, C::IDESC_S, kk != 0);
+          }
+          umma_commit(S_FULL(b));
+          umma_commit(K_EMPTY(r));
+        };
+        issue_s(0);
+        if (nt > 1) issue_s(1);
+        for (int j = 0; j < nt; ++j) {
+          const int s = j & 1, r = j % NKV;
+          mbar_wait(V_FULL(r), (j / NKV) & 1);
+          mbar_wait(P_FULL(s), (j >> 1) & 1);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk) {
+            const uint64_t db = sdesc_sw128(sV(r) + kk * 16 * 128, C::HALF, 1024);
+            umma_ts(tmem + C::TM_O, tmem + C::TM_S + s * KT + kk * 8, db, C::IDESC_O, (j | kk) != 0);
+          }
+          umma_commit(V_EMPTY(r));
+          umma_commit(O_DONE);
+          if (j + 2 < nt) issue_s(j + 2);  // overwrites S_j / P_j after P_j V_j in the tensor pipe's order
+        }
+        umma_commit(O_FINAL);
+      }
+    } else if (CTX4 && warp >= 6) {
+      // ---------------- codes -> bf16 tiles ----------------
+      // warp 6: the lower half of the head dimension, warp 7: the upper; a
+      // lane has keys lane and lane + 32, so the eight 16-byte chunks that a
+      // quarter warp stores fall on different banks under the swizzle.
+      constexpr int W = HDT / 16;      // words of eight codes per key and warp
+      constexpr int NG = HDT / 64;     // groups of 32 per key and warp
+      const int part = warp - 6, hd = p.hd, groups = kv4_groups(hd);
+      const bool wide = hd % KV4_GROUP == 0;  // 16-byte aligned groups of codes
+      struct Codes {
+        uint32_t w[2][W];
+        uint16_t s[2][NG];
+        bool ok[2];
+      };
+      // operation i: K0 K1 V0 K2 V1 K3 ... V(nt-1), the order of the TMA warp
+      auto op_of = [&](int i, bool& is_v, int& j) {
+        if (nt == 1) {
+          is_v = i == 1;
+          j = 0;
+        } else if (i < 2) {
+          is_v = false;
+          j = i;
+        } else {
+          const int u = i - 2;  // V0 K2 V1 K3 ... then V(nt-2) V(nt-1)
+          is_v = (u & 1) == 0 || u >= 2 * (nt - 2);
+          j = u >= 2 * (nt - 2) ? nt - 2 + (u - 2 * (nt - 2)) : (u & 1) ? u / 2 + 2 : u / 2;
+        }
+      };
+      auto fetch = [&](int i, Codes& c) {
+        bool is_v;
+        int j;
+        op_of(i, is_v, j);
+        if (t0 + j < n_self) return;
+        const uint8_t* base = is_v ? p.vc : p.kc;
+        const bf16* sc = is_v ? p.vscale : p.kscale;
+        const int nkeys = keys_of(j);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = lane + 32 * e;
+          const long row = (long)row_of(j) + key;
+          c.ok[e] = key < nkeys && (!p.mask || p.mask[row]);
+          const long cr = (long)hk * p.k_rows + row;
+#pragma unroll
+          for (int i4 = 0; i4 < W; i4 += 4) {
+            const int o = part * W + i4;
+            if (wide) {
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (c.ok[e] && 8 * o < hd) v = *reinterpret_cast<const uint4*>(base + cr * (hd / 2) + 4 * o);
+              c.w[e][i4] = v.x; c.w[e][i4 + 1] = v.y; c.w[e][i4 + 2] = v.z; c.w[e][i4 + 3] = v.w;
+            } else {
+#pragma unroll
+              for (int i1 = 0; i1 < 4; ++i1)
+                c.w[e][i4 + i1] = c.ok[e] && 8 * (o + i1) < hd
+                                      ? *reinterpret_cast<const uint32_t*>(base + cr * (hd / 2) + 4 * (o + i1))
+                                      : 0x88888888u;
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const int gi = part * NG + g;
+            c.s[e][g] = c.ok[e] && gi < groups ? reinterpret_cast<const uint16_t*>(sc)[cr * groups + gi] : 0;
+          }
+        }
+      };
+      auto put = [&](int i, const Codes& c) {
+        bool is_v;
+        int j;
+        op_of(i, is_v, j);
+        const int r = j % NKV;
+        const uint32_t full = is_v ? V_FULL(r) : K_FULL(r), empty = is_v ? V_EMPTY(r) : K_EMPTY(r);
+        mbar_wait(empty, ((j / NKV) & 1) ^ 1);
+        if (t0 + j >= n_self) {
+          const uint32_t dst = is_v ? sV(r) : sK(r);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int key = lane + 32 * e;
+#pragma unroll
+            for (int o = 0; o < W; ++o) {
+              const uint16_t sb = c.s[e][o / 4];
+              const uint32_t s2 = (uint32_t)sb << 16 | sb;
+              const uint4 v = kv4_bf16x8(c.w[e][o], *reinterpret_cast<const __nv_bfloat162*>(&s2));
+              const int chunk = part * W + o;  // 16-byte chunk of the row
+              st_shared16(dst + (chunk >> 3) * C::HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), v);
+            }
+          }
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
+      };
+      Codes c0, c1;
+      const int ops = 2 * nt;
+      fetch(0, c0);
+      for (int i = 0; i < ops; i += 2) {  // an even number of operations
+        fetch(i + 1, c1);
+        put(i, c0);
+        if (i + 2 < ops) fetch(i + 2, c0);
+        put(i + 1, c1);
+      }
+    } else if (warp < sm_warps) {
+      // ---------------- softmax ----------------
+      const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+      for (int j = 0; j < nt; ++j) {
+        const int b = j & 1;
+        const bool own = t0 + j < n_self;
+        const int nkeys = keys_of(j);
+        // bit i: key i counts
+        uint32_t on0 = nkeys >= 32 ? 0xffffffffu : (1u << nkeys) - 1;
+        uint32_t on1 = nkeys >= 64 ? 0xffffffffu : nkeys > 32 ? (1u << (nkeys - 32)) - 1 : 0u;
+        if (p.mask && !own) {
+          const uint8_t* mk = p.mask + row_of(j);
+          on0 &= __ballot_sync(0xffffffffu, lane < nkeys && mk[lane]);
+          on1 &= __ballot_sync(0xffffffffu, lane + 32 < nkeys && mk[lane + 32]);
+        }
+        const bool partial = (on0 & on1) != 0xffffffffu;
+        mbar_wait(S_FULL(b), (j >> 1) & 1);
+        tc_fence_after();
+        uint32_t sr[KT];
+#pragma unroll
+        for (int g = 0; g < KT / 32; ++g)
+          tmem_ld32(tmem + lane_off + C::TM_S + b * KT + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * g]));
+        tmem_wait_ld();
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+            if (!((i < 32 ? on0 >> i : on1 >> (i - 32)) & 1)) sr[i] = __float_as_uint(-INFINITY);
+          if (!CTX4 || own) {  // V rows that do not count: zeros
+            mbar_wait(V_FULL(j % NKV), (j / NKV) & 1);
+            for (int key = warp; key < KT; key += sm_warps)
+              if (!((key < 32 ? on0 >> key : on1 >> (key - 32)) & 1)) {
+                if (HDT == 128) st_shared8_zero(sV(j % NKV) + (lane >> 4) * C::HALF + key * 128 + (lane & 15) * 8);
+                else if (lane < 16) st_shared8_zero(sV(j % NKV) + key * 128 + lane * 8);
+              }
+            fence_proxy_async();
+          }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < KT; i += 4) {
+          mx0 = fmaxf(mx0, __uint_as_float(sr[i]));
+          mx1 = fmaxf(mx1, __uint_as_float(sr[i + 1]));
+          mx2 = fmaxf(mx2, __uint_as_float(sr[i + 2]));
+          mx3 = fmaxf(mx3, __uint_as_float(sr[i + 3]));
+        }
+        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2;
+        float corr = 1.f;
+        const bool raise = mx > m_run + RESCALE_LOG2 || (m_run == -INFINITY && mx > -INFINITY);
+        if (raise) {
+          corr = m_run == -INFINITY ? 0.f : ex2(m_run - mx);
+          m_run = mx;
+        }
+        const float nbase = m_run == -INFINITY ? 0.f : -m_run;
+        // P_{j-1} V_{j-1} must be done before O is read; the phase in flight
+        // is j - 1 or already j
+        if (__any_sync(0xffffffffu, raise) && j > 0) {
+          mbar_wait(O_DONE, (j - 1) & 1);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < HDT / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(tmem + lane_off + C::TM_O + c * 32, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+            tmem_st32(tmem + lane_off + C::TM_O + c * 32, r);
+          }
+        }
+        uint32_t pk[KT / 2];
+        const uint64_t sc2 = f2_pack(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
+        const uint64_t nb2 = f2_pack(__float_as_uint(nbase), __float_as_uint(nbase));
+        uint64_t rs2 = 0;
+#pragma unroll
+        for (int c = 0; c < KT / 2; ++c) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(sr[2 * c], sr[2 * c + 1]), sc2, nb2), x0, x1);
+          const float p0 = ex2(x0), p1 = ex2(x1);
+          rs2 = f2_add(rs2, f2_pack(__float_as_uint(p0), __float_as_uint(p1)));
+          pk[c] = pack_bf16x2(p0, p1);
+        }
+        float rs0, rs1;
+        f2_unpack(rs2, rs0, rs1);
+        tmem_st32(tmem + lane_off + C::TM_S + b * KT, pk);
+        tmem_wait_st();
+        l_run = l_run * corr + (rs0 + rs1);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(P_FULL(b));
+      }
+      mbar_wait(O_FINAL, 0);
+      tc_fence_after();
+    }
+  }
+
+  // ---------------- output ----------------
+  const int qrow = warp * 32 + lane;
+  if (split == 1) {
+    if (warp < sm_warps) {
+      const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+      const bool ok = qrow < rows;
+      const long row = (long)sd.q_start + q0 + qrow / Gp;
+      const int head = head0 + qrow % Gp;
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      bf16* out = static_cast<bf16*>(p.out.data) + (ok ? row * p.out.row_stride + head * p.out.head_stride : 0);
+      const bf16* gate = p.gate.data && ok
+                             ? static_cast<const bf16*>(p.gate.data) + row * p.gate.row_stride + head * p.gate.head_stride
+                             : nullptr;
+#pragma unroll 1
+      for (int c = 0; c < HDT / 32; ++c) {
+        uint4 gv[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (gate && c * 32 + u * 8 < p.hd) gv[u] = *reinterpret_cast<const uint4*>(gate + c * 32 + u * 8);
+        uint32_t r[32];
+        if (nt > 0) {
+          tmem_ld32(tmem + lane_off + C::TM_O + c * 32, r);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (!ok || c * 32 + u * 8 >= p.hd) continue;
+          const __nv_bfloat162* gp = reinterpret_cast<const __nv_bfloat162*>(&gv[u]);
+          uint32_t op[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float g0 = gate ? __bfloat162float(gp[k].x) : 1.f, g1 = gate ? __bfloat162float(gp[k].y) : 1.f;
+            op[k] = pack_bf16x2(__uint_as_float(r[u * 8 + 2 * k]) * inv * g0,
+                                __uint_as_float(r[u * 8 + 2 * k + 1]) * inv * g1);
+          }
+          *reinterpret_cast<uint4*>(out + c * 32 + u * 8) = make_uint4(op[0], op[1], op[2], op[3]);
+        }
+      }
+      if (ok && p.lse)
+        p.lse[row * p.H + head] = l_run == 0.f ? -INFINITY : fmaf(m_run, LN2, logf(l_run));
+    }
+  } else {
+    // this CTA's O, m and l over its tiles (all products are done, so nothing
+    // else uses the shared memory)
+    float* so = reinterpret_cast<float*>(sm);
+    float* sml = so + QT * C::OLD;  // m, then l
+    if (warp < sm_warps) {
+      const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+      sml[qrow] = m_run;
+      sml[QT + qrow] = l_run;
+#pragma unroll 1
+      for (int c = 0; c < HDT / 32; ++c) {
+        uint32_t r[32];
+        if (nt > 0) {
+          tmem_ld32(tmem + lane_off + C::TM_O + c * 32, r);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<uint4*>(so + qrow * C::OLD + c * 32 + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+      }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    __syncwarp();
+    cluster.sync();
+    const int per_row = p.hd / 4;
+    for (int e = threadIdx.x; e < ((rows - rank + split - 1) / split) * per_row; e += C::THREADS) {
+      const int r = (e / per_row) * split + rank, d = (e % per_row) * 4;  // rows dealt out to the CTAs
+      float mt = -INFINITY;
+      for (int c = 0; c < split; ++c) mt = fmaxf(mt, cluster.map_shared_rank(sml, c)[r]);
+      const float base = mt == -INFINITY ? 0.f : mt;
+      float lt = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < split; ++c) {
+        const float* om = cluster.map_shared_rank(sml, c);
+        const float f = ex2(om[r] - base);
+        const float4 o = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, c) + r * C::OLD + d);
+        lt = fmaf(om[QT + r], f, lt);
+        x.x = fmaf(o.x, f, x.x);
+        x.y = fmaf(o.y, f, x.y);
+        x.z = fmaf(o.z, f, x.z);
+        x.w = fmaf(o.w, f, x.w);
+      }
+      const float inv = lt == 0.f ? 0.f : 1.f / lt;
+      x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+      const long row = (long)sd.q_start + q0 + r / Gp;
+      const int head = head0 + r % Gp;
+      if (p.gate.data) {
+        const uint2 g = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(p.gate.data) +
+                                                        row * p.gate.row_stride + head * p.gate.head_stride + d);
+        x.x *= __uint_as_float(g.x << 16);
+        x.y *= __uint_as_float(g.x & 0xffff0000u);
+        x.z *= __uint_as_float(g.y << 16);
+        x.w *= __uint_as_float(g.y & 0xffff0000u);
+      }
+      *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out.data) + row * p.out.row_stride + head * p.out.head_stride +
+                                d) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
+      if (p.lse && d == 0) p.lse[row * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
+    }
+    __syncwarp();
+    cluster.sync();  // the others may still read this CTA's part
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TM_COLS);
+  }
+}
+
+// (d, head, row) map with boxes of 64 values x `heads` x `rows`; false when
+// the strides cannot be encoded.
+bool rows_map(CUtensorMap& m, const irt_rows& r, long rows, int heads, int hd, int box_heads, int box_rows) {
+  const cuuint64_t dim[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t stride[2] = {(cuuint64_t)r.head_stride * 2, (cuuint64_t)r.row_stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return tma_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, r.data, dim, stride, box, step,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HDT, bool CTX4>
+bool launch(const CtxAttnParams& p, cudaStream_t s) {
+  using C = Cfg<HDT, CTX4>;
+  TcArgs a{};
+  a.p = p;
+  a.scale_log2 = p.scale * 1.4426950408889634f;
+  a.Gp = QT % p.G == 0 ? p.G : 1;
+  CUtensorMap q, ks, vs, k, v;
+  if (!rows_map(q, p.q, p.q_rows, p.H, p.hd, a.Gp, QT / a.Gp)) return false;
+  ks = vs = k = v = q;
+  if (p.ks.data && (!rows_map(ks, p.ks, p.q_rows, p.Hkv, p.hd, 1, KT) ||
+                    !rows_map(vs, p.vs, p.q_rows, p.Hkv, p.hd, 1, KT)))
+    return false;
+  if (p.k.data && p.k_rows > 0 &&
+      (!rows_map(k, p.k, p.k_rows, p.Hkv, p.hd, 1, KT) || !rows_map(v, p.v, p.k_rows, p.Hkv, p.hd, 1, KT)))
+    return false;
+  int dev = 0, sms = 0;
+  IRT_CUDA(cudaGetDevice(&dev));
+  IRT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const long qtiles = ((long)p.max_q * a.Gp + QT - 1) / QT;
+  const long ctas = qtiles * (p.H / a.Gp) * p.nseq;
+  const long ktiles = (p.max_k + KT - 1L) / KT + (p.ks.data ? (p.max_q + KT - 1L) / KT : 0);
+  // Key tiles are shared by a cluster while half the CTA slots (two per SM)
+  // would stay empty.
+  a.split = 1;
+  while (a.split < 8 && ctas * a.split * 2 <= 2L * sms && a.split * 2 <= ktiles) a.split *= 2;
+  auto kernel = ctx_attn_tc_kernel<HDT, CTX4>;
+  IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(qtiles * a.split), p.H / a.Gp, p.nseq);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)a.split, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  IRT_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, ks, vs, k, v, a));
+  IRT_CHECK_LAUNCH();
+  return true;
+}
+
+}  // namespace
+
+bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s) {
+  // The row maximum is taken before the scale, so the scale must be positive;
+  // tensors must be readable and writable 16 bytes at a time.
+  if (!p.bf16_io || p.hd > 128 || !(p.scale > 0.f) || p.H / (QT % p.G == 0 ? p.G : 1) > 65535) return false;
+  const irt_rows* const rows[7] = {&p.q, &p.out, &p.gate, &p.k, &p.v, &p.ks, &p.vs};
+  for (const irt_rows* r : rows)
+    if (r->data && !rows_vec(*r, 1)) return false;
+  if (p.kc) return p.hd > 64 ? launch<128, true>(p, s) : launch<64, true>(p, s);
+  return p.hd > 64 ? launch<128, false>(p, s) : launch<64, false>(p, s);
+}
+
+int read_and_clear_ctx_attn_error() { return read_and_clear_flag(); }
+
+}  // namespace irt

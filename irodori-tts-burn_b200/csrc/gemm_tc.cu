@@ -858,6 +858,8 @@ CUtensorMap tma_map_tile32_phased(const void* p, bool f32, long q_rows, long col
   return m;
 }
 
+TmaEncodeFn tma_encode_fn() { return tc::get_encode(); }
+
 // bf16 2-D tensor map with a {64, box_rows} box and 128-byte swizzle (cached).
 const CUtensorMap& tma_map_bf16(const void* p, long rows, long cols, long ld, int box_rows) {
   return tc::tensor_map(p, rows, cols, ld, box_rows);

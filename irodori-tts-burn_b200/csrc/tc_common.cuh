@@ -9,6 +9,13 @@
 #include <cstdint>
 
 namespace irt {
+
+// cuTensorMapEncodeTiled, looked up once through the runtime (gemm_tc.cu).
+using TmaEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TmaEncodeFn tma_encode_fn();
+
 namespace tcx {
 
 // Watchdog flag of this translation unit (each .cu that includes this header
