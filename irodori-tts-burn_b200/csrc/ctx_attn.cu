@@ -8,20 +8,15 @@
 // split over lanes, warps and the CTAs of a cluster, whose partial
 // (maximum, sum, output) triples are merged in a fixed order: results do not
 // depend on timing, and no workspace is needed.
-#include <cooperative_groups.h>
-
 #include <algorithm>
 
 #include "ctx_attn.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace irt {
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 
 constexpr int ROW_WARPS = 8;
 
@@ -152,59 +147,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
       pl[warp * R + r] = lw;
     }
   }
-  __syncthreads();
-  // warps of the CTA
-  for (int e = threadIdx.x; e < R * hd; e += 32 * ROW_WARPS) {
-    const int r = e / hd, d = e % hd;
-    float mc = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < ROW_WARPS; ++w) mc = fmaxf(mc, pm[w * R + r]);
-    const float base = mc == -INFINITY ? 0.f : mc;
-    float lc = 0.f, x = 0.f;
-#pragma unroll
-    for (int w = 0; w < ROW_WARPS; ++w) {
-      const float f = exp2f(pm[w * R + r] - base);
-      lc = fmaf(pl[w * R + r], f, lc);
-      x = fmaf(part[(w * R + r) * hd + d], f, x);
-    }
-    cpart[e] = x;
-    if (d == 0) {
-      cm[r] = mc;
-      cl[r] = lc;
-    }
-  }
-  cg::cluster_group cluster = cg::this_cluster();
-  if (split > 1) cluster.sync();
-  else __syncthreads();
-  // CTAs of the cluster: each finishes a share of the block's values
-  for (int e = rank * 32 * ROW_WARPS + threadIdx.x; e < R * hd; e += split * 32 * ROW_WARPS) {
-    const int r = e / hd, d = e % hd, pr = row0 + r;
-    if (pr >= sd.q_len * G) continue;
-    float mt = -INFINITY;
-    for (int c = 0; c < split; ++c) mt = fmaxf(mt, split > 1 ? cluster.map_shared_rank(cm, c)[r] : cm[r]);
-    const float base = mt == -INFINITY ? 0.f : mt;
-    float lt = 0.f, x = 0.f;
-    for (int c = 0; c < split; ++c) {
-      const float* om = split > 1 ? cluster.map_shared_rank(cm, c) : cm;
-      const float* ol = split > 1 ? cluster.map_shared_rank(cl, c) : cl;
-      const float* op = split > 1 ? cluster.map_shared_rank(cpart, c) : cpart;
-      const float f = exp2f(om[r] - base);
-      lt = fmaf(ol[r], f, lt);
-      x = fmaf(op[e], f, x);
-    }
-    x *= lt == 0.f ? 0.f : 1.f / lt;
-    const long row = sd.q_start + pr / G;
-    const int head = hk * G + pr % G;
-    if (p.gate.data) {
-      const long off = row * p.gate.row_stride + head * p.gate.head_stride + d;
-      x *= BF ? __bfloat162float(static_cast<const bf16*>(p.gate.data)[off]) : static_cast<const float*>(p.gate.data)[off];
-    }
-    const long off = row * p.out.row_stride + head * p.out.head_stride + d;
-    if (BF) static_cast<bf16*>(p.out.data)[off] = __float2bfloat16_rn(x);
-    else static_cast<float*>(p.out.data)[off] = x;
-    if (p.lse && d == 0) p.lse[row * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
-  }
-  if (split > 1) cluster.sync();  // the others may still read this CTA's part
+  merge_partials<BF, R, ROW_WARPS>(p, sd, split, rank, hk, row0, part, pm, pl, cpart, cm, cl);
 }
 
 int device_sms() {
@@ -413,7 +356,7 @@ CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache
 
 void ctx_attention(const CtxAttnParams& p, cudaStream_t s) {
   if (p.nseq == 0 || p.max_q == 0 || p.q_rows == 0) return;
-  if (ctx_attention_tc(p, s)) return;
+  if (ctx_attention_kv4_rows(p, s) || ctx_attention_tc(p, s)) return;
   if (p.bf16_io) rows_path<true>(p, s);
   else rows_path<false>(p, s);
 }

@@ -50,7 +50,9 @@ void ctx_attention(const CtxAttnParams& p, cudaStream_t s);
 // The same on tcgen05 (ctx_attn_tc.cu): bf16, head_dim <= 128, 16-byte rows.
 // Returns false, with nothing queued, where the call is outside what it handles.
 bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s);
-// Bounded-wait flag of its kernels on the current device (0 = ok).
+// Few query rows over a 4-bit cache (ctx_attn_kv4.cu); false as above.
+bool ctx_attention_kv4_rows(const CtxAttnParams& p, cudaStream_t s);
+// Bounded-wait flag of the tcgen05 kernels on the current device (0 = ok).
 int read_and_clear_ctx_attn_error();
 
 // cache rows [row_start, row_start + n) from source rows idx[i] (or i); see
