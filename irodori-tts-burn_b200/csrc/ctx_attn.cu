@@ -24,7 +24,7 @@ struct RowArgs {
   CtxAttnParams p;
   int lanes;  // lanes that share a key: a power of two >= head_dim / 8
   int split;  // CTAs of a cluster over the keys of one row block
-  int q_vec, k_vec, v_vec, ks_vec, vs_vec;
+  int q_vec, k_vec, v_vec, ks_vec, vs_vec, out_vec;
 };
 
 // R packed query rows (query x grouped head) of one KV head per CTA.  A key is
@@ -40,14 +40,11 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
   const int hk = blockIdx.y, G = p.G, hd = p.hd;
   const int row0 = (blockIdx.x / split) * R;
   if (row0 >= sd.q_len * G) return;  // the whole cluster
-  extern __shared__ float sm[];
-  // [warp][R][hd] partial outputs, [warp][R] maxima and sums; then the CTA's own
+  extern __shared__ __align__(16) float sm[];
+  // states of the warps, see merge_partials
   float* part = sm;
-  float* pm = part + ROW_WARPS * R * hd;
+  float* pm = part + (ROW_WARPS + 1) * R * hd;
   float* pl = pm + ROW_WARPS * R;
-  float* cpart = pl + ROW_WARPS * R;
-  float* cm = cpart + R * hd;
-  float* cl = cm + R;
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int LK = a.lanes, sub = lane / LK, o = lane % LK, per = 32 / LK;
@@ -147,7 +144,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
       pl[warp * R + r] = lw;
     }
   }
-  merge_partials<BF, R, ROW_WARPS>(p, sd, split, rank, hk, row0, part, pm, pl, cpart, cm, cl);
+  merge_partials<BF, R, ROW_WARPS>(p, sd, split, rank, hk, row0, sm, a.out_vec);
 }
 
 int device_sms() {
@@ -168,6 +165,7 @@ void launch_rows(const CtxAttnParams& p, cudaStream_t s) {
   a.v_vec = rows_vec(p.v, BF);
   a.ks_vec = rows_vec(p.ks, BF);
   a.vs_vec = rows_vec(p.vs, BF);
+  a.out_vec = rows_vec(p.out, BF) && (!p.gate.data || rows_vec(p.gate, BF));
   const long blocks = ((long)p.max_q * p.G + R - 1) / R;
   const long ctas = blocks * p.Hkv * p.nseq;
   const long keys = (long)p.max_k + (p.ks.data ? p.max_q : 0);
@@ -176,9 +174,9 @@ void launch_rows(const CtxAttnParams& p, cudaStream_t s) {
   const int sms = device_sms();
   const long least = 2L * ROW_WARPS * U * (32 / a.lanes);
   a.split = 1;
-  while (a.split < 8 && ctas * a.split * 2 <= 2L * sms && keys >= 2L * a.split * least) a.split *= 2;
-  const size_t smem = ((size_t)(ROW_WARPS + 1) * R * p.hd + 2 * (ROW_WARPS + 1) * R) * sizeof(float);
-  auto kernel = ctx_attn_rows_kernel<BF, CTX4, R, U>;  // smem <= 37.2 KB (R = 4, head_dim 256)
+  while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 2L * sms && keys >= 2L * a.split * least) a.split *= 2;
+  const size_t smem = (size_t)merge_floats(R, ROW_WARPS, p.hd) * sizeof(float);
+  auto kernel = ctx_attn_rows_kernel<BF, CTX4, R, U>;  // smem <= 37.3 KB (R = 4, head_dim 256)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
   cfg.blockDim = dim3(32 * ROW_WARPS);

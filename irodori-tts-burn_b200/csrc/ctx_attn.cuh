@@ -78,70 +78,139 @@ __device__ __forceinline__ void kv4_unpack8(uint32_t w, float s, float (&x)[8]) 
   for (int j = 0; j < 8; ++j) x[j] = (float)((int)((w >> (4 * j)) & 15u) - 8) * s;
 }
 
-// Joins the partial softmax states of R packed query rows (from row0 on) that
-// W warps of each CTA of a cluster hold over their shares of the keys, in a
-// fixed order, and writes the rows: out = gate sum_w 2^(m_w - m) O_w /
-// sum_w 2^(m_w - m) l_w.  part [W][R][hd], pm (base-2 maxima) and pl (sums)
-// [W][R] are this CTA's; cpart [R][hd], cm and cl [R] hold its joined state for
-// the cluster.  Called by every thread of every CTA of the cluster, after the
-// CTA's warps have written their parts.
+// Four values of a row of the output (or gate).
+template <bool BF>
+__device__ __forceinline__ float4 load4(const void* base, long off, bool vec) {
+  if (BF) {
+    const bf16* p = static_cast<const bf16*>(base) + off;
+    if (vec) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p);
+      return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                         __uint_as_float(u.y & 0xffff0000u));
+    }
+    return make_float4(__bfloat162float(p[0]), __bfloat162float(p[1]), __bfloat162float(p[2]), __bfloat162float(p[3]));
+  }
+  const float* p = static_cast<const float*>(base) + off;
+  if (vec) return *reinterpret_cast<const float4*>(p);
+  return make_float4(p[0], p[1], p[2], p[3]);
+}
+template <bool BF>
+__device__ __forceinline__ void store4(void* base, long off, bool vec, float4 x) {
+  if (BF) {
+    bf16* p = static_cast<bf16*>(base) + off;
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+    if (vec) {
+      *reinterpret_cast<uint2*>(p) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      p[0] = a.x; p[1] = a.y; p[2] = b.x; p[3] = b.y;
+    }
+  } else {
+    float* p = static_cast<float*>(base) + off;
+    if (vec) {
+      *reinterpret_cast<float4*>(p) = x;
+    } else {
+      p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w;
+    }
+  }
+}
+
+constexpr int MAX_SPLIT = 8;  // CTAs of a cluster that share a query block's keys
+
+// Shared memory of merge_partials in floats: part [W][R][hd], the CTA's own
+// joined rows [R][hd], and maxima, sums and weights.
+constexpr __host__ __device__ int merge_floats(int R, int W, int hd) { return (W + 1) * R * hd + (3 * W + 2) * R; }
+
+// Joins the partial softmax states of the packed query rows [row0, row0 + R)
+// that W warps of each CTA of a cluster hold over their shares of the keys, in
+// a fixed order, and writes the rows:
+//   out = gate sum_w 2^(m_w - m) O_w / sum_w 2^(m_w - m) l_w.
+// sm: part [W][R][hd], then pm [W][R] (base-2 maxima) and pl [W][R] (sums),
+// written by the warps; the rest is used here.  16-byte aligned.  Called by
+// every thread of every CTA of the cluster.  vec: rows of out and gate can be
+// accessed four values at a time.
 template <bool BF, int R, int W>
 __device__ __forceinline__ void merge_partials(const CtxAttnParams& p, const irt_attn_seq& sd, int split, int rank,
-                                               int hk, int row0, const float* part, const float* pm, const float* pl,
-                                               float* cpart, float* cm, float* cl) {
+                                               int hk, int row0, float* sm, bool vec) {
   namespace cg = cooperative_groups;
   constexpr float LN2 = 0.6931471805599453f;
-  const int hd = p.hd, G = p.G;
+  const int hd = p.hd, G = p.G, rows = min(R, sd.q_len * G - row0), q4 = hd / 4;
+  float* cpart = sm + W * R * hd;  // joined rows; before them the parts, behind them the statistics
+  float* pm = cpart + R * hd;
+  float* pl = pm + W * R;
+  float* pf = pl + W * R;
+  float* cm = pf + W * R;
+  float* cl = cm + R;
   __syncthreads();
-  for (int e = threadIdx.x; e < R * hd; e += 32 * W) {
-    const int r = e / hd, d = e % hd;
+  for (int e = threadIdx.x; e < W * rows; e += 32 * W) {
+    const int r = e / W, w = e % W;
     float mc = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) mc = fmaxf(mc, pm[w * R + r]);
+    for (int i = 0; i < W; ++i) mc = fmaxf(mc, pm[i * R + r]);
     const float base = mc == -INFINITY ? 0.f : mc;
-    float lc = 0.f, x = 0.f;
+    pf[w * R + r] = exp2f(pm[w * R + r] - base);
+    if (w == 0) {
+      float lc = 0.f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float f = exp2f(pm[w * R + r] - base);
-      lc = fmaf(pl[w * R + r], f, lc);
-      x = fmaf(part[(w * R + r) * hd + d], f, x);
-    }
-    cpart[e] = x;
-    if (d == 0) {
+      for (int i = 0; i < W; ++i) lc = fmaf(pl[i * R + r], exp2f(pm[i * R + r] - base), lc);
       cm[r] = mc;
       cl[r] = lc;
     }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < rows * q4; e += 32 * W) {
+    const int r = e / q4, d = e % q4 * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = pf[w * R + r];
+      const float4 o = *reinterpret_cast<const float4*>(sm + (w * R + r) * hd + d);
+      x.x = fmaf(o.x, f, x.x);
+      x.y = fmaf(o.y, f, x.y);
+      x.z = fmaf(o.z, f, x.z);
+      x.w = fmaf(o.w, f, x.w);
+    }
+    *reinterpret_cast<float4*>(cpart + r * hd + d) = x;
   }
   cg::cluster_group cluster = cg::this_cluster();
   if (split > 1) cluster.sync();
   else __syncthreads();
   // each CTA finishes a share of the rows' values
-  for (int e = rank * 32 * W + threadIdx.x; e < R * hd; e += split * 32 * W) {
-    const int r = e / hd, d = e % hd, pr = row0 + r;
-    if (pr >= sd.q_len * G) continue;
+  for (int e = rank * 32 * W + threadIdx.x; e < rows * q4; e += split * 32 * W) {
+    const int r = e / q4, d = e % q4 * 4, pr = row0 + r;
+    float om[MAX_SPLIT], ol[MAX_SPLIT];
+    float4 o[MAX_SPLIT];
     float mt = -INFINITY;
-    for (int c = 0; c < split; ++c) mt = fmaxf(mt, split > 1 ? cluster.map_shared_rank(cm, c)[r] : cm[r]);
+#pragma unroll
+    for (int c = 0; c < MAX_SPLIT; ++c)
+      if (c < split) {
+        om[c] = split > 1 ? cluster.map_shared_rank(cm, c)[r] : cm[r];
+        ol[c] = split > 1 ? cluster.map_shared_rank(cl, c)[r] : cl[r];
+        o[c] = *reinterpret_cast<const float4*>((split > 1 ? cluster.map_shared_rank(cpart, c) : cpart) + r * hd + d);
+        mt = fmaxf(mt, om[c]);
+      }
     const float base = mt == -INFINITY ? 0.f : mt;
-    float lt = 0.f, x = 0.f;
-    for (int c = 0; c < split; ++c) {
-      const float* om = split > 1 ? cluster.map_shared_rank(cm, c) : cm;
-      const float* ol = split > 1 ? cluster.map_shared_rank(cl, c) : cl;
-      const float* op = split > 1 ? cluster.map_shared_rank(cpart, c) : cpart;
-      const float f = exp2f(om[r] - base);
-      lt = fmaf(ol[r], f, lt);
-      x = fmaf(op[e], f, x);
-    }
-    x *= lt == 0.f ? 0.f : 1.f / lt;
+    float lt = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < MAX_SPLIT; ++c)
+      if (c < split) {
+        const float f = exp2f(om[c] - base);
+        lt = fmaf(ol[c], f, lt);
+        x.x = fmaf(o[c].x, f, x.x);
+        x.y = fmaf(o[c].y, f, x.y);
+        x.z = fmaf(o[c].z, f, x.z);
+        x.w = fmaf(o[c].w, f, x.w);
+      }
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
     const long row = (long)sd.q_start + pr / G;
     const int head = hk * G + pr % G;
     if (p.gate.data) {
-      const long off = row * p.gate.row_stride + head * p.gate.head_stride + d;
-      x *= BF ? __bfloat162float(static_cast<const bf16*>(p.gate.data)[off])
-              : static_cast<const float*>(p.gate.data)[off];
+      const float4 g = load4<BF>(p.gate.data, row * p.gate.row_stride + head * p.gate.head_stride + d, vec);
+      x.x *= g.x; x.y *= g.y; x.z *= g.z; x.w *= g.w;
     }
-    const long off = row * p.out.row_stride + head * p.out.head_stride + d;
-    if (BF) static_cast<bf16*>(p.out.data)[off] = __float2bfloat16_rn(x);
-    else static_cast<float*>(p.out.data)[off] = x;
+    store4<BF>(p.out.data, row * p.out.row_stride + head * p.out.head_stride + d, vec, x);
     if (p.lse && d == 0) p.lse[row * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
   }
   if (split > 1) cluster.sync();  // the others may still read this CTA's part

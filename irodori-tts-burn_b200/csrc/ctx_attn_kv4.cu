@@ -2,24 +2,30 @@
 // 128, up to 16 packed query rows a KV head): the newest frames of a stream
 // against its context.
 //
-// Bound by reading the cache: 4.5 bits a value, so a value may cost no more
-// than two or three instructions.  Codes go into mma.sync.m16n8k16 as integers
+// Bound by reading the cache, 4.5 bits a value, and nearly as much by taking
+// the codes apart: 7 integer instructions for 8 codes, 65 % of that pipe at
+// 4.66 TB/s (0.71 of the copy peak; 16 streams over 20000 to 32768 rows in
+// 217 us).  Codes go into mma.sync.m16n8k16 as integers
 // and the scales, constant over 32 values of a key, are applied to the sums:
 //   score(q, j)  = sum_G sK[j][G] * (sum_{d in G} q_d c_jd)
 //   out(q, d)    = sum_j (p_qj sV[j][G(d)]) c_jd
 // The small products are exact; p sV is rounded to bf16 as p would be.
 //
 //   codes: a word holds eight codes u = c + 8; (w >> 4i) & 0xf000f are codes i
-//     and i + 4, and shifted to bit 3 under the exponent of 16 they are the
-//     bf16 pair 16 + u.  The sum over d of q (24 + c) is started at -24 sum(q)
-//     (K); 24 is subtracted exactly where the error would not cancel (V).
-//   K as the B operand [d][key]: ldmatrix hands lane (g, t) word t of key g of
-//     a group, whose pairs are the k slots of two MMAs; q is laid out alike.
+//     and i + 4, and under the exponent of 128 (16, shifted to bit 3) they are
+//     the bf16 pair 136 + c (24 + c): one or two instructions for two values.
+//     K: the sum of q over a group's offsets is subtracted from its score sum.
+//     V: the offset is subtracted from the pair, which is exact (it would grow
+//     with the number of keys in the output).
+//   K as the A operand [key][d]: ldmatrix hands lane (g, t) word t of keys g
+//     and g + 8 of a group, whose pairs are the k slots of two MMAs; q, the B
+//     operand, is laid out alike.
 //   V as the A operand [d][key]: ldmatrix.trans hands lane (g, t) the codes
 //     4g..4g+3 of keys 2t and 2t + 1 side by side, so each nibble pair is an
-//     operand register; the scores' registers are the B operand as they are.
+//     operand register.  The weights come out of the scores' layout [key][row]
+//     by movmatrix.
 //
-// A warp takes 16 keys at a time through its own ring of asynchronous copies
+// A warp takes 32 keys at a time through its own ring of asynchronous copies
 // (no CTA barrier in the loop); warps and the CTAs of a cluster share the keys
 // and join their states at the end.
 #include <algorithm>
@@ -35,13 +41,13 @@ using tcx::ex2;
 using tcx::pack_bf16x2;
 using tcx::smem_u32;
 
-constexpr int WARPS = 8, STAGES = 4, KEYS = 16;
+constexpr int WARPS = 8, STAGES = 3, KEYS = 32, SUB = KEYS / 16;
 constexpr float RESCALE_LOG2 = 8.f;  // raise the running maximum only beyond 2^8 growth
 
 template <int NGR>
 struct Ring {
   static constexpr int CODES = KEYS * NGR * 16, SCALES = KEYS * NGR * 2;  // bytes of K (and of V)
-  static constexpr int OFF_V = CODES, OFF_SK = 2 * CODES, OFF_SV = OFF_SK + SCALES;
+  static constexpr int OFF_V = CODES, OFF_SK = 2 * CODES;  // then the scales of K and of V
   static constexpr int STAGE = 2 * (CODES + SCALES);
 };
 
@@ -49,14 +55,22 @@ struct Kv4RowArgs {
   CtxAttnParams p;
   float scale_log2;
   int split;
+  int out_vec;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
   const int n = ok ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 template <int BYTES>
-__device__ __forceinline__ void cp_small(uint32_t dst, const void* src, bool ok) {
+__device__ __forceinline__ void cp_small(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_small_or_zero(uint32_t dst, const void* src, bool ok) {
   const int n = ok ? BYTES : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
 }
@@ -84,52 +98,126 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes i and i + 4 of a word (or code i of two keys' half words) as the bf16
-// pair 16 + u.
-template <int I>
-__device__ __forceinline__ uint32_t pair16(uint32_t w) {
-  const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+// The same from zero.
+__device__ __forceinline__ void mma0(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-// The same as c = u - 8.
+// 8 x 8 transpose of 16-bit elements across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Codes i and i + 4 of a word (or code i of two keys' half words) as the bf16
+// pair OFF<i> + c: codes 0 and 4 stay in place under the exponent of 128, the
+// others are shifted to bit 3 under the exponent of 16.
+// exps = {0x43004300, 0x41804180}: registers, so that mask and exponent are
+// one three-input instruction.
+struct Exponents {
+  uint32_t e128 = 0x43004300u, e16 = 0x41804180u;
+};
 template <int I>
-__device__ __forceinline__ uint32_t pair_c(uint32_t w) {
-  uint32_t x = pair16<I>(w);
-  __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), __floats2bfloat162_rn(24.f, 24.f));
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, const Exponents& x) {
+  uint32_t r;
+  if constexpr (I == 0)
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(r) : "r"(w), "r"(x.e128));  // (a & b) | c
+  else
+    asm("lop3.b32 %0, %1, 0x00780078, %2, 0xea;" : "=r"(r) : "r"(w >> (4 * I - 3)), "r"(x.e16));
+  return r;
+}
+constexpr float OFF0 = 136.f, OFFX = 24.f;
+// Both halves minus an offset.
+__device__ __forceinline__ uint32_t sub2(uint32_t x, float off) {
+  __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&x), __floats2bfloat162_rn(off, off));
   return *reinterpret_cast<uint32_t*>(&v);
 }
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// Scales of keys 2t and 2t + 1 (both halves of the 16 keys): s[half][key][G].
-template <int NGR>
-__device__ __forceinline__ void load_scales(const uint8_t* base, int t, float (&s)[2][2][NGR]) {
+// N scales at `a` (one key's, or the two of a lane) as f32.
+template <int N>
+__device__ __forceinline__ void load_scales(uint32_t a, float (&s)[N]) {
+  uint32_t w[N / 2];
+  if constexpr (N == 4) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+  else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a));
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t w[NGR];
-    const uint8_t* a = base + (8 * h + 2 * t) * NGR * 2;
-    if constexpr (NGR == 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(a);
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(a);
-      w[0] = v.x; w[1] = v.y;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int G = 0; G < NGR; ++G) {
-        const uint32_t x = w[(k * NGR + G) / 2];
-        s[h][k][G] = (G & 1) ? bf_hi(x) : bf_lo(x);
-      }
-  }
+  for (int i = 0; i < N; ++i) s[i] = (i & 1) ? bf_hi(w[i / 2]) : bf_lo(w[i / 2]);
 }
 
-// NGR = head_dim / 32 groups, NQ = packed query rows / 8.
-template <int NGR, int NQ>
+// The ring of one warp: 32 keys a stage.
+template <int NGR>
+struct Loader {
+  using RG = Ring<NGR>;
+  static constexpr int HD = 32 * NGR, KPL = 32 / NGR;
+  // This lane's chunks of a tile: every KPL-th key from ckey on, one group; and
+  // the scales of one K and one V row.
+  const CtxAttnParams& p;
+  const uint8_t *kptr, *vptr;
+  const bf16 *ksp, *vsp;
+  uint32_t cdst, sdst;
+  int ckey, lane, te, k_len;
+
+  __device__ __forceinline__ Loader(const CtxAttnParams& p_, const irt_attn_seq& sd, int hk, int first, int te_,
+                                    uint32_t ring, int lane_)
+      : p(p_), lane(lane_), te(te_), k_len(sd.k_len) {
+    ckey = lane / NGR;
+    const int G = lane % NGR;
+    const long row = (long)hk * p.k_rows + sd.k_start + (long)first * KEYS;
+    kptr = p.kc + (row + ckey) * (HD / 2) + G * 16;
+    vptr = p.vc + (row + ckey) * (HD / 2) + G * 16;
+    ksp = p.kscale + (row + lane) * NGR;
+    vsp = p.vscale + (row + lane) * NGR;
+    // chunks swizzled so that the eight rows of a matrix fall on different banks (the same for keys KPL apart)
+    cdst = ring + (ckey * NGR + (NGR == 4 ? G ^ ((ckey >> 1) & 3) : G ^ ((ckey >> 2) & 1))) * 16;
+    sdst = ring + RG::OFF_SK + lane * NGR * 2;
+  }
+  // Starts the copies of a tile (the warp's next one) into a stage.
+  __device__ __forceinline__ void issue(int tile, uint32_t stage_off) {
+    const int left = k_len - tile * KEYS;
+    if (tile < te && left >= KEYS) {
+#pragma unroll
+      for (int i = 0; i < KEYS / KPL; ++i) {
+        cp16(cdst + stage_off + i * KPL * NGR * 16, kptr + i * KPL * (HD / 2));
+        cp16(cdst + stage_off + i * KPL * NGR * 16 + RG::OFF_V, vptr + i * KPL * (HD / 2));
+      }
+      cp_small<2 * NGR>(sdst + stage_off, ksp);
+      cp_small<2 * NGR>(sdst + stage_off + RG::SCALES, vsp);
+    } else if (tile < te) {  // the last rows: zeros behind them
+#pragma unroll
+      for (int i = 0; i < KEYS / KPL; ++i) {
+        const bool ok = ckey + i * KPL < left;
+        cp16_or_zero(cdst + stage_off + i * KPL * NGR * 16, ok ? kptr + i * KPL * (HD / 2) : p.kc, ok);
+        cp16_or_zero(cdst + stage_off + i * KPL * NGR * 16 + RG::OFF_V, ok ? vptr + i * KPL * (HD / 2) : p.vc, ok);
+      }
+      cp_small_or_zero<2 * NGR>(sdst + stage_off, lane < left ? ksp : p.kscale, lane < left);
+      cp_small_or_zero<2 * NGR>(sdst + stage_off + RG::SCALES, lane < left ? vsp : p.vscale, lane < left);
+    }
+    kptr += WARPS * KEYS * (HD / 2);
+    vptr += WARPS * KEYS * (HD / 2);
+    ksp += WARPS * KEYS * NGR;
+    vsp += WARPS * KEYS * NGR;
+    cp_commit();
+  }
+};
+
+// NGR = head_dim / 32 groups.  The eight columns of the score and output
+// products are
+//   FEW: (query row, group) pairs of R = 8 / NGR packed query rows (2 at
+//     head_dim 128).  Column (r, G) of Q holds q in group G and zeros
+//     elsewhere, so one accumulator gathers the group sums and a lane scales
+//     its own two groups'; column (r, G) of P has p sV[G], and of the product
+//     with the codes of group G only the columns of G are kept.
+//   otherwise: R = 8 packed query rows, each group's sums in an accumulator of
+//     its own.
+template <int NGR, bool FEW>
 __global__ void __launch_bounds__(32 * WARPS, 2) ctx_attn_kv4_rows_kernel(const __grid_constant__ Kv4RowArgs a) {
   using RG = Ring<NGR>;
-  constexpr int HD = 32 * NGR, R = 8 * NQ;
+  constexpr int HD = 32 * NGR, R = FEW ? 8 / NGR : 8;
+  constexpr int NC = FEW ? 1 : 2;  // query rows of a lane's two columns
   const CtxAttnParams& p = a.p;
   irt_attn_seq sd;
   if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
@@ -139,241 +227,258 @@ __global__ void __launch_bounds__(32 * WARPS, 2) ctx_attn_kv4_rows_kernel(const 
   const int hk = blockIdx.y;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  uint8_t* ring = smem + warp * STAGES * RG::STAGE;
-  const uint32_t ring_s = smem_u32(ring);
-
-  // q of rows g (and g + 8): lane t has values 8t..8t+7 of each group, paired
-  // (e, e + 4) as the codes are
-  uint32_t qf[NGR][2][4];
-  float bias[NGR][NQ];  // -24 sum of q over the group
-#pragma unroll
-  for (int G = 0; G < NGR; ++G) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      const int pr = row0 + g + 8 * n;
-      if (n < NQ && pr < nrows)
-        v = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q.data) +
-                                            ((long)sd.q_start + pr / p.G) * p.q.row_stride +
-                                            (hk * p.G + pr % p.G) * p.q.head_stride + 32 * G + 8 * t);
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint32_t e = s ? v.y : v.x, f = s ? v.w : v.z;  // values 2s, 2s + 1 and 2s + 4, 2s + 5
-        qf[G][s][n] = __byte_perm(e, f, 0x5410);
-        qf[G][s][n + 2] = __byte_perm(e, f, 0x7632);
-      }
-      if (n < NQ) {
-        float x = (bf_lo(v.x) + bf_hi(v.x)) + (bf_lo(v.y) + bf_hi(v.y)) + (bf_lo(v.z) + bf_hi(v.z)) +
-                  (bf_lo(v.w) + bf_hi(v.w));
-        x += __shfl_xor_sync(0xffffffffu, x, 1);
-        x += __shfl_xor_sync(0xffffffffu, x, 2);
-        bias[G][n] = -24.f * x;
-      }
-    }
-  }
-
+  const uint32_t ring_s = smem_u32(smem) + warp * STAGES * RG::STAGE;
   const int ntiles = (sd.k_len + KEYS - 1) / KEYS;
   const int tb = (int)((long)ntiles * rank / split), te = (int)((long)ntiles * (rank + 1) / split);
-  const long head_row = (long)hk * p.k_rows + sd.k_start;
-  auto issue = [&](int tile, int stage) {
-    if (tile < te) {
-      const uint32_t dst = ring_s + stage * RG::STAGE;
-      const int k0 = tile * KEYS;
+  const int first = tb + warp;
+  Loader<NGR> ld(p, sd, hk, first, te, ring_s, lane);
 #pragma unroll
-      for (int i = 0; i < KEYS * NGR / 32; ++i) {
-        const int c = lane + 32 * i, key = c / NGR, G = c % NGR;
-        const bool ok = k0 + key < sd.k_len;
-        const long off = (head_row + k0 + (ok ? key : 0)) * (HD / 2) + G * 16;
-        // 16-byte chunks swizzled so that the eight rows of a matrix fall on different banks
-        const int sw = NGR == 4 ? G ^ ((key >> 1) & 3) : G ^ ((key >> 2) & 1);
-        cp16(dst + (key * NGR + sw) * 16, p.kc + off, ok);
-        cp16(dst + RG::OFF_V + (key * NGR + sw) * 16, p.vc + off, ok);
-      }
-      const int key = lane % 16;
-      const bool ok = k0 + key < sd.k_len;
-      const bf16* sc = (lane < 16 ? p.kscale : p.vscale) + (head_row + k0 + (ok ? key : 0)) * NGR;
-      cp_small<2 * NGR>(dst + (lane < 16 ? RG::OFF_SK : RG::OFF_SV) + key * NGR * 2, sc, ok);
+  for (int s = 0; s < STAGES - 1; ++s) ld.issue(first + s * WARPS, s * RG::STAGE);
+
+  // q of column g: lane t has values 8t..8t+7 of each group, paired (e, e + 4)
+  // as the codes are; bias: minus the codes' offsets times q, summed over the
+  // group, of this lane's columns 2t and 2t + 1
+  uint32_t qf[NGR][2][2];
+  float bias[FEW ? 1 : NGR][2];
+  const int qrow = row0 + (FEW ? g / NGR : g);
+#pragma unroll
+  for (int G = 0; G < NGR; ++G) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (qrow < nrows && (!FEW || g % NGR == G))
+      v = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q.data) +
+                                          ((long)sd.q_start + qrow / p.G) * p.q.row_stride +
+                                          (hk * p.G + qrow % p.G) * p.q.head_stride + 32 * G + 8 * t);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t e = s ? v.y : v.x, f = s ? v.w : v.z;  // values 2s, 2s + 1 and 2s + 4, 2s + 5
+      qf[G][s][0] = __byte_perm(e, f, 0x5410);
+      qf[G][s][1] = __byte_perm(e, f, 0x7632);
     }
-    cp_commit();
-  };
-  float o[NQ][NGR][2][4];
-  float m[NQ], l[NQ];
+    // values 0 and 4 have the offset OFF0
+    float x = OFF0 * (bf_lo(v.x) + bf_lo(v.z)) +
+              OFFX * ((bf_hi(v.x) + bf_hi(v.z)) + (bf_lo(v.y) + bf_hi(v.y)) + (bf_lo(v.w) + bf_hi(v.w)));
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    x += __shfl_xor_sync(0xffffffffu, x, 2);
+    const float b0 = -__shfl_sync(0xffffffffu, x, 8 * t), b1 = -__shfl_sync(0xffffffffu, x, 8 * t + 4);
+    if (FEW) {  // a column has one group
+      bias[0][0] = G == 0 ? b0 : bias[0][0] + b0;
+      bias[0][1] = G == 0 ? b1 : bias[0][1] + b1;
+    } else {
+      bias[FEW ? 0 : G][0] = b0;
+      bias[FEW ? 0 : G][1] = b1;
+    }
+  }
+  Exponents ex;
+  asm volatile("" : "+r"(ex.e128), "+r"(ex.e16));  // opaque: they stay in registers
+
+  float o[NGR][2][4];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
+  for (int G = 0; G < NGR; ++G)
 #pragma unroll
-    for (int G = 0; G < NGR; ++G)
+    for (int i = 0; i < 8; ++i) o[G][i / 4][i % 4] = 0.f;
+  float m[NC], l[NC];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[n][G][i / 4][i % 4] = 0.f;
+  for (int n = 0; n < NC; ++n) {
     m[n] = -INFINITY;
     l[n] = 0.f;
   }
-  const int first = tb + warp;
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(first + s * WARPS, s);
-  int stage = 0;
+  uint32_t stage_off = 0;
   // ldmatrix row of this lane: matrix lane / 8 = (group of the pair, key half)
   const int lkey = (lane & 7) + ((lane >> 3) & 1) * 8, lG = lane >> 4;
+  const uint32_t lrow = ring_s + lkey * NGR * 16;
+  const uint32_t lchunk = (NGR == 4 ? lG ^ ((lkey >> 1) & 3) : lG ^ ((lkey >> 2) & 1)) * 16;
+  const uint32_t srow = ring_s + RG::OFF_SK + (g * NGR + (FEW ? 2 * t % NGR : 0)) * 2;
+  constexpr int NS = FEW ? 2 : NGR;  // scales of a key that a lane uses
   for (int tile = first; tile < te; tile += WARPS) {
-    const int k0 = tile * KEYS;
-    uint32_t on = 0xffffu;  // keys that count
-    if (p.mask) on = __ballot_sync(0xffffffffu, lane < KEYS && k0 + lane < sd.k_len && p.mask[(long)sd.k_start + k0 + lane]);
-    else if (sd.k_len - k0 < KEYS) on = (1u << (sd.k_len - k0)) - 1;
+    const int left = sd.k_len - tile * KEYS;
+    uint32_t on = 0xffffffffu;  // keys that count
+    if (left < KEYS) on = (1u << left) - 1;
+    if (p.mask) on &= __ballot_sync(0xffffffffu, lane < left && p.mask[(long)sd.k_start + tile * KEYS + lane]);
     cp_wait<STAGES - 2>();
     __syncwarp();
-    const uint32_t st = ring_s + stage * RG::STAGE;
-    const uint8_t* sb = ring + stage * RG::STAGE;
 
-    // scores of keys 2t, 2t + 1 (+ 8) for query rows g (and g + 8)
-    float sc[NQ][2][2];
-    {
-      float sk[2][2][NGR];
-      load_scales<NGR>(sb + RG::OFF_SK, t, sk);
+    // scores of keys 16 u + 8 h + g
+    float sc[SUB][2][NC];
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+    for (int u = 0; u < SUB; ++u) {
+      float sk[2][NS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i / 2][i % 2] = 0.f;
+      for (int h = 0; h < 2; ++h) load_scales<NS>(srow + stage_off + (16 * u + 8 * h) * NGR * 2, sk[h]);
+      float c[4];
 #pragma unroll
       for (int hG = 0; hG < NGR / 2; ++hG) {
-        const int G0 = 2 * hG + lG;
-        const int sw = NGR == 4 ? G0 ^ ((lkey >> 1) & 3) : G0 ^ ((lkey >> 2) & 1);
         uint32_t w[4];
-        ldsm4(st + (lkey * NGR + sw) * 16, w);
+        ldsm4(lrow + stage_off + u * 16 * NGR * 16 + (lchunk ^ (hG << 5)), w);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int G = 2 * hG + x / 2, h = x % 2;
-          float c[4] = {bias[G][0], bias[G][0], bias[G][NQ - 1], bias[G][NQ - 1]};
-          mma(c, qf[G][0], pair16<0>(w[x]), pair16<1>(w[x]));
-          mma(c, qf[G][1], pair16<2>(w[x]), pair16<3>(w[x]));
+        for (int x = 0; x < 2; ++x) {
+          const int G = 2 * hG + x;
+          const uint32_t w0 = w[2 * x], w1 = w[2 * x + 1];  // keys g and g + 8
+          const uint32_t a0[4] = {code_pair<0>(w0, ex), code_pair<0>(w1, ex), code_pair<1>(w0, ex), code_pair<1>(w1, ex)};
+          const uint32_t a1[4] = {code_pair<2>(w0, ex), code_pair<2>(w1, ex), code_pair<3>(w0, ex), code_pair<3>(w1, ex)};
+          if (G == 0 || !FEW) mma0(c, a0, qf[G][0][0], qf[G][0][1]);
+          else mma(c, a0, qf[G][0][0], qf[G][0][1]);
+          mma(c, a1, qf[G][1][0], qf[G][1][1]);
+          if constexpr (!FEW) {
 #pragma unroll
-          for (int n = 0; n < NQ; ++n)
+            for (int i = 0; i < 4; ++i) {
+              float& s = sc[u][i / 2][i % 2 % NC];
+              s = fmaf(sk[i / 2][G % NS], c[i] + bias[G % (FEW ? 1 : NGR)][i % 2], G == 0 ? 0.f : s);
+            }
+          }
+        }
+      }
+      if constexpr (FEW) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) sc[n][h][k] = fmaf(sk[h][k][G], c[2 * n + k], sc[n][h][k]);
+        for (int h = 0; h < 2; ++h) {
+          float s = fmaf(sk[h][0], c[2 * h] + bias[0][0], sk[h][1] * (c[2 * h + 1] + bias[0][1]));
+          if (NGR == 4) s += __shfl_xor_sync(0xffffffffu, s, 1);  // the row's other two groups
+          sc[u][h][0] = s;
         }
       }
     }
+    if (on != 0xffffffffu) {
+#pragma unroll
+      for (int i = 0; i < 2 * SUB; ++i)
+        if (!((on >> (8 * i + g)) & 1)) {
+#pragma unroll
+          for (int n = 0; n < NC; ++n) sc[i / 2][i % 2][n] = -INFINITY;
+        }
+    }
     bool raise = false;
+    float mx[NC];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float mx = -INFINITY;
+    for (int n = 0; n < NC; ++n) {
+      mx[n] = sc[0][0][n];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float& s = sc[n][i / 2][i % 2];
-        s *= a.scale_log2;
-        if (on != 0xffffu && !((on >> (8 * (i / 2) + 2 * t + i % 2)) & 1)) s = -INFINITY;
-        mx = fmaxf(mx, s);
-      }
-      raise |= mx > m[n] + RESCALE_LOG2 || (m[n] == -INFINITY && mx > -INFINITY);
+      for (int i = 1; i < 2 * SUB; ++i) mx[n] = fmaxf(mx[n], sc[i / 2][i % 2][n]);
+      mx[n] *= a.scale_log2;
+      raise |= mx[n] > m[n] + RESCALE_LOG2 || (m[n] == -INFINITY && mx[n] > -INFINITY);
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        float mx = fmaxf(fmaxf(sc[n][0][0], sc[n][0][1]), fmaxf(sc[n][1][0], sc[n][1][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mx = fmaxf(mx, m[n]);
-        const float corr = m[n] == -INFINITY ? 0.f : ex2(m[n] - mx);
-        m[n] = mx;
+      for (int n = 0; n < NC; ++n) {
+        float mn = fmaxf(mx[n], m[n]);
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
+        const float corr = m[n] == -INFINITY ? 0.f : ex2(m[n] - mn);
+        m[n] = mn;
         l[n] *= corr;
-        // the outputs' columns are query rows 2t and 2t + 1
-        const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
 #pragma unroll
         for (int G = 0; G < NGR; ++G)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[n][G][i / 4][i % 4] *= (i & 1) ? c1 : c0;
+          for (int i = 0; i < 8; ++i)
+            if (FEW || i % 2 == n) o[G][i / 4][i % 4] *= corr;
       }
     }
-    float sv[2][2][NGR];
-    load_scales<NGR>(sb + RG::OFF_SV, t, sv);
-    if (on != 0xffffu) {  // a masked key's scale may be NaN
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!((on >> (8 * (i / 2) + 2 * t + i % 2)) & 1)) {
+    for (int u = 0; u < SUB; ++u) {
+      float sv[2][NS];
 #pragma unroll
-          for (int G = 0; G < NGR; ++G) sv[i / 2][i % 2][G] = 0.f;
+      for (int h = 0; h < 2; ++h) {
+        load_scales<NS>(srow + stage_off + RG::SCALES + (16 * u + 8 * h) * NGR * 2, sv[h]);
+        if (on != 0xffffffffu && !((on >> (16 * u + 8 * h + g)) & 1)) {  // a masked key's scale may be NaN
+#pragma unroll
+          for (int i = 0; i < NS; ++i) sv[h][i] = 0.f;
         }
-    }
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      const float base = m[n] == -INFINITY ? 0.f : m[n];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = ex2(sc[n][i / 2][i % 2] - base);
-        sc[n][i / 2][i % 2] = e;
-        l[n] += e;
-      }
-    }
-#pragma unroll
-    for (int hG = 0; hG < NGR / 2; ++hG) {
-      const int G0 = 2 * hG + lG;
-      const int sw = NGR == 4 ? G0 ^ ((lkey >> 1) & 3) : G0 ^ ((lkey >> 2) & 1);
-      uint32_t w[4];
-      ldsm4_trans(st + RG::OFF_V + (lkey * NGR + sw) * 16, w);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int G = 2 * hG + x;
-        const uint32_t w0 = w[2 * x], w1 = w[2 * x + 1];  // keys 2t, 2t + 1 and those + 8
-        const uint32_t a0[4] = {pair_c<0>(w0), pair_c<1>(w0), pair_c<0>(w1), pair_c<1>(w1)};
-        const uint32_t a1[4] = {pair_c<2>(w0), pair_c<3>(w0), pair_c<2>(w1), pair_c<3>(w1)};
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          const uint32_t b0 = pack_bf16x2(sc[n][0][0] * sv[0][0][G], sc[n][0][1] * sv[0][1][G]);
-          const uint32_t b1 = pack_bf16x2(sc[n][1][0] * sv[1][0][G], sc[n][1][1] * sv[1][1][G]);
-          mma(o[n][G][0], a0, b0, b1);
-          mma(o[n][G][1], a1, b0, b1);
+        for (int n = 0; n < NC; ++n) {
+          const float base = m[n] == -INFINITY ? 0.f : -m[n];
+          const float e = ex2(fmaf(sc[u][h][n], a.scale_log2, base));
+          l[n] += e;
+          sc[u][h][n] = e;
         }
       }
+      uint32_t b[2];
+      if constexpr (FEW) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          b[h] = transpose8(pack_bf16x2(sc[u][h][0] * sv[h][0], sc[u][h][0] * sv[h][1]));
+      }
+#pragma unroll
+      for (int hG = 0; hG < NGR / 2; ++hG) {
+        uint32_t w[4];
+        ldsm4_trans(lrow + stage_off + RG::OFF_V + u * 16 * NGR * 16 + (lchunk ^ (hG << 5)), w);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int G = 2 * hG + x;
+          const uint32_t w0 = w[2 * x], w1 = w[2 * x + 1];  // keys 2t, 2t + 1 and those + 8
+          const uint32_t a0[4] = {sub2(code_pair<0>(w0, ex), OFF0), sub2(code_pair<1>(w0, ex), OFFX),
+                                  sub2(code_pair<0>(w1, ex), OFF0), sub2(code_pair<1>(w1, ex), OFFX)};
+          const uint32_t a1[4] = {sub2(code_pair<2>(w0, ex), OFFX), sub2(code_pair<3>(w0, ex), OFFX),
+                                  sub2(code_pair<2>(w1, ex), OFFX), sub2(code_pair<3>(w1, ex), OFFX)};
+          if constexpr (!FEW) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              b[h] = transpose8(pack_bf16x2(sc[u][h][0] * sv[h][G % NS], sc[u][h][NC - 1] * sv[h][G % NS]));
+          }
+          mma(o[G][0], a0, b[0], b[1]);
+          mma(o[G][1], a1, b[0], b[1]);
+        }
+      }
     }
-    issue(tile + (STAGES - 1) * WARPS, stage == 0 ? STAGES - 1 : stage - 1);
-    stage = stage == STAGES - 1 ? 0 : stage + 1;
+    // the stage that the previous iteration read
+    ld.issue(tile + (STAGES - 1) * WARPS, stage_off == 0 ? (STAGES - 1) * RG::STAGE : stage_off - RG::STAGE);
+    stage_off = stage_off == (STAGES - 1) * RG::STAGE ? 0 : stage_off + RG::STAGE;
   }
   cp_wait<0>();
   __syncthreads();  // the rings become the partial states
 
   float* part = reinterpret_cast<float*>(smem);
-  float* pm = part + WARPS * R * HD;
+  float* pm = part + (WARPS + 1) * R * HD;
   float* pl = pm + WARPS * R;
-  float* cpart = pl + WARPS * R;
-  float* cm = cpart + R * HD;
-  float* cl = cm + R;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    float ls = l[n];
-    ls += __shfl_xor_sync(0xffffffffu, ls, 1);
-    ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-    if (t == 0) {
-      pm[warp * R + 8 * n + g] = m[n];
-      pl[warp * R + 8 * n + g] = ls;
+  for (int n = 0; n < NC; ++n) {
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], w);
+    const int r = FEW ? 2 * t / NGR : 2 * t + n;
+    if (g == 0 && (!FEW || 2 * t % NGR == 0)) {
+      pm[warp * R + r] = m[n];
+      pl[warp * R + r] = l[n];
     }
-#pragma unroll
-    for (int G = 0; G < NGR; ++G)
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int d = 32 * G + 4 * g + 2 * mt;
-        const float* c = o[n][G][mt];
-        float* dst = part + (warp * R + 8 * n + 2 * t) * HD + d;
-        *reinterpret_cast<float2*>(dst) = make_float2(c[0], c[2]);
-        *reinterpret_cast<float2*>(dst + HD) = make_float2(c[1], c[3]);
-      }
   }
-  merge_partials<true, R, WARPS>(p, sd, split, rank, hk, row0, part, pm, pl, cpart, cm, cl);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {  // columns 2t, 2t + 1
+    const int col = 2 * t + k, r = FEW ? col / NGR : col;
+    float* dst = part + (warp * R + r) * HD + 4 * g;
+    if (row0 + r >= nrows) continue;
+    if constexpr (FEW) {  // the column's group: k, or 2 + k in odd lanes
+      const bool upper = NGR == 4 && (t & 1);
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+        *reinterpret_cast<float2*>(dst + (upper ? 64 : 0) + 32 * k + 2 * mt) =
+            make_float2(upper ? o[(2 + k) % NGR][mt][k] : o[k][mt][k],
+                        upper ? o[(2 + k) % NGR][mt][2 + k] : o[k][mt][2 + k]);
+    } else {
+#pragma unroll
+      for (int G = 0; G < NGR; ++G)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+          *reinterpret_cast<float2*>(dst + 32 * G + 2 * mt) = make_float2(o[G][mt][k], o[G][mt][2 + k]);
+    }
+  }
+  merge_partials<true, R, WARPS>(p, sd, split, rank, hk, row0, part, a.out_vec);
 }
 
-template <int NGR, int NQ>
-void launch(const CtxAttnParams& p, cudaStream_t s) {
-  constexpr int R = 8 * NQ, HD = 32 * NGR;
-  constexpr size_t merge = ((WARPS + 1) * R * HD + 2 * (WARPS + 1) * R) * sizeof(float);
+template <int NGR, int R>
+void launch(void (*kernel)(Kv4RowArgs), const CtxAttnParams& p, cudaStream_t s) {
+  constexpr int HD = 32 * NGR;
+  constexpr size_t merge = merge_floats(R, WARPS, HD) * sizeof(float);
   constexpr size_t smem = std::max((size_t)WARPS * STAGES * Ring<NGR>::STAGE, merge);
   Kv4RowArgs a{};
   a.p = p;
   a.scale_log2 = p.scale * 1.4426950408889634f;
+  a.out_vec = rows_vec(p.out, 1) && (!p.gate.data || rows_vec(p.gate, 1));
   int dev = 0, sms = 0;
   IRT_CUDA(cudaGetDevice(&dev));
   IRT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const long blocks = ((long)p.max_q * p.G + R - 1) / R;
   const long ctas = blocks * p.Hkv * p.nseq;
+  // Keys are split over a cluster up to four times the two CTAs an SM holds,
+  // which evens out ragged sequences (16 streams x 16 heads of 20000 to 32768
+  // rows: 221 / 217 / 231 us at 2 / 4 / 8), while every warp keeps a tile (one
+  // frame over 576 rows: 9.1 / 8.2 / 6.8 / 7.4 us at 1 / 2 / 4 / 8).
   a.split = 1;
-  while (a.split < 8 && ctas * a.split * 2 <= 8L * sms && p.max_k >= 2L * a.split * WARPS * KEYS) a.split *= 2;
-  auto kernel = ctx_attn_kv4_rows_kernel<NGR, NQ>;
+  while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 8L * sms && p.max_k >= (long)a.split * WARPS * KEYS) a.split *= 2;
   IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
@@ -389,18 +494,22 @@ void launch(const CtxAttnParams& p, cudaStream_t s) {
   IRT_CHECK_LAUNCH();
 }
 
+template <int NGR>
+void launch_rows(long rows, const CtxAttnParams& p, cudaStream_t s) {
+  if (rows <= 8 / NGR) launch<NGR, 8 / NGR>(ctx_attn_kv4_rows_kernel<NGR, true>, p, s);
+  else launch<NGR, 8>(ctx_attn_kv4_rows_kernel<NGR, false>, p, s);
+}
+
 }  // namespace
 
 bool ctx_attention_kv4_rows(const CtxAttnParams& p, cudaStream_t s) {
   const long rows = (long)p.max_q * p.G;
-  if (!p.bf16_io || !p.kc || p.ks.data || (p.hd != 64 && p.hd != 128) || rows > 16 || !rows_vec(p.q, 1)) return false;
-  if (p.hd == 128) {
-    if (rows <= 8) launch<4, 1>(p, s);
-    else launch<4, 2>(p, s);
-  } else {
-    if (rows <= 8) launch<2, 1>(p, s);
-    else launch<2, 2>(p, s);
-  }
+  // the maximum is taken before the scale, so the scale must be positive
+  if (!p.bf16_io || !p.kc || p.ks.data || (p.hd != 64 && p.hd != 128) || rows > 16 || !(p.scale > 0.f) ||
+      !rows_vec(p.q, 1))
+    return false;
+  if (p.hd == 128) launch_rows<4>(rows, p, s);
+  else launch_rows<2>(rows, p, s);
   return true;
 }
 
