@@ -22,7 +22,6 @@ refused while gradients are recorded.
 from __future__ import annotations
 
 import ctypes
-import math
 
 from . import IrodoriError, PREC, _check, lib
 
@@ -62,16 +61,19 @@ SIGNATURES = {
 
 GROUP = 32  # values that share a scale in the 4-bit cache
 
+_NO_ROWS = _Rows()
 _torch = None
-_dtype_code = None
+_dtype_code = None  # torch dtype -> irt_precision
+_INT32 = _MASKS = None
 
 
 def _t():
     """torch, imported at the first call (the package itself does not need it)."""
-    global _torch, _dtype_code
+    global _torch, _dtype_code, _INT32, _MASKS
     if _torch is None:
         import torch
         _torch = torch
+        _INT32, _MASKS = (torch.int32,), (torch.uint8, torch.bool)
         _dtype_code = {torch.bfloat16: PREC["bf16"], torch.float32: PREC["f32"]}
     return _torch
 
@@ -82,8 +84,8 @@ def _heads(name, t, device, dtype, shape):
         raise IrodoriError(9, f"{name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
-    if t.device != device:
-        raise IrodoriError(22, f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != device:
+        raise IrodoriError(22, f"{name} must be on cuda:{device}, got {t.device}")
     if t.requires_grad and _torch.is_grad_enabled():
         raise IrodoriError(4, f"Unsupported mode: {name} requires a gradient; the operators are forward only "
                               "(call them under torch.no_grad())")
@@ -106,41 +108,40 @@ def _first(name, t):
 
 def _plain(name, t, device, dtypes, shape):
     """A contiguous helper tensor (table, mask, index, cache buffer)."""
-    if not isinstance(t, _torch.Tensor) or t.device != device:
-        raise IrodoriError(22, f"{name} must be a tensor on {device}")
+    if not isinstance(t, _torch.Tensor) or t.get_device() != device:
+        raise IrodoriError(22, f"{name} must be a tensor on cuda:{device}")
     if t.dtype not in dtypes:
         raise IrodoriError(9, f"{name} must be {dtypes[0]}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
     if not t.is_contiguous():
         raise IrodoriError(22, f"{name} must be contiguous")
     return t.data_ptr()
 
 
-class _Queue:
-    """The stream of one call.  Without an explicit stream: torch's current one on the tensors' GPU."""
+def _stream(stream, device):
+    """(handle, torch stream or None) of one call.  Without an explicit stream: torch's current one on the tensors' GPU."""
+    if stream is None:
+        return _torch._C._cuda_getCurrentRawStream(device), None
+    if isinstance(stream, int):
+        stream = _torch.cuda.ExternalStream(stream, device=device)
+    return stream.cuda_stream, stream
 
-    def __init__(self, stream, device):
-        self.torch_stream = None
-        if stream is None:
-            self.handle = _torch.cuda.current_stream(device).cuda_stream
-        else:
-            self.torch_stream = (_torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int)
-                                 else stream)
-            self.handle = self.torch_stream.cuda_stream
 
-    def empty(self, shape, dtype, device):
-        if self.torch_stream is None:
-            return _torch.empty(shape, dtype=dtype, device=device)
-        with _torch.cuda.stream(self.torch_stream):
-            return _torch.empty(shape, dtype=dtype, device=device)
+def _empty(side, shape, dtype, device):
+    """Memory for a result, of the stream that writes it."""
+    if side is None:
+        return _torch.empty(shape, dtype=dtype, device=device)
+    with _torch.cuda.stream(side):
+        return _torch.empty(shape, dtype=dtype, device=device)
 
-    def uses(self, *tensors):
-        """Keeps the allocator from handing out these tensors' memory before an explicit stream is done with them."""
-        if self.torch_stream is not None:
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(self.torch_stream)
+
+def _keep(side, *tensors):
+    """Keeps the allocator from handing out these tensors' memory before an explicit stream is done with them."""
+    if side is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(side)
 
 
 def attention_table(q_lens, k_lens, k_starts=None, device=0):
@@ -193,8 +194,8 @@ class Kv4Cache:
         torch = _t()
         if not isinstance(k_codes, torch.Tensor) or not k_codes.is_cuda or k_codes.dim() != 3:
             raise IrodoriError(22, "k_codes must be a CUDA tensor [kv_heads, rows, head_dim / 2]")
-        h, n, half = k_codes.shape
-        shape, scale_shape, dev = (h, n, half), (h, n, -(-2 * half // GROUP)), k_codes.device
+        h, n, half = shape = k_codes.shape
+        scale_shape, dev = (h, n, -(-2 * half // GROUP)), k_codes.get_device()
         u8, b16 = (torch.uint8,), (torch.bfloat16,)
         self.buffers = (k_codes, k_scales, v_codes, v_scales)
         self.rows, self.kv_heads, self.head_dim, self.device = n, h, 2 * half, dev
@@ -217,11 +218,10 @@ def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=
     n, idx = n_src, None
     if src_rows is not None:
         n = src_rows.shape[0] if isinstance(src_rows, torch.Tensor) and src_rows.dim() == 1 else -1
-        idx = _plain("src_rows", src_rows, cache.device, (torch.int32,), (n,))
-    q = _Queue(stream, cache.device)
-    _check(lib().irt_kv4_append(cache.device.index, _dtype_code[k.dtype], ctypes.byref(cache._c), row_start, n,
-                                ctypes.byref(kr), ctypes.byref(vr), n_src, idx, q.handle))
-    q.uses(k, v, src_rows, *cache.buffers)
+        idx = _plain("src_rows", src_rows, cache.device, _INT32, (n,))
+    handle, side = _stream(stream, cache.device)
+    _check(lib().irt_kv4_append(cache.device, _dtype_code[k.dtype], cache._c, row_start, n, kr, vr, n_src, idx, handle))
+    _keep(side, k, v, src_rows, *cache.buffers)
 
 
 def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=None):
@@ -235,13 +235,13 @@ def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=
     n = cache.rows - row_start if rows is None else rows
     if n < 0:
         raise IrodoriError(2, f"Shape mismatch: {n} rows from {row_start} of a cache of {cache.rows}")
-    q = _Queue(stream, cache.device)
+    handle, side = _stream(stream, cache.device)
     shape = (n, cache.kv_heads, cache.head_dim)
-    k, v = q.empty(shape, dtype, cache.device), q.empty(shape, dtype, cache.device)
-    kr, vr = (_Rows(t.data_ptr(), t.stride(0), t.stride(1)) for t in (k, v))
-    _check(lib().irt_kv4_read(cache.device.index, _dtype_code[dtype], ctypes.byref(cache._c), row_start, n,
-                              ctypes.byref(kr), ctypes.byref(vr), q.handle))
-    q.uses(*cache.buffers)
+    k, v = _empty(side, shape, dtype, cache.device), _empty(side, shape, dtype, cache.device)
+    row = cache.kv_heads * cache.head_dim
+    _check(lib().irt_kv4_read(cache.device, _dtype_code[dtype], cache._c, row_start, n,
+                              _Rows(k.data_ptr(), row, cache.head_dim), _Rows(v.data_ptr(), row, cache.head_dim), handle))
+    _keep(side, *cache.buffers)
     return k, v
 
 
@@ -249,11 +249,14 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
                context, keep):
     torch = _torch
     n, h, d = shape = q.shape
-    dev, dtype = q.device, q.dtype
-    st = _Queue(stream, dev)
+    dev, dtype = q.get_device(), q.dtype
+    handle, side = _stream(stream, dev)
     if out is None:
-        out = st.empty(shape, dtype, dev)
-    lse = st.empty((n, h), torch.float32, dev) if return_lse else None
+        out = _empty(side, shape, dtype, dev)
+        out_rows = _Rows(out.data_ptr(), h * d, d)
+    else:
+        out_rows = _heads("out", out, dev, dtype, shape)
+    lse = _empty(side, (n, h), torch.float32, dev) if return_lse else None
     if seqs is None:
         nseq, tab = (n // max_q_len if max_q_len > 0 else 0), None
         if nseq * max_q_len != n or nseq * max_k_len != k_rows:
@@ -261,16 +264,19 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
                                   f"the same number of sequences of {max_q_len} and {max_k_len}")
     else:
         nseq = seqs.shape[0] if isinstance(seqs, torch.Tensor) and seqs.dim() == 2 else -1
-        tab = _plain("seqs", seqs, dev, (torch.int32,), (nseq, 4))
+        tab = _plain("seqs", seqs, dev, _INT32, (nseq, 4))
     mask = None
     if key_mask is not None:
-        mask = _plain("key_mask", key_mask, dev, (torch.uint8, torch.bool), (k_rows,))
-    a = _AttnArgs(dev.index, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
-                  1.0 / math.sqrt(d) if scale is None else scale, n, tab, _heads("q", q, dev, dtype, shape),
-                  _Rows() if gate is None else _heads("gate", gate, dev, dtype, shape),
-                  _heads("out", out, dev, dtype, shape), mask, None if lse is None else lse.data_ptr())
-    _check(call(ctypes.byref(a), *context, st.handle))
-    st.uses(q, seqs, key_mask, gate, out, *keep)
+        mask = _plain("key_mask", key_mask, dev, _MASKS, (k_rows,))
+    a = _AttnArgs(dev, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
+                  d ** -0.5 if scale is None else scale, n, tab, _heads("q", q, dev, dtype, shape),
+                  _NO_ROWS if gate is None else _heads("gate", gate, dev, dtype, shape), out_rows, mask,
+                  None if lse is None else lse.data_ptr())
+    status = call(a, *context, handle)
+    if status:
+        _check(status)
+    if side is not None:
+        _keep(side, q, seqs, key_mask, gate, out, *keep)
     return (out, lse) if return_lse else out
 
 
@@ -296,10 +302,10 @@ def cross_attention(q, k, v, seqs, max_q_len: int, max_k_len: int, key_mask=None
     _first("k", k)
     n = k.shape[0]
     shape = (n, k.shape[1], q.shape[2])
-    kr = _heads("k", k, q.device, q.dtype, shape)
-    vr = _heads("v", v, q.device, q.dtype, shape)
+    dev = q.get_device()
+    context = (_heads("k", k, dev, q.dtype, shape), _heads("v", v, dev, q.dtype, shape), n)
     return _attention(lib().irt_cross_attention, q, shape[1], n, seqs, max_q_len, max_k_len, key_mask, gate, scale,
-                      out, return_lse, stream, (ctypes.byref(kr), ctypes.byref(vr), n), (k, v))
+                      out, return_lse, stream, context, (k, v))
 
 
 def kv4_attention(q, cache: Kv4Cache, seqs, max_q_len: int, max_k_len: int, k_self=None, v_self=None, key_mask=None,
@@ -310,13 +316,14 @@ def kv4_attention(q, cache: Kv4Cache, seqs, max_q_len: int, max_k_len: int, k_se
     as in the model's joint attention.  The other arguments and the result are
     those of ``cross_attention``, the cache's rows in the place of ``k``, ``v``."""
     _first("q", q)
-    if cache.device != q.device:
-        raise IrodoriError(22, f"the cache must be on {q.device}, got {cache.device}")
+    dev = q.get_device()
+    if cache.device != dev:
+        raise IrodoriError(22, f"the cache must be on cuda:{dev}, got cuda:{cache.device}")
     shape = (q.shape[0], cache.kv_heads, q.shape[2])
-    kr = None if k_self is None else ctypes.byref(_heads("k_self", k_self, q.device, q.dtype, shape))
-    vr = None if v_self is None else ctypes.byref(_heads("v_self", v_self, q.device, q.dtype, shape))
+    kr = None if k_self is None else _heads("k_self", k_self, dev, q.dtype, shape)
+    vr = None if v_self is None else _heads("v_self", v_self, dev, q.dtype, shape)
     return _attention(lib().irt_kv4_attention, q, cache.kv_heads, cache.rows, seqs, max_q_len, max_k_len, key_mask,
-                      gate, scale, out, return_lse, stream, (ctypes.byref(cache._c), kr, vr),
+                      gate, scale, out, return_lse, stream, (cache._c, kr, vr),
                       (k_self, v_self, *cache.buffers))
 
 
