@@ -354,7 +354,7 @@ CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache
 
 void ctx_attention(const CtxAttnParams& p, cudaStream_t s) {
   if (p.nseq == 0 || p.max_q == 0 || p.q_rows == 0) return;
-  if (ctx_attention_kv4_rows(p, s) || ctx_attention_tc(p, s)) return;
+  if (ctx_attention_kv4_rows(p, s) || ctx_attention_tc(p, s) || ctx_attention_tile(p, s)) return;
   if (p.bf16_io) rows_path<true>(p, s);
   else rows_path<false>(p, s);
 }

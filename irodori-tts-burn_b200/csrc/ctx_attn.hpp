@@ -52,6 +52,8 @@ void ctx_attention(const CtxAttnParams& p, cudaStream_t s);
 bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s);
 // Few query rows over a 4-bit cache (ctx_attn_kv4.cu); false as above.
 bool ctx_attention_kv4_rows(const CtxAttnParams& p, cudaStream_t s);
+// Many query rows in f32 arithmetic, head_dim <= 128 (ctx_attn_tile.cu); false as above.
+bool ctx_attention_tile(const CtxAttnParams& p, cudaStream_t s);
 // Bounded-wait flag of the tcgen05 kernels on the current device (0 = ok).
 int read_and_clear_ctx_attn_error();
 

@@ -1,0 +1,386 @@
+// Attention over context states in f32 arithmetic for many query rows: the f32
+// mode, and bf16 tensors that the tcgen05 kernel does not take (strides or
+// bases that are not multiples of 16 bytes, a scale that is not positive).
+// head_dim <= 128.
+//
+// One CTA = 64 packed query rows (query x grouped head) of one KV head, in
+// tiles of 64 keys; 256 threads as 16 x 16, each with 4 x 4 scores (rows
+// r + 16 i, keys c + 16 j) and 4 x HDT / 16 outputs, so both products run from
+// registers at 16 multiply-adds for each 16-byte shared-memory load, as packed
+// f32 pairs along the head dimension (half the instructions of scalar ones).
+// Bound by the FP32 pipe.  Query rows are scaled by scale log2(e) on the way
+// in.  K of the next tile is loaded during softmax and P V, V during the next
+// scores.  Shared rows of Q, K, V are f32, their 16-byte chunks XOR-swizzled by
+// the row against bank conflicts.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "ctx_attn.cuh"
+#include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace irt {
+
+namespace {
+
+using tcx::f2_fma;
+using tcx::f2_unpack;
+using tcx::smem_u32;
+
+constexpr int QT = 64, KT = 64, THREADS = 256;
+constexpr float LN2 = 0.6931471805599453f;
+
+struct TileArgs {
+  CtxAttnParams p;
+  int split;
+  int q_vec, k_vec, v_vec, ks_vec, vs_vec, out_vec;
+};
+
+template <int HDT>
+struct Smem {
+  static constexpr int CH = HDT / 4;  // 16-byte chunks of a row
+  static constexpr int OFF_K = QT * HDT, OFF_V = OFF_K + KT * HDT, OFF_P = OFF_V + KT * HDT, OFF_B = OFF_P + KT * QT;
+  static constexpr int FLOATS = OFF_B + KT;
+  // cluster merge over the tiles: O rows, then m and l
+  static_assert(QT * HDT + 2 * QT <= OFF_P, "merge state fits K and V");
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  return tcx::f2_pack(__float_as_uint(lo), __float_as_uint(hi));
+}
+
+template <bool BF, bool CTX4, int HDT>
+__global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_constant__ TileArgs a) {
+  using S = Smem<HDT>;
+  constexpr int CH = S::CH, OC = HDT / 8, NV = HDT / 64;  // NV: output chunks of four values per thread and row
+  const CtxAttnParams& p = a.p;
+  irt_attn_seq sd;
+  if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
+  const int split = a.split, rank = blockIdx.x % split;
+  const int hk = blockIdx.y, G = p.G, hd = p.hd;
+  const int row0 = (blockIdx.x / split) * QT, nrows = sd.q_len * G;
+  if (row0 >= nrows) return;  // the whole cluster
+  extern __shared__ __align__(16) float sm[];
+  float* sq = sm;
+  float* sk = sm + S::OFF_K;
+  float* sv = sm + S::OFF_V;
+  float* sp = sm + S::OFF_P;
+  float* sb = sm + S::OFF_B;  // 0 or -inf per key
+  const int tid = threadIdx.x, r = tid / 16, c = tid % 16;
+  const int n_self = p.ks.data ? (sd.q_len + KT - 1) / KT : 0;
+  const int n_all = n_self + (sd.k_len + KT - 1) / KT;
+  const int t0 = (int)((long)n_all * rank / split), nt = (int)((long)n_all * (rank + 1) / split) - t0;
+
+  // Q rows, scaled
+  const float qs = p.scale * 1.4426950408889634f;
+  for (int e = tid; e < QT * OC; e += THREADS) {
+    const int row = e / OC, o = e % OC, pr = row0 + row;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (pr < nrows && 8 * o < hd)
+      load8<BF>(p.q.data, ((long)sd.q_start + pr / G) * p.q.row_stride + (hk * G + pr % G) * p.q.head_stride + 8 * o,
+                a.q_vec, x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<float4*>(sq + row * HDT + (((2 * o + i) ^ (row & 7)) * 4)) =
+          make_float4(x[4 * i] * qs, x[4 * i + 1] * qs, x[4 * i + 2] * qs, x[4 * i + 3] * qs);
+  }
+
+  // K (or V) rows of local tile j into shared memory; rows that do not count
+  // become zeros, whatever they hold
+  auto load_tile = [&](int j, bool is_v) {
+    const int t = t0 + j;
+    const bool own = t < n_self;
+    const int k0 = own ? t * KT : (t - n_self) * KT;
+    const int left = (own ? sd.q_len : sd.k_len) - k0;
+    const long base = (long)(own ? sd.q_start : sd.k_start) + k0;
+    const uint8_t* mask = own || !p.mask ? nullptr : p.mask + base;
+    float* dst = is_v ? sv : sk;
+    const irt_rows& src = own ? (is_v ? p.vs : p.ks) : (is_v ? p.v : p.k);
+    const bool vec = own ? (is_v ? a.vs_vec : a.ks_vec) : (is_v ? a.v_vec : a.k_vec);
+    if (!is_v && tid < KT) sb[tid] = tid < left && (!mask || mask[tid]) ? 0.f : -INFINITY;
+    if (!BF && vec && (own || !CTX4)) {
+      const float* x = static_cast<const float*>(src.data) + base * src.row_stride + hk * src.head_stride;
+#pragma unroll
+      for (int i = 0; i < KT * CH / THREADS; ++i) {
+        const int e = tid + i * THREADS, key = e / CH, ch = e % CH;
+        const bool ok = key < left && 4 * ch < hd && (!mask || mask[key]);
+        cp16(smem_u32(dst + key * HDT + ((ch ^ (key & 7)) * 4)), ok ? x + key * src.row_stride + 4 * ch : x, ok);
+      }
+      return;
+    }
+    constexpr int N = KT * OC / THREADS;
+    float x[N][8];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * THREADS, key = e / OC, o = e % OC;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[i][u] = 0.f;
+      if (key >= left || 8 * o >= hd || (mask && !mask[key])) continue;
+      if (CTX4 && !own) {
+        const long cr = (long)hk * p.k_rows + base + key;
+        const uint8_t* codes = is_v ? p.vc : p.kc;
+        const bf16* sc = is_v ? p.vscale : p.kscale;
+        kv4_unpack8(*reinterpret_cast<const uint32_t*>(codes + cr * (hd / 2) + 4 * o),
+                    __bfloat162float(sc[cr * kv4_groups(hd) + o / 4]), x[i]);
+      } else {
+        load8<BF>(src.data, (base + key) * src.row_stride + hk * src.head_stride + 8 * o, vec, x[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = tid + i * THREADS, key = e / OC, o = e % OC;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        *reinterpret_cast<float4*>(dst + key * HDT + (((2 * o + u) ^ (key & 7)) * 4)) =
+            make_float4(x[i][4 * u], x[i][4 * u + 1], x[i][4 * u + 2], x[i][4 * u + 3]);
+    }
+  };
+
+  uint64_t acc[4][2 * NV];
+  float m[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int d = 0; d < 2 * NV; ++d) acc[i][d] = 0;
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
+  if (nt > 0) {
+    load_tile(0, false);
+    cp_commit();
+    load_tile(0, true);
+    cp_commit();
+  }
+  for (int j = 0; j < nt; ++j) {
+    cp_wait<1>();  // K of this tile (its V may still fly)
+    __syncthreads();
+    float s[4][4];
+    {
+      uint64_t s2[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s2[i][n] = 0;
+      const ulonglong2* q2 = reinterpret_cast<const ulonglong2*>(sq);
+      const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(sk);
+#pragma unroll 4
+      for (int ch = 0; ch < CH; ++ch) {
+        ulonglong2 qa[4], kb[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qa[i] = q2[(r + 16 * i) * CH + (ch ^ (r & 7))];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) kb[n] = k2[(c + 16 * n) * CH + (ch ^ (c & 7))];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) s2[i][n] = f2_fma(qa[i].y, kb[n].y, f2_fma(qa[i].x, kb[n].x, s2[i][n]));
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const bool off = sb[c + 16 * n] != 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x, y;
+          f2_unpack(s2[i][n], x, y);
+          s[i][n] = off ? -INFINITY : x + y;
+        }
+      }
+    }
+    __syncthreads();  // every thread is done with K of this tile
+    if (j + 1 < nt) load_tile(j + 1, false);
+    cp_commit();
+
+    // online softmax: a row's scores are in the 16 threads of a half warp
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+      mx = fmaxf(mx, m[i]);
+      const float base = mx == -INFINITY ? 0.f : mx;  // NaN scores stay NaN in P and the sum
+      const float corr = exp2f(m[i] - base);
+      m[i] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        s[i][n] = exp2f(s[i][n] - base);
+        sum += s[i][n];
+      }
+      l[i] = fmaf(l[i], corr, sum);
+      const uint64_t c2 = pack2(corr, corr);
+#pragma unroll
+      for (int d = 0; d < 2 * NV; ++d) acc[i][d] = f2_fma(acc[i][d], c2, 0);
+    }
+    // P transposed: the four rows of a thread are one chunk of a key
+    float4* p4 = reinterpret_cast<float4*>(sp);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int key = c + 16 * n;
+      p4[key * 16 + (r ^ (key & 15))] = make_float4(s[0][n], s[1][n], s[2][n], s[3][n]);
+    }
+    cp_wait<1>();  // V of this tile (K of the next may still fly)
+    __syncthreads();
+    const ulonglong2* v2 = reinterpret_cast<const ulonglong2*>(sv);
+#pragma unroll 4
+    for (int key = 0; key < KT; ++key) {
+      const float4 pr = p4[key * 16 + (r ^ (key & 15))];
+      ulonglong2 v[NV];
+#pragma unroll
+      for (int u = 0; u < NV; ++u) v[u] = v2[key * CH + ((c + 16 * u) ^ (key & 7))];
+      const float pv[4] = {pr.x, pr.y, pr.z, pr.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t pp = pack2(pv[i], pv[i]);
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+          acc[i][2 * u] = f2_fma(pp, v[u].x, acc[i][2 * u]);
+          acc[i][2 * u + 1] = f2_fma(pp, v[u].y, acc[i][2 * u + 1]);
+        }
+      }
+    }
+    __syncthreads();  // every thread is done with V and P of this tile
+    if (j + 1 < nt) load_tile(j + 1, true);
+    cp_commit();
+  }
+  cp_wait<0>();
+
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+  auto write = [&](int row, int d, float4 x, float ms, float ls) {  // four values from d of a row of the block
+    const float inv = ls == 0.f ? 0.f : 1.f / ls;
+    x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+    const int pr = row0 + row;
+    const long q = (long)sd.q_start + pr / G;
+    const int head = hk * G + pr % G;
+    if (p.gate.data) {
+      const float4 g = load4<BF>(p.gate.data, q * p.gate.row_stride + head * p.gate.head_stride + d, a.out_vec);
+      x.x *= g.x; x.y *= g.y; x.z *= g.z; x.w *= g.w;
+    }
+    store4<BF>(p.out.data, q * p.out.row_stride + head * p.out.head_stride + d, a.out_vec, x);
+    if (p.lse && d == 0) p.lse[q * p.H + head] = ls == 0.f ? -INFINITY : fmaf(ms, LN2, logf(ls));
+  };
+  if (split == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = r + 16 * i;
+      if (row0 + row >= nrows) continue;
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int d = 4 * (c + 16 * u);
+        float4 x;
+        f2_unpack(acc[i][2 * u], x.x, x.y);
+        f2_unpack(acc[i][2 * u + 1], x.z, x.w);
+        if (d < hd) write(row, d, x, m[i], l[i]);
+      }
+    }
+    return;
+  }
+  // this CTA's rows for the others, over its tiles
+  __syncthreads();
+  float* so = sm;
+  float* sml = sm + QT * HDT;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r + 16 * i;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      *reinterpret_cast<ulonglong2*>(so + row * HDT + 4 * (c + 16 * u)) = make_ulonglong2(acc[i][2 * u], acc[i][2 * u + 1]);
+    if (c == 0) {
+      sml[row] = m[i];
+      sml[QT + row] = l[i];
+    }
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int valid = min(QT, nrows - row0), per_row = hd / 4;
+  for (int e = tid; e < ((valid - rank + split - 1) / split) * per_row; e += THREADS) {
+    const int row = (e / per_row) * split + rank, d = (e % per_row) * 4;  // rows dealt out to the CTAs
+    float mt = -INFINITY;
+    for (int u = 0; u < split; ++u) mt = fmaxf(mt, cluster.map_shared_rank(sml, u)[row]);
+    const float base = mt == -INFINITY ? 0.f : mt;
+    float lt = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int u = 0; u < split; ++u) {
+      const float* om = cluster.map_shared_rank(sml, u);
+      const float f = exp2f(om[row] - base);
+      const float4 o = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, u) + row * HDT + d);
+      lt = fmaf(om[QT + row], f, lt);
+      x.x = fmaf(o.x, f, x.x);
+      x.y = fmaf(o.y, f, x.y);
+      x.z = fmaf(o.z, f, x.z);
+      x.w = fmaf(o.w, f, x.w);
+    }
+    write(row, d, x, mt, lt);
+  }
+  cluster.sync();  // the others may still read this CTA's rows
+}
+
+template <bool BF, bool CTX4, int HDT>
+void launch(const CtxAttnParams& p, cudaStream_t s) {
+  TileArgs a{};
+  a.p = p;
+  a.q_vec = rows_vec(p.q, BF);
+  a.k_vec = rows_vec(p.k, BF);
+  a.v_vec = rows_vec(p.v, BF);
+  a.ks_vec = rows_vec(p.ks, BF);
+  a.vs_vec = rows_vec(p.vs, BF);
+  a.out_vec = rows_vec(p.out, BF) && (!p.gate.data || rows_vec(p.gate, BF));
+  int dev = 0, sms = 0;
+  IRT_CUDA(cudaGetDevice(&dev));
+  IRT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const long blocks = ((long)p.max_q * p.G + QT - 1) / QT;
+  const long ctas = blocks * p.Hkv * p.nseq;
+  const long ktiles = (p.max_k + KT - 1L) / KT + (p.ks.data ? (p.max_q + KT - 1L) / KT : 0);
+  a.split = 1;
+  while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 2L * sms && a.split * 2 <= ktiles) a.split *= 2;
+  constexpr size_t smem = Smem<HDT>::FLOATS * sizeof(float);
+  auto kernel = ctx_attn_tile_kernel<BF, CTX4, HDT>;
+  IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)a.split, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IRT_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  IRT_CHECK_LAUNCH();
+}
+
+template <bool BF, bool CTX4>
+void launch_hd(const CtxAttnParams& p, cudaStream_t s) {
+  if (p.hd <= 64) launch<BF, CTX4, 64>(p, s);
+  else launch<BF, CTX4, 128>(p, s);
+}
+
+}  // namespace
+
+bool ctx_attention_tile(const CtxAttnParams& p, cudaStream_t s) {
+  // Up to 8 rows the row kernel reads the keys once or twice and has no idle threads.
+  if (p.hd > 128 || (long)p.max_q * p.G <= 8) return false;
+  if (p.bf16_io) {
+    if (p.kc) launch_hd<true, true>(p, s);
+    else launch_hd<true, false>(p, s);
+  } else {
+    if (p.kc) launch_hd<false, true>(p, s);
+    else launch_hd<false, false>(p, s);
+  }
+  return true;
+}
+
+}  // namespace irt

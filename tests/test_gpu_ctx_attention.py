@@ -493,3 +493,57 @@ def test_the_step_agrees_with_attention_over_the_values(pkg, dev):
     ref = reference(q, hk, hv, seqs, 1 / math.sqrt(hd))
     for out in (pkg.kv4_attention(q, c, tab, 40, 301), pkg.cross_attention(q, hk, hv, tab, 40, 301)):
         check(out, None, ref)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("ql,scale", [(2, -0.1), (2, 0.0), (75, -0.1), (75, 0.0), (75, 3e-3)])
+def test_any_finite_scale(pkg, dev, dtype, four_bit, ql, scale):
+    """A negative scale turns the order of the scores, zero makes them equal;
+    masked keys stay out of both."""
+    g = gen(dev, 41)
+    h, hd, nk = 4, 128, 131
+    q = torch.randn(ql, h, hd, device=dev, generator=g).to(dtype)
+    k = torch.randn(nk, h, hd, device=dev, generator=g).to(dtype)
+    v = torch.randn(nk, h, hd, device=dev, generator=g).to(dtype)
+    mask = (torch.arange(nk, device=dev) % 3 != 0).to(torch.uint8)
+    seqs = [(0, ql, 0, nk)]
+    tab = device_table(seqs, dev)
+    if four_bit:
+        c = pkg.Kv4Cache(nk, h, hd)
+        pkg.kv4_append(c, k, v)
+        k, v = pkg.kv4_read(c, dtype=F32)
+        out, lse = pkg.kv4_attention(q, c, tab, ql, nk, key_mask=mask, scale=scale, return_lse=True)
+    else:
+        out, lse = pkg.cross_attention(q, k, v, tab, ql, nk, key_mask=mask, scale=scale, return_lse=True)
+    check(out, lse, reference(q, k, v, seqs, scale, mask=mask))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n,kl", [(1, 40), (3, 2000), (40, 64), (64, 1100)])
+def test_split_and_unsplit_key_ranges(pkg, dev, dtype, n, kl):
+    """From one sequence, whose keys are shared by a cluster, to batches that
+    fill the GPU; ragged, with sequences far shorter than the longest."""
+    g = gen(dev, n * kl)
+    h, hd = 4, 128
+    for q_hi in (1, 5, 90):
+        r = torch.Generator().manual_seed(n + kl + q_hi)
+        ql = [int(x) for x in torch.randint(0, q_hi + 1, (n,), generator=r)]
+        kls = [int(x) for x in torch.randint(0, kl + 1, (n,), generator=r)]
+        ql[0], kls[-1] = q_hi, kl
+        seqs, nq, nk = table(ql, kls)
+        q = torch.randn(nq, h, hd, device=dev, generator=g).to(dtype)
+        k = torch.randn(nk, h, hd, device=dev, generator=g).to(dtype)
+        v = torch.randn(nk, h, hd, device=dev, generator=g).to(dtype)
+        tab = device_table(seqs, dev)
+        out, lse = pkg.cross_attention(q, k, v, tab, q_hi, kl, return_lse=True)
+        check(out, lse, reference(q, k, v, seqs, 1 / math.sqrt(hd)))
+        c = pkg.Kv4Cache(nk, h, hd)
+        pkg.kv4_append(c, k, v)
+        ck, cv = pkg.kv4_read(c, dtype=F32)
+        out, lse = pkg.kv4_attention(q, c, tab, q_hi, kl, return_lse=True)
+        check(out, lse, reference(q, ck, cv, seqs, 1 / math.sqrt(hd)))
+        ks, vs = torch.randn(2, nq, h, hd, device=dev, generator=g).to(dtype).unbind(0)
+        out, lse = pkg.kv4_attention(q, c, tab, q_hi, kl, k_self=ks, v_self=vs, return_lse=True)
+        check(out, lse, reference(q, ck, cv, seqs, 1 / math.sqrt(hd), ks=ks, vs=vs))
+    pkg.attention_check(0)
