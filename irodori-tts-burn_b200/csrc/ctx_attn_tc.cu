@@ -105,6 +105,12 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
                : "memory");
 }
+__device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void st_shared8_zero(uint32_t addr) {
   asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(addr), "r"(0) : "memory");
 }
@@ -113,7 +119,8 @@ template <int HDT, bool CTX4>
 __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     ctx_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKS,
                        const __grid_constant__ CUtensorMap tmVS, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcArgs a) {
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
+                       const __grid_constant__ TcArgs a) {
   using C = Cfg<HDT, CTX4>;
   pdl_wait();
   pdl_trigger();
@@ -140,7 +147,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   auto V_EMPTY = [&](int s) { return bar(3 + 3 * NKV + s); };
   auto S_FULL = [&](int b) { return bar(3 + 4 * NKV + b); };
   auto P_FULL = [&](int b) { return bar(5 + 4 * NKV + b); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 7 + 4 * NKV);
+  const uint32_t G_FULL = bar(7 + 4 * NKV);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 4 * NKV);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sm_warps = (rows + 31) / 32;  // softmax warps that have a query row
@@ -148,6 +156,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     mbar_init(Q_FULL, 1);
     mbar_init(O_DONE, 1);
     mbar_init(O_FINAL, 1);
+    mbar_init(G_FULL, 1);
     for (int r = 0; r < NKV; ++r) {
       mbar_init(K_FULL(r), C::FULL_COUNT);
       mbar_init(K_EMPTY(r), 1);
@@ -205,6 +214,13 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         for (int j = 0; j < nt; ++j) {
           load_v(j);
           if (j + 2 < nt) load_k(j + 2);
+        }
+        if (split == 1 && p.gate.data) {  // the gate takes Q's place once the last scores are done
+          mbar_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1);
+          mbar_expect_tx(G_FULL, C::Q_BYTES);
+#pragma unroll
+          for (int h = 0; h < HDT / 64; ++h)
+            tma_load_3d(sQ + h * C::Q_HALF, &tmG, G_FULL, 64 * h, head0, sd.q_start + q0);
         }
       }
     } else if (warp == 5) {
@@ -439,22 +455,16 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   // ---------------- output ----------------
   const int qrow = warp * 32 + lane;
   if (split == 1) {
+    // Rows go through shared memory in Q's place (all products that read Q are
+    // done), so that a warp writes 256 contiguous bytes of a row at a time: a
+    // thread's own 16-byte stores, a row apart, took twice as long.
     if (warp < sm_warps) {
       const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-      const bool ok = qrow < rows;
-      const long row = (long)sd.q_start + q0 + qrow / Gp;
-      const int head = head0 + qrow % Gp;
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-      bf16* out = static_cast<bf16*>(p.out.data) + (ok ? row * p.out.row_stride + head * p.out.head_stride : 0);
-      const bf16* gate = p.gate.data && ok
-                             ? static_cast<const bf16*>(p.gate.data) + row * p.gate.row_stride + head * p.gate.head_stride
-                             : nullptr;
+      const bool gated = p.gate.data && nt > 0;
+      if (gated) mbar_wait(G_FULL, 0);
 #pragma unroll 1
       for (int c = 0; c < HDT / 32; ++c) {
-        uint4 gv[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (gate && c * 32 + u * 8 < p.hd) gv[u] = *reinterpret_cast<const uint4*>(gate + c * 32 + u * 8);
         uint32_t r[32];
         if (nt > 0) {
           tmem_ld32(tmem + lane_off + C::TM_O + c * 32, r);
@@ -465,20 +475,41 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          if (!ok || c * 32 + u * 8 >= p.hd) continue;
-          const __nv_bfloat162* gp = reinterpret_cast<const __nv_bfloat162*>(&gv[u]);
+          const int chunk = (c & 1) * 4 + u;
+          const uint32_t addr = sQ + (c >> 1) * C::Q_HALF + qrow * 128 + ((chunk ^ (qrow & 7)) << 4);
+          uint32_t g[4];
+          if (gated) ld_shared16(addr, g);
           uint32_t op[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float g0 = gate ? __bfloat162float(gp[k].x) : 1.f, g1 = gate ? __bfloat162float(gp[k].y) : 1.f;
-            op[k] = pack_bf16x2(__uint_as_float(r[u * 8 + 2 * k]) * inv * g0,
-                                __uint_as_float(r[u * 8 + 2 * k + 1]) * inv * g1);
+            float x = __uint_as_float(r[u * 8 + 2 * k]) * inv, y = __uint_as_float(r[u * 8 + 2 * k + 1]) * inv;
+            if (gated) {
+              x *= __uint_as_float(g[k] << 16);
+              y *= __uint_as_float(g[k] & 0xffff0000u);
+            }
+            op[k] = pack_bf16x2(x, y);
           }
-          *reinterpret_cast<uint4*>(out + c * 32 + u * 8) = make_uint4(op[0], op[1], op[2], op[3]);
+          st_shared16(addr, make_uint4(op[0], op[1], op[2], op[3]));
         }
       }
-      if (ok && p.lse)
-        p.lse[row * p.H + head] = l_run == 0.f ? -INFINITY : fmaf(m_run, LN2, logf(l_run));
+      if (qrow < rows && p.lse)
+        p.lse[((long)sd.q_start + q0 + qrow / Gp) * p.H + head0 + qrow % Gp] =
+            l_run == 0.f ? -INFINITY : fmaf(m_run, LN2, logf(l_run));
+      __syncwarp();
+      constexpr int LPR = HDT / 8;  // lanes of a row
+      const int chunk = lane % LPR;
+      if (8 * chunk < p.hd) {
+        bf16* out = static_cast<bf16*>(p.out.data) + 8 * chunk;
+#pragma unroll 4
+        for (int i = lane / LPR; i < 32; i += 32 / LPR) {
+          const int row = warp * 32 + i;
+          if (row >= rows) break;
+          uint32_t v[4];
+          ld_shared16(sQ + (chunk >> 3) * C::Q_HALF + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), v);
+          *reinterpret_cast<uint4*>(out + ((long)sd.q_start + q0 + row / Gp) * p.out.row_stride +
+                                    (head0 + row % Gp) * p.out.head_stride) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
     }
   } else {
     // this CTA's O, m and l over its tiles (all products are done, so nothing
@@ -572,9 +603,10 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
   a.p = p;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.Gp = QT % p.G == 0 ? p.G : 1;
-  CUtensorMap q, ks, vs, k, v;
+  CUtensorMap q, ks, vs, k, v, g;
   if (!rows_map(q, p.q, p.q_rows, p.H, p.hd, a.Gp, QT / a.Gp)) return false;
-  ks = vs = k = v = q;
+  ks = vs = k = v = g = q;
+  if (p.gate.data && !rows_map(g, p.gate, p.q_rows, p.H, p.hd, a.Gp, QT / a.Gp)) return false;
   if (p.ks.data && (!rows_map(ks, p.ks, p.q_rows, p.Hkv, p.hd, 1, KT) ||
                     !rows_map(vs, p.vs, p.q_rows, p.Hkv, p.hd, 1, KT)))
     return false;
@@ -605,7 +637,7 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  IRT_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, ks, vs, k, v, a));
+  IRT_CUDA(cudaLaunchKernelEx(&cfg, kernel, q, ks, vs, k, v, g, a));
   IRT_CHECK_LAUNCH();
   return true;
 }
