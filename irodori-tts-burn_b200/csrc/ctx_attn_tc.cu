@@ -13,7 +13,7 @@
 //   4     TMA: Q once, K and V of native tiles (2-stage rings, K two tiles
 //         ahead of V).
 //   5     tcgen05.mma issue: S_j = Q K_j^T, O += P_j V_j.
-//   6, 7  (4-bit context) codes -> bf16 K and V tiles in the same swizzled
+//   6..9  (4-bit context) codes -> bf16 K and V tiles in the same swizzled
 //         layout.  A value c s has at most 8 significant bits, so the bf16 tile
 //         is exact and the products are those of the cache's values.
 // Keys that do not count (past the sequence, masked) must not meet the P V
@@ -45,15 +45,15 @@ constexpr float LN2 = 0.6931471805599453f;
 
 template <int HDT, bool CTX4>
 struct Cfg {
-  static constexpr int THREADS = CTX4 ? 256 : 192;
+  static constexpr int CODE_WARPS = CTX4 ? 4 : 0, THREADS = 192 + 32 * CODE_WARPS;
   static constexpr uint32_t Q_HALF = QT * 128, Q_BYTES = Q_HALF * (HDT / 64);  // 64-column halves
   static constexpr uint32_t HALF = KT * 128, TILE = HALF * (HDT / 64);
   static constexpr uint32_t OFF_K = Q_BYTES, OFF_V = OFF_K + NKV * TILE, OFF_BAR = OFF_V + NKV * TILE;
   static constexpr size_t SMEM = OFF_BAR + 256 + 1024;
   static constexpr uint32_t IDESC_S = idesc_bf16(128, KT, false), IDESC_O = idesc_bf16(128, HDT, true);
   static constexpr uint32_t TM_S = 0, TM_O = 2 * KT, TM_COLS = 256;
-  // arrivals that fill a K or V stage: the TMA thread and both code warps
-  static constexpr uint32_t FULL_COUNT = CTX4 ? 3 : 1;
+  // arrivals that fill a K or V stage: the TMA thread and the code warps of K or V
+  static constexpr uint32_t FULL_COUNT = 1 + CODE_WARPS / 2;
   // cluster merge: f32 O rows (padded against bank conflicts), m and l
   static constexpr int OLD = HDT + 4;
   static_assert((uint32_t)QT * OLD * 4 + 2 * QT * 4 <= OFF_BAR, "merge buffers fit the tiles");
@@ -74,6 +74,17 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
       "r"(tmem_a), "l"(db), "r"(idesc), "r"(acc));
 }
 
+// 32 lanes x 16 or 32 columns from the warp's registers.
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
+__device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 // Box of a (d, head, row) tensor.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
@@ -83,20 +94,22 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// Eight codes -> eight bf16 values c s, in order.  (128 + code) is a bf16
-// number with the code in its low mantissa bits; minus 136 and times s are
-// exact.
-__device__ __forceinline__ uint4 kv4_bf16x8(uint32_t w, __nv_bfloat162 s2) {
-  const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;  // codes 0 2 4 6 / 1 3 5 7
+// Eight codes u -> eight bf16 values (u - 8) s, in order.  Under the exponent
+// of 16 a code is the bf16 number 16 + u; (16 + u) s - 24 s is exact in one
+// fused step, since 24 s has at most 7 significant bits.  n2 = -24 s, twice.
+// BIG: 24 s is beyond bf16's range; (16 + u - 24) s in two exact steps.
+template <bool BIG>
+__device__ __forceinline__ uint4 kv4_bf16x8(uint32_t w, __nv_bfloat162 s2, __nv_bfloat162 n2) {
+  const uint32_t lo = ((w << 3) & 0x78787878u) | 0x80808080u;                        // codes 0 2 4 6, low bytes
+  const uint32_t hi = ((w >> 1) & 0x78787878u) | 0x80808080u;                        // codes 1 3 5 7
   const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);  // 0 1 2 3 / 4 5 6 7
-  uint32_t r[4] = {__byte_perm(a, 0x43434343u, 0x4140), __byte_perm(a, 0x43434343u, 0x4342),
-                   __byte_perm(b, 0x43434343u, 0x4140), __byte_perm(b, 0x43434343u, 0x4342)};
-  const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);
+  uint32_t r[4] = {__byte_perm(a, 0x41414141u, 0x4140), __byte_perm(a, 0x41414141u, 0x4342),
+                   __byte_perm(b, 0x41414141u, 0x4140), __byte_perm(b, 0x41414141u, 0x4342)};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    __nv_bfloat162 v = *reinterpret_cast<__nv_bfloat162*>(&r[i]);
-    v = __hmul2(__hsub2(v, off), s2);
-    r[i] = *reinterpret_cast<uint32_t*>(&v);
+    const __nv_bfloat162 u = *reinterpret_cast<__nv_bfloat162*>(&r[i]);
+    const __nv_bfloat162 v = BIG ? __hmul2(__hsub2(u, __floats2bfloat162_rn(24.f, 24.f)), s2) : __hfma2(u, s2, n2);
+    r[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
@@ -261,102 +274,79 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       }
     } else if (CTX4 && warp >= 6) {
       // ---------------- codes -> bf16 tiles ----------------
-      // warp 6: the lower half of the head dimension, warp 7: the upper; a
-      // lane has keys lane and lane + 32, so the eight 16-byte chunks that a
-      // quarter warp stores fall on different banks under the swizzle.
-      constexpr int W = HDT / 16;      // words of eight codes per key and warp
-      constexpr int NG = HDT / 64;     // groups of 32 per key and warp
-      const int part = warp - 6, hd = p.hd, groups = kv4_groups(hd);
-      const bool wide = hd % KV4_GROUP == 0;  // 16-byte aligned groups of codes
+      // Warps 6 and 7 fill the K tiles, 8 and 9 the V tiles, each half of the
+      // head dimension; a lane has keys lane and lane + 32, so the eight
+      // 16-byte chunks that a quarter warp stores fall on different banks under
+      // the swizzle.  The codes of a tile are read while the one before it is
+      // written.  One small copy of the code: unrolled over tiles it outgrew
+      // the instruction cache next to the softmax (64 utterances 523 us
+      // against 429 us).
+      constexpr int W = HDT / 16;   // words of eight codes per key and lane
+      constexpr int NG = HDT / 64;  // groups of 32
+      const bool is_v = warp >= 8;
+      const int part = warp & 1, hd = p.hd, groups = kv4_groups(hd);
+      const long row0 = (long)hk * p.k_rows + sd.k_start + lane;
+      const uint8_t* codes = (is_v ? p.vc : p.kc) + row0 * (hd / 2) + part * W * 4;
+      const bf16* scales = (is_v ? p.vscale : p.kscale) + row0 * groups + part * NG;
+      const uint8_t* mask = p.mask ? p.mask + sd.k_start + lane : nullptr;
       struct Codes {
-        uint32_t w[2][W];
+        uint4 w[2][NG];
         uint16_t s[2][NG];
-        bool ok[2];
-      };
-      // operation i: K0 K1 V0 K2 V1 K3 ... V(nt-1), the order of the TMA warp
-      auto op_of = [&](int i, bool& is_v, int& j) {
-        if (nt == 1) {
-          is_v = i == 1;
-          j = 0;
-        } else if (i < 2) {
-          is_v = false;
-          j = i;
-        } else {
-          const int u = i - 2;  // V0 K2 V1 K3 ... then V(nt-2) V(nt-1)
-          is_v = (u & 1) == 0 || u >= 2 * (nt - 2);
-          j = u >= 2 * (nt - 2) ? nt - 2 + (u - 2 * (nt - 2)) : (u & 1) ? u / 2 + 2 : u / 2;
-        }
-      };
-      auto fetch = [&](int i, Codes& c) {
-        bool is_v;
-        int j;
-        op_of(i, is_v, j);
-        if (t0 + j < n_self) return;
-        const uint8_t* base = is_v ? p.vc : p.kc;
-        const bf16* sc = is_v ? p.vscale : p.kscale;
-        const int nkeys = keys_of(j);
+      } next;
+      auto fetch = [&](int j) {
+        const int k0 = (t0 + j - n_self) * KT;
+        if (k0 < 0) return;  // a tile of own rows
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int key = lane + 32 * e;
-          const long row = (long)row_of(j) + key;
-          c.ok[e] = key < nkeys && (!p.mask || p.mask[row]);
-          const long cr = (long)hk * p.k_rows + row;
+          const int k = k0 + 32 * e;  // of lane 0
+          const bool ok = k + lane < sd.k_len && (!mask || mask[k]);
 #pragma unroll
-          for (int i4 = 0; i4 < W; i4 += 4) {
-            const int o = part * W + i4;
-            if (wide) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (c.ok[e] && 8 * o < hd) v = *reinterpret_cast<const uint4*>(base + cr * (hd / 2) + 4 * o);
-              c.w[e][i4] = v.x; c.w[e][i4 + 1] = v.y; c.w[e][i4 + 2] = v.z; c.w[e][i4 + 3] = v.w;
-            } else {
-#pragma unroll
-              for (int i1 = 0; i1 < 4; ++i1)
-                c.w[e][i4 + i1] = c.ok[e] && 8 * (o + i1) < hd
-                                      ? *reinterpret_cast<const uint32_t*>(base + cr * (hd / 2) + 4 * (o + i1))
-                                      : 0x88888888u;
-            }
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const int gi = part * NG + g;
-            c.s[e][g] = c.ok[e] && gi < groups ? reinterpret_cast<const uint16_t*>(sc)[cr * groups + gi] : 0;
+          for (int g = 0; g < NG; ++g) {  // scale 0: a row that does not count, or what is behind head_dim, becomes zeros
+            const bool in = ok && part * NG + g < groups;
+            next.w[e][g] = in ? *reinterpret_cast<const uint4*>(codes + (long)k * (hd / 2) + 16 * g) : make_uint4(0, 0, 0, 0);
+            next.s[e][g] = in ? reinterpret_cast<const uint16_t*>(scales)[(long)k * groups + g] : 0;
           }
         }
       };
-      auto put = [&](int i, const Codes& c) {
-        bool is_v;
-        int j;
-        op_of(i, is_v, j);
+      fetch(0);
+#pragma unroll 1
+      for (int j = 0; j < nt; ++j) {
+        const Codes cur = next;
+        if (j + 1 < nt) fetch(j + 1);
         const int r = j % NKV;
-        const uint32_t full = is_v ? V_FULL(r) : K_FULL(r), empty = is_v ? V_EMPTY(r) : K_EMPTY(r);
-        mbar_wait(empty, ((j / NKV) & 1) ^ 1);
+        mbar_wait(is_v ? V_EMPTY(r) : K_EMPTY(r), ((j / NKV) & 1) ^ 1);
         if (t0 + j >= n_self) {
           const uint32_t dst = is_v ? sV(r) : sK(r);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int key = lane + 32 * e;
+            const uint32_t row = dst + (lane + 32 * e) * 128;
 #pragma unroll
-            for (int o = 0; o < W; ++o) {
-              const uint16_t sb = c.s[e][o / 4];
-              const uint32_t s2 = (uint32_t)sb << 16 | sb;
-              const uint4 v = kv4_bf16x8(c.w[e][o], *reinterpret_cast<const __nv_bfloat162*>(&s2));
-              const int chunk = part * W + o;  // 16-byte chunk of the row
-              st_shared16(dst + (chunk >> 3) * C::HALF + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), v);
+            for (int g = 0; g < NG; ++g) {
+              const uint32_t sb = (uint32_t)cur.s[e][g] << 16 | cur.s[e][g];
+              const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&sb);
+              const __nv_bfloat162 n2 = __hmul2(s2, __floats2bfloat162_rn(-24.f, -24.f));
+              const uint32_t w[4] = {cur.w[e][g].x, cur.w[e][g].y, cur.w[e][g].z, cur.w[e][g].w};
+              const int c0 = part * W + 4 * g;  // 16-byte chunk of the row
+              const uint32_t at = row + (c0 >> 3) * C::HALF;
+              if (cur.s[e][g] < 0x7d00) {  // 2^123
+#pragma unroll
+                for (int o = 0; o < 4; ++o)
+                  st_shared16(at + ((((c0 + o) & 7) ^ (lane & 7)) << 4), kv4_bf16x8<false>(w[o], s2, n2));
+              } else {
+                uint64_t lo = (uint64_t)w[1] << 32 | w[0], hi = (uint64_t)w[3] << 32 | w[2];
+#pragma unroll 1
+                for (int o = 0; o < 4; ++o) {
+                  st_shared16(at + ((((c0 + o) & 7) ^ (lane & 7)) << 4), kv4_bf16x8<true>((uint32_t)lo, s2, n2));
+                  lo = lo >> 32 | hi << 32;
+                  hi >>= 32;
+                }
+              }
             }
           }
           fence_proxy_async();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(full);
-      };
-      Codes c0, c1;
-      const int ops = 2 * nt;
-      fetch(0, c0);
-      for (int i = 0; i < ops; i += 2) {  // an even number of operations
-        fetch(i + 1, c1);
-        put(i, c0);
-        if (i + 2 < ops) fetch(i + 2, c0);
-        put(i + 1, c1);
+        if (lane == 0) mbar_arrive(is_v ? V_FULL(r) : K_FULL(r));
       }
     } else if (warp < sm_warps) {
       // ---------------- softmax ----------------
@@ -376,34 +366,48 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         const bool partial = (on0 & on1) != 0xffffffffu;
         mbar_wait(S_FULL(b), (j >> 1) & 1);
         tc_fence_after();
-        uint32_t sr[KT];
+        // Scores in halves of 32 columns.  One register copy of a tile's scores
+        // (native context), or two readings of them: 96 registers a thread
+        // leave room for the code warps.
+        constexpr int HC = CTX4 ? 32 : KT;
+        uint32_t sr[HC];
+        auto load_scores = [&](int col) {
 #pragma unroll
-        for (int g = 0; g < KT / 32; ++g)
-          tmem_ld32(tmem + lane_off + C::TM_S + b * KT + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * g]));
-        tmem_wait_ld();
-        if (partial) {
+          for (int g = 0; g < HC / 32; ++g)
+            tmem_ld32(tmem + lane_off + C::TM_S + b * KT + col + 32 * g, *reinterpret_cast<uint32_t(*)[32]>(&sr[32 * g]));
+          tmem_wait_ld();
+          if (partial) {
 #pragma unroll
-          for (int i = 0; i < KT; ++i)
-            if (!((i < 32 ? on0 >> i : on1 >> (i - 32)) & 1)) sr[i] = __float_as_uint(-INFINITY);
-          if (!CTX4 || own) {  // V rows that do not count: zeros
-            mbar_wait(V_FULL(j % NKV), (j / NKV) & 1);
-            for (int key = warp; key < KT; key += sm_warps)
-              if (!((key < 32 ? on0 >> key : on1 >> (key - 32)) & 1)) {
-                if (HDT == 128) st_shared8_zero(sV(j % NKV) + (lane >> 4) * C::HALF + key * 128 + (lane & 15) * 8);
-                else if (lane < 16) st_shared8_zero(sV(j % NKV) + key * 128 + lane * 8);
-              }
-            fence_proxy_async();
+            for (int i = 0; i < HC; ++i) {
+              const uint32_t on = i < 32 ? (col ? on1 : on0) : on1;
+              if (!((on >> (i & 31)) & 1)) sr[i] = __float_as_uint(-INFINITY);
+            }
           }
-        }
-        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int col = 0; col < KT; col += HC) {
+          load_scores(col);
+          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < KT; i += 4) {
-          mx0 = fmaxf(mx0, __uint_as_float(sr[i]));
-          mx1 = fmaxf(mx1, __uint_as_float(sr[i + 1]));
-          mx2 = fmaxf(mx2, __uint_as_float(sr[i + 2]));
-          mx3 = fmaxf(mx3, __uint_as_float(sr[i + 3]));
+          for (int i = 0; i < HC; i += 4) {
+            mx0 = fmaxf(mx0, __uint_as_float(sr[i]));
+            mx1 = fmaxf(mx1, __uint_as_float(sr[i + 1]));
+            mx2 = fmaxf(mx2, __uint_as_float(sr[i + 2]));
+            mx3 = fmaxf(mx3, __uint_as_float(sr[i + 3]));
+          }
+          mx = fmaxf(mx, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)));
         }
-        const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2;
+        mx *= a.scale_log2;
+        if (partial && (!CTX4 || own)) {  // V rows that do not count: zeros
+          mbar_wait(V_FULL(j % NKV), (j / NKV) & 1);
+          for (int key = warp; key < KT; key += sm_warps)
+            if (!((key < 32 ? on0 >> key : on1 >> (key - 32)) & 1)) {
+              if (HDT == 128) st_shared8_zero(sV(j % NKV) + (lane >> 4) * C::HALF + key * 128 + (lane & 15) * 8);
+              else if (lane < 16) st_shared8_zero(sV(j % NKV) + key * 128 + lane * 8);
+            }
+          fence_proxy_async();
+        }
         float corr = 1.f;
         const bool raise = mx > m_run + RESCALE_LOG2 || (m_run == -INFINITY && mx > -INFINITY);
         if (raise) {
@@ -426,21 +430,26 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
             tmem_st32(tmem + lane_off + C::TM_O + c * 32, r);
           }
         }
-        uint32_t pk[KT / 2];
         const uint64_t sc2 = f2_pack(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
         const uint64_t nb2 = f2_pack(__float_as_uint(nbase), __float_as_uint(nbase));
         uint64_t rs2 = 0;
+#pragma unroll 1
+        for (int col = 0; col < KT; col += HC) {
+          if (CTX4) load_scores(col);
+          uint32_t pk[HC / 2];
 #pragma unroll
-        for (int c = 0; c < KT / 2; ++c) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(sr[2 * c], sr[2 * c + 1]), sc2, nb2), x0, x1);
-          const float p0 = ex2(x0), p1 = ex2(x1);
-          rs2 = f2_add(rs2, f2_pack(__float_as_uint(p0), __float_as_uint(p1)));
-          pk[c] = pack_bf16x2(p0, p1);
+          for (int c = 0; c < HC / 2; ++c) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(sr[2 * c], sr[2 * c + 1]), sc2, nb2), x0, x1);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            rs2 = f2_add(rs2, f2_pack(__float_as_uint(p0), __float_as_uint(p1)));
+            pk[c] = pack_bf16x2(p0, p1);
+          }
+          // P of these columns: half as many, over scores that have been read
+          tmem_st_cols(tmem + lane_off + C::TM_S + b * KT + col / 2, pk);
         }
         float rs0, rs1;
         f2_unpack(rs2, rs0, rs1);
-        tmem_st32(tmem + lane_off + C::TM_S + b * KT, pk);
         tmem_wait_st();
         l_run = l_run * corr + (rs0 + rs1);
         tc_fence_before();
@@ -651,6 +660,8 @@ bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s) {
   const irt_rows* const rows[7] = {&p.q, &p.out, &p.gate, &p.k, &p.v, &p.ks, &p.vs};
   for (const irt_rows* r : rows)
     if (r->data && !rows_vec(*r, 1)) return false;
+  // whole groups of codes, 16 bytes each
+  if (p.kc && p.hd % KV4_GROUP) return false;
   if (p.kc) return p.hd > 64 ? launch<128, true>(p, s) : launch<64, true>(p, s);
   return p.hd > 64 ? launch<128, false>(p, s) : launch<64, false>(p, s);
 }

@@ -547,3 +547,21 @@ def test_split_and_unsplit_key_ranges(pkg, dev, dtype, n, kl):
         out, lse = pkg.kv4_attention(q, c, tab, q_hi, kl, k_self=ks, v_self=vs, return_lse=True)
         check(out, lse, reference(q, ck, cv, seqs, 1 / math.sqrt(hd), ks=ks, vs=vs))
     pkg.attention_check(0)
+
+
+@pytest.mark.parametrize("ql", [1, 40])
+@pytest.mark.parametrize("size", [2.0 ** 124, 2.0 ** 121, 2.0 ** -90])
+def test_kv4_values_at_the_ends_of_the_range(pkg, dev, ql, size):
+    """The cache's largest and smallest scales: one key's value comes back as
+    the cache holds it (a softmax over one key is 1)."""
+    g = gen(dev, 43)
+    h, hd = 2, 128
+    x = torch.randn(4, h, hd, device=dev, generator=g)
+    x = (x / x.abs().amax() * size).to(BF)
+    c = pkg.Kv4Cache(4, h, hd)
+    pkg.kv4_append(c, torch.randn(4, h, hd, device=dev, generator=g).to(BF), x)
+    _, v = pkg.kv4_read(c)
+    q = torch.randn(ql, h, hd, device=dev, generator=g).to(BF)
+    out = pkg.kv4_attention(q, c, device_table([(0, ql, 2, 1)], dev), ql, 1)
+    pkg.attention_check(0)
+    assert torch.equal(out, v[2].expand(ql, h, hd))
