@@ -87,9 +87,9 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
           const long cr = (long)hk * p.k_rows + row;
           const int g = kv4_groups(hd);
           kv4_unpack8(*reinterpret_cast<const uint32_t*>(p.kc + cr * (hd / 2) + 4 * o),
-                      __bfloat162float(p.kscale[cr * g + o / 4]), k[u]);
+                      reinterpret_cast<const uint16_t*>(p.kscale)[cr * g + o / 4], k[u]);
           kv4_unpack8(*reinterpret_cast<const uint32_t*>(p.vc + cr * (hd / 2) + 4 * o),
-                      __bfloat162float(p.vscale[cr * g + o / 4]), v[u]);
+                      reinterpret_cast<const uint16_t*>(p.vscale)[cr * g + o / 4], v[u]);
         } else {
           load8<BF>(p.k.data, row * p.k.row_stride + hk * p.k.head_stride + 8 * o, a.k_vec, k[u]);
           load8<BF>(p.v.data, row * p.v.row_stride + hk * p.v.head_stride + 8 * o, a.v_vec, v[u]);

@@ -72,10 +72,37 @@ inline bool rows_vec(const irt_rows& r, int bf16_io) {
   return (reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.row_stride % per == 0 && r.head_stride % per == 0;
 }
 
-// Eight codes (one word) of a 4-bit group with scale s.
-__device__ __forceinline__ void kv4_unpack8(uint32_t w, float s, float (&x)[8]) {
+// Eight codes u -> eight bf16 values (u - 8) s, in order.  Under the exponent
+// of 16 a code is the bf16 number 16 + u; (16 + u) s - 24 s is exact in one
+// fused step, since 24 s has at most 7 significant bits.  n2 = -24 s, twice.
+// BIG: 24 s is beyond bf16's range; (16 + u - 24) s in two exact steps.
+template <bool BIG>
+__device__ __forceinline__ uint4 kv4_bf16x8(uint32_t w, __nv_bfloat162 s2, __nv_bfloat162 n2) {
+  const uint32_t lo = ((w << 3) & 0x78787878u) | 0x80808080u;                        // codes 0 2 4 6, low bytes
+  const uint32_t hi = ((w >> 1) & 0x78787878u) | 0x80808080u;                        // codes 1 3 5 7
+  const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);  // 0 1 2 3 / 4 5 6 7
+  uint32_t r[4] = {__byte_perm(a, 0x41414141u, 0x4140), __byte_perm(a, 0x41414141u, 0x4342),
+                   __byte_perm(b, 0x41414141u, 0x4140), __byte_perm(b, 0x41414141u, 0x4342)};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = (float)((int)((w >> (4 * j)) & 15u) - 8) * s;
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 u = *reinterpret_cast<__nv_bfloat162*>(&r[i]);
+    const __nv_bfloat162 v = BIG ? __hmul2(__hsub2(u, __floats2bfloat162_rn(24.f, 24.f)), s2) : __hfma2(u, s2, n2);
+    r[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// Eight codes (one word) of a 4-bit group with scale s, bf16 bits `sb`.
+__device__ __forceinline__ void kv4_unpack8(uint32_t w, uint16_t sb, float (&x)[8]) {
+  const uint32_t s = (uint32_t)sb << 16 | sb;
+  const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&s);
+  const uint4 v = kv4_bf16x8<true>(w, s2, s2);
+  const uint32_t p[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(p[i] << 16);
+    x[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+  }
 }
 
 // Four values of a row of the output (or gate).

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
         const uint8_t* codes = is_v ? p.vc : p.kc;
         const bf16* sc = is_v ? p.vscale : p.kscale;
         kv4_unpack8(*reinterpret_cast<const uint32_t*>(codes + cr * (hd / 2) + 4 * o),
-                    __bfloat162float(sc[cr * kv4_groups(hd) + o / 4]), x[i]);
+                    reinterpret_cast<const uint16_t*>(sc)[cr * kv4_groups(hd) + o / 4], x[i]);
       } else {
         load8<BF>(src.data, (base + key) * src.row_stride + hk * src.head_stride + 8 * o, vec, x[i]);
       }

@@ -12,27 +12,41 @@ namespace irt {
 
 namespace {
 
-constexpr float KV4_MIN_MAX = 7.88860905e-31f; // 2^-100: smaller groups hold zeros
+constexpr float KV4_MIN_MAX = 7.88860905e-31f;  // 2^-100: smaller groups hold zeros
+constexpr float MAGIC = 12582912.f;              // 1.5 * 2^23: adding it rounds to a whole number
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Scale of a group with largest magnitude `amax` (finite).
 __device__ __forceinline__ float kv4_scale(float amax) {
   if (amax < KV4_MIN_MAX) return 0.f;
-  // largest 5-bit number <= amax / 7, then the next one up where 7 s < amax
-  const uint32_t t = __float_as_uint(amax / 7.f) & 0xfff80000u;
-  float s = __uint_as_float(t);
-  if (7.f * s < amax) s = __uint_as_float(t + 0x80000u);
-  return fminf(s, __uint_as_float(0x7e100000u));  // 1.125 * 2^125
+  // a 5-bit number at or just below amax / 7, then the next ones up while 7 s < amax
+  uint32_t t = __float_as_uint(amax * 0.14285709f) & 0xfff80000u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (7.f * __uint_as_float(t) < amax) t += 0x80000u;
+  return fminf(__uint_as_float(t), __uint_as_float(0x7e100000u));  // 1.125 * 2^125
 }
 
-// Code + 8 of x in a group of scale s > 0, inv ~ 1 / s.
-__device__ __forceinline__ uint32_t kv4_code(float x, float s, float inv) {
-  const float a = fabsf(x);
-  float c = rintf(a * inv);
-  // a * inv may have been rounded across a border
-  if (a >= (c + 0.5f) * s) c += 1.f;
-  else if (a < (c - 0.5f) * s) c -= 1.f;
-  const int u = (int)fminf(c, 7.f);
-  return (uint32_t)(8 + (x < 0.f ? -u : u));
+// x / s rounded half away from zero.  inv is a little below 1 / s, so the
+// first rounding ends on a border's inner side at worst; the remainder x - c s
+// is exact and tells.
+__device__ __forceinline__ float kv4_code(float x, float s, float half, float inv) {
+  float c = fmaf(x, inv, MAGIC) - MAGIC;
+  const float e = fmaf(-c, s, x);
+  if (fabsf(e) >= half) c += copysignf(1.f, x);
+  return c;
+}
+// Codes of eight values, plus 8, in one word: four are a whole number below
+// 2^16 that f32 multiply-adds put together exactly.
+__device__ __forceinline__ uint32_t kv4_pack(const float (&c)[8]) {
+  const float lo = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + (MAGIC + 34952.f);  // 0x8888
+  const float hi = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + (MAGIC + 34952.f);
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
 struct Kv4Side {
@@ -49,76 +63,164 @@ struct Kv4Args {
 };
 
 constexpr int KV4_TILE = 64;  // rows of one head per CTA
+constexpr int KV4_APPEND_THREADS = 128, KV4_READ_THREADS = 256;
 
-// Four lanes hold a group, eight values each: its maximum takes two shuffles
-// and every lane stores its eight codes as one word.  A CTA covers 64 rows of
-// one head, whose codes and scales are contiguous in the cache.  Bound by
-// memory: 2 (or 4) bytes a value in, 4.5 bits out.
+// Eight values as they are in memory; zeros where `in` is false.
 template <bool BF>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__ Kv4Args a) {
-  const Kv4Side& sd = a.side[blockIdx.z];
-  const int h = blockIdx.y;
-  const int octs = 4 * a.groups;  // lanes of a row, the last group's missing ones included
-  const long r0 = (long)blockIdx.x * KV4_TILE;
-  const int items = KV4_TILE * octs;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < items; i += 256) {  // items is a multiple of 32: whole warps stay together
-    const long r = r0 + i / octs;
-    const int o = i % octs;
-    long src = -1;
-    if (r < a.n) {
-      src = a.idx ? a.idx[r] : r;
-      if (src >= a.src_rows) src = -1;
-    }
-    const bool in = src >= 0 && 8 * o < a.hd;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (in) load8<BF>(sd.x.data, src * sd.x.row_stride + h * sd.x.head_stride + 8 * o, sd.vec, x);
-    float m = 0.f;
-    bool bad = false;
+struct Raw {
+  uint4 v[BF ? 1 : 2];
+};
+template <bool BF>
+__device__ __forceinline__ void load_raw(const Kv4Side& sd, long off, bool in, Raw<BF>& r) {
+  constexpr int N = BF ? 1 : 2;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      m = fmaxf(m, fabsf(x[j]));
-      bad |= !(fabsf(x[j]) <= 3.402823466e+38f);  // NaN or infinity
-    }
-    if (bad) m = INFINITY;  // fmaxf drops NaN
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    float s = m == INFINITY ? __uint_as_float(0x7fc00000u) : kv4_scale(m);
-    uint32_t w = 0x88888888u;
-    if (s > 0.f) {  // not for zero or NaN
-      const float inv = 1.f / s;
-      w = 0;
+  for (int i = 0; i < N; ++i) r.v[i] = make_uint4(0, 0, 0, 0);
+  if (!in) return;
+  const uint8_t* p = static_cast<const uint8_t*>(sd.x.data) + off * (BF ? 2 : 4);
+  if (sd.vec) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w |= kv4_code(x[j], s, inv) << (4 * j);
-    } else if (s != 0.f) {
-      w = 0x99999999u;
+    for (int i = 0; i < N; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = BF ? (uint32_t) reinterpret_cast<const uint16_t*>(p)[2 * k] |
+                        (uint32_t) reinterpret_cast<const uint16_t*>(p)[2 * k + 1] << 16
+                  : reinterpret_cast<const uint32_t*>(p)[4 * i + k];
+      r.v[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if (in) {
-      const long row = (long)h * a.rows + a.row_start + r;
-      *reinterpret_cast<uint32_t*>(sd.codes + row * (a.hd / 2) + 4 * o) = w;
-      if ((o & 3) == 0) sd.scales[row * a.groups + o / 4] = __float2bfloat16_rn(s);
+  }
+}
+template <bool BF>
+__device__ __forceinline__ void expand(const Raw<BF>& r, float (&x)[8]) {
+  const uint32_t a[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  if constexpr (BF) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(a[i] << 16);
+      x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+    }
+  } else {
+    const uint32_t b[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = __uint_as_float(a[i]);
+      x[4 + i] = __uint_as_float(b[i]);
     }
   }
 }
 
+// Largest magnitude of eight values; NaN if one is NaN.
 template <bool BF>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4Args a) {
+__device__ __forceinline__ float amax8(const Raw<BF>& r) {
+  if constexpr (BF) {  // two at a time as they are
+    const uint32_t a[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+    __nv_bfloat162 m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = a[i] & 0x7fff7fffu;
+      m[i] = *reinterpret_cast<const __nv_bfloat162*>(&u);
+    }
+    const __nv_bfloat162 t = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
+    return max_nan(__bfloat162float(t.x), __bfloat162float(t.y));
+  } else {
+    float x[8], m = 0.f;
+    expand<BF>(r, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(x[j]));
+    return m;
+  }
+}
+
+// Two lanes hold a group, sixteen values each: one shuffle joins its maximum.
+// A CTA covers 64 rows of one head (NG groups a row), whose codes and scales
+// are contiguous in the cache; a thread's loads are in flight together.  Bound
+// by the issue of instructions for bf16 (2 bytes a value in, 4.5 bits out).
+template <bool BF, int NG>
+__global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __grid_constant__ Kv4Args a) {
+  constexpr int HALVES = 2 * NG, N = KV4_TILE * HALVES / KV4_APPEND_THREADS;  // half groups of a row, missing ones included
+  constexpr int B = BF ? (N < 4 ? N : 4) : (N < 2 ? N : 2);          // of a thread, in flight
   const Kv4Side& sd = a.side[blockIdx.z];
   const int h = blockIdx.y;
-  const int octs = a.hd / 8;
+  const long r0 = (long)blockIdx.x * KV4_TILE, head = h * sd.x.head_stride;
+  uint8_t* codes = sd.codes + ((long)h * a.rows + a.row_start + r0) * (a.hd / 2);
+  bf16* scales = sd.scales + ((long)h * a.rows + a.row_start + r0) * NG;
+#pragma unroll 1
+  for (int i0 = 0; i0 < N; i0 += B) {
+    Raw<BF> raw[B][2];
+    bool in[B][2];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int e = threadIdx.x + KV4_APPEND_THREADS * (i0 + i), d = e % HALVES * 16;
+      const long r = r0 + e / HALVES;
+      long src = -1;
+      if (r < a.n && (N % B == 0 || i0 + i < N)) {
+        src = a.idx ? a.idx[r] : r;
+        if (src >= a.src_rows) src = -1;
+      }
+      const long off = src * sd.x.row_stride + head + d;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        in[i][u] = src >= 0 && d + 8 * u < a.hd;
+        load_raw<BF>(sd, off + 8 * u, in[i][u], raw[i][u]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int e = threadIdx.x + KV4_APPEND_THREADS * (i0 + i), half = e % HALVES;
+      float m = max_nan(amax8<BF>(raw[i][0]), amax8<BF>(raw[i][1]));
+      m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      float s = kv4_scale(m), inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+      inv *= 0.9999996f;  // one part in 2.5e6 below, more than rcp.approx is off
+      float hs = 0.5f * s;
+      if (s == 0.f) {  // the values are too small: codes 0
+        inv = 0.f;
+        hs = INFINITY;
+      }
+      const bool bad = !(m <= 3.402823466e+38f);  // NaN or infinity
+      if (bad) s = __uint_as_float(0x7fc00000u);
+      const int row = e / HALVES;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float x[8];
+        expand<BF>(raw[i][u], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = kv4_code(x[j], s, hs, inv);
+        const uint32_t w = bad ? 0x99999999u : kv4_pack(x);
+        if (in[i][u]) *reinterpret_cast<uint32_t*>(codes + row * (a.hd / 2) + half * 8 + 4 * u) = w;
+      }
+      if (in[i][0] && !(half & 1)) scales[row * NG + half / 2] = __float2bfloat16_rn(s);
+    }
+  }
+}
+
+template <bool BF, int NG>
+__global__ void __launch_bounds__(KV4_READ_THREADS) kv4_read_kernel(const __grid_constant__ Kv4Args a) {
+  constexpr int OCTS = 4 * NG, N = KV4_TILE * OCTS / KV4_READ_THREADS;
+  const Kv4Side& sd = a.side[blockIdx.z];
+  const int h = blockIdx.y;
   const long r0 = (long)blockIdx.x * KV4_TILE;
-  const int items = KV4_TILE * octs;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < items; i += 256) {
-    const long r = r0 + i / octs;
-    const int o = i % octs;
-    if (r >= a.n) break;
-    const long row = (long)h * a.rows + a.row_start + r;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(sd.codes + row * (a.hd / 2) + 4 * o);
-    const float s = __bfloat162float(sd.scales[row * a.groups + o / 4]);
+  uint32_t w[N];
+  uint16_t sb[N];
+  bool in[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = threadIdx.x + KV4_READ_THREADS * i, o = e % OCTS;
+    in[i] = r0 + e / OCTS < a.n && 8 * o < a.hd;
+    const long row = (long)h * a.rows + a.row_start + r0 + e / OCTS;
+    w[i] = in[i] ? *reinterpret_cast<const uint32_t*>(sd.codes + row * (a.hd / 2) + 4 * o) : 0u;
+    sb[i] = in[i] ? reinterpret_cast<const uint16_t*>(sd.scales)[row * NG + o / 4] : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int e = threadIdx.x + KV4_READ_THREADS * i, o = e % OCTS;
+    const long r = r0 + e / OCTS;
     float x[8];
-    kv4_unpack8(w, s, x);
-    store8<BF>(sd.x.data, r * sd.x.row_stride + h * sd.x.head_stride + 8 * o, sd.vec, x);
+    kv4_unpack8(w[i], sb[i], x);
+    if (in[i]) store8<BF>(sd.x.data, r * sd.x.row_stride + h * sd.x.head_stride + 8 * o, sd.vec, x);
   }
 }
 
@@ -134,6 +236,24 @@ Kv4Args kv4_args(const irt_kv4_cache& c, int bf16_io, long row_start, long n, co
   return a;
 }
 
+template <int NG>
+void launch(const Kv4Args& a, int bf16_io, bool read, dim3 grid, cudaStream_t s) {
+  if (read) {
+    if (bf16_io) kv4_read_kernel<true, NG><<<grid, KV4_READ_THREADS, 0, s>>>(a);
+    else kv4_read_kernel<false, NG><<<grid, KV4_READ_THREADS, 0, s>>>(a);
+  } else {
+    if (bf16_io) kv4_append_kernel<true, NG><<<grid, KV4_APPEND_THREADS, 0, s>>>(a);
+    else kv4_append_kernel<false, NG><<<grid, KV4_APPEND_THREADS, 0, s>>>(a);
+  }
+}
+
+void launch(const Kv4Args& a, int kv_heads, int bf16_io, bool read, cudaStream_t s) {
+  using F = void (*)(const Kv4Args&, int, bool, dim3, cudaStream_t);
+  static const F by_groups[8] = {launch<1>, launch<2>, launch<3>, launch<4>, launch<5>, launch<6>, launch<7>, launch<8>};
+  by_groups[a.groups - 1](a, bf16_io, read, dim3((unsigned)((a.n + KV4_TILE - 1) / KV4_TILE), kv_heads, 2), s);
+  IRT_CHECK_LAUNCH();
+}
+
 }  // namespace
 
 void kv4_append(const irt_kv4_cache& c, int bf16_io, long row_start, long n, const irt_rows& k, const irt_rows& v,
@@ -142,20 +262,13 @@ void kv4_append(const irt_kv4_cache& c, int bf16_io, long row_start, long n, con
   Kv4Args a = kv4_args(c, bf16_io, row_start, n, k, v);
   a.src_rows = src_rows;
   a.idx = idx;
-  const dim3 grid((unsigned)((n + KV4_TILE - 1) / KV4_TILE), c.kv_heads, 2);
-  if (bf16_io) kv4_append_kernel<true><<<grid, 256, 0, s>>>(a);
-  else kv4_append_kernel<false><<<grid, 256, 0, s>>>(a);
-  IRT_CHECK_LAUNCH();
+  launch(a, c.kv_heads, bf16_io, false, s);
 }
 
 void kv4_read(const irt_kv4_cache& c, int bf16_io, long row_start, long n, const irt_rows& k, const irt_rows& v,
               cudaStream_t s) {
   if (n <= 0) return;
-  const Kv4Args a = kv4_args(c, bf16_io, row_start, n, k, v);
-  const dim3 grid((unsigned)((n + KV4_TILE - 1) / KV4_TILE), c.kv_heads, 2);
-  if (bf16_io) kv4_read_kernel<true><<<grid, 256, 0, s>>>(a);
-  else kv4_read_kernel<false><<<grid, 256, 0, s>>>(a);
-  IRT_CHECK_LAUNCH();
+  launch(kv4_args(c, bf16_io, row_start, n, k, v), c.kv_heads, bf16_io, true, s);
 }
 
 }  // namespace irt
