@@ -22,46 +22,28 @@ refused while gradients are recorded.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import IrodoriError, PREC, _check, lib
 
 
-class _Rows(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+# The header's structures, as their bytes: irt_rows; irt_attn_args (device, dtype, heads, kv_heads, head_dim, num_seqs,
+# max_q_len, max_k_len, scale, q_rows, seqs, q, gate, out, key_mask, lse); irt_kv4_cache.
+_ROWS = struct.Struct("@Pqq")
+_ATTN = struct.Struct("@8ifqPPqqPqqPqqPP")
+_CACHE = struct.Struct("@qiiPPPP")
 
-
-class _AttnArgs(ctypes.Structure):
-    _fields_ = [
-        ("device", ctypes.c_int32), ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
-        ("head_dim", ctypes.c_int32), ("num_seqs", ctypes.c_int32), ("max_q_len", ctypes.c_int32),
-        ("max_k_len", ctypes.c_int32), ("scale", ctypes.c_float), ("q_rows", ctypes.c_int64),
-        ("seqs", ctypes.c_void_p), ("q", _Rows), ("gate", _Rows), ("out", _Rows), ("key_mask", ctypes.c_void_p),
-        ("lse", ctypes.c_void_p),
-    ]
-
-
-class _Cache(ctypes.Structure):
-    _fields_ = [("rows", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
-                ("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
-                ("v_scales", ctypes.c_void_p)]
-
-
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
 SIGNATURES = {
-    "irt_cross_attention": (ctypes.c_int, [ctypes.POINTER(_AttnArgs), ctypes.POINTER(_Rows), ctypes.POINTER(_Rows),
-                                           ctypes.c_int64, ctypes.c_void_p]),
-    "irt_kv4_append": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.POINTER(_Cache), ctypes.c_int64,
-                                      ctypes.c_int64, ctypes.POINTER(_Rows), ctypes.POINTER(_Rows), ctypes.c_int64,
-                                      ctypes.c_void_p, ctypes.c_void_p]),
-    "irt_kv4_read": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.POINTER(_Cache), ctypes.c_int64, ctypes.c_int64,
-                                    ctypes.POINTER(_Rows), ctypes.POINTER(_Rows), ctypes.c_void_p]),
-    "irt_kv4_attention": (ctypes.c_int, [ctypes.POINTER(_AttnArgs), ctypes.POINTER(_Cache), ctypes.POINTER(_Rows),
-                                         ctypes.POINTER(_Rows), ctypes.c_void_p]),
-    "irt_attention_check": (ctypes.c_int, [ctypes.c_int]),
+    "irt_cross_attention": (_I, [_P, _P, _P, _L, _P]),
+    "irt_kv4_append": (_I, [_I, _I, _P, _L, _L, _P, _P, _L, _P, _P]),
+    "irt_kv4_read": (_I, [_I, _I, _P, _L, _L, _P, _P, _P]),
+    "irt_kv4_attention": (_I, [_P, _P, _P, _P, _P]),
+    "irt_attention_check": (_I, [_I]),
 }
 
 GROUP = 32  # values that share a scale in the 4-bit cache
 
-_NO_ROWS = _Rows()
 _torch = None
 _dtype_code = None  # torch dtype -> irt_precision
 _INT32 = _MASKS = None
@@ -79,7 +61,11 @@ def _t():
 
 
 def _heads(name, t, device, dtype, shape):
-    """Rows of heads of a [rows, heads, head_dim] tensor (any strides, the last one 1)."""
+    """(address, row stride, head stride) of a [rows, heads, head_dim] tensor (any strides, the last one 1)."""
+    if t.dtype is dtype and t.get_device() == device and t.shape == shape and not t.requires_grad:
+        row, head, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), row, head
     if t.dtype is not dtype:
         raise IrodoriError(9, f"{name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
@@ -89,10 +75,9 @@ def _heads(name, t, device, dtype, shape):
     if t.requires_grad and _torch.is_grad_enabled():
         raise IrodoriError(4, f"Unsupported mode: {name} requires a gradient; the operators are forward only "
                               "(call them under torch.no_grad())")
-    st = t.stride()
-    if st[2] != 1 and shape[2] != 1 and t.numel():
+    if t.stride(2) != 1 and t.numel():
         raise IrodoriError(22, f"{name}: the values of a head must be contiguous")
-    return _Rows(t.data_ptr(), st[0], st[1])
+    return t.data_ptr(), t.stride(0), t.stride(1)
 
 
 def _first(name, t):
@@ -107,16 +92,17 @@ def _first(name, t):
 
 
 def _plain(name, t, device, dtypes, shape):
-    """A contiguous helper tensor (table, mask, index, cache buffer)."""
+    """Address of a contiguous helper tensor (table, mask, index, cache buffer)."""
+    if isinstance(t, _torch.Tensor) and t.dtype in dtypes and t.get_device() == device and t.shape == shape and \
+            t.is_contiguous():
+        return t.data_ptr()
     if not isinstance(t, _torch.Tensor) or t.get_device() != device:
         raise IrodoriError(22, f"{name} must be a tensor on cuda:{device}")
     if t.dtype not in dtypes:
         raise IrodoriError(9, f"{name} must be {dtypes[0]}, got {t.dtype}")
     if t.shape != shape:
         raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
-    if not t.is_contiguous():
-        raise IrodoriError(22, f"{name} must be contiguous")
-    return t.data_ptr()
+    raise IrodoriError(22, f"{name} must be contiguous")
 
 
 def _stream(stream, device):
@@ -134,6 +120,13 @@ def _empty(side, shape, dtype, device):
         return _torch.empty(shape, dtype=dtype, device=device)
     with _torch.cuda.stream(side):
         return _torch.empty(shape, dtype=dtype, device=device)
+
+
+def _empty_like(side, t):
+    if side is None:
+        return _torch.empty_like(t)
+    with _torch.cuda.stream(side):
+        return _torch.empty_like(t)
 
 
 def _keep(side, *tensors):
@@ -199,10 +192,10 @@ class Kv4Cache:
         u8, b16 = (torch.uint8,), (torch.bfloat16,)
         self.buffers = (k_codes, k_scales, v_codes, v_scales)
         self.rows, self.kv_heads, self.head_dim, self.device = n, h, 2 * half, dev
-        self._c = _Cache(n, h, 2 * half, _plain("k_codes", k_codes, dev, u8, shape),
-                         _plain("k_scales", k_scales, dev, b16, scale_shape),
-                         _plain("v_codes", v_codes, dev, u8, shape),
-                         _plain("v_scales", v_scales, dev, b16, scale_shape))
+        self._c = _CACHE.pack(n, h, 2 * half, _plain("k_codes", k_codes, dev, u8, shape),
+                              _plain("k_scales", k_scales, dev, b16, scale_shape),
+                              _plain("v_codes", v_codes, dev, u8, shape),
+                              _plain("v_scales", v_scales, dev, b16, scale_shape))
 
 
 def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=None) -> None:
@@ -213,8 +206,8 @@ def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=
     torch = _first("k", k)
     n_src = k.shape[0]
     shape = (n_src, cache.kv_heads, cache.head_dim)
-    kr = _heads("k", k, cache.device, k.dtype, shape)
-    vr = _heads("v", v, cache.device, k.dtype, shape)
+    kr = _ROWS.pack(*_heads("k", k, cache.device, k.dtype, shape))
+    vr = _ROWS.pack(*_heads("v", v, cache.device, k.dtype, shape))
     n, idx = n_src, None
     if src_rows is not None:
         n = src_rows.shape[0] if isinstance(src_rows, torch.Tensor) and src_rows.dim() == 1 else -1
@@ -237,10 +230,12 @@ def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=
         raise IrodoriError(2, f"Shape mismatch: {n} rows from {row_start} of a cache of {cache.rows}")
     handle, side = _stream(stream, cache.device)
     shape = (n, cache.kv_heads, cache.head_dim)
-    k, v = _empty(side, shape, dtype, cache.device), _empty(side, shape, dtype, cache.device)
+    k = _empty(side, shape, dtype, cache.device)
+    v = _empty_like(side, k)
     row = cache.kv_heads * cache.head_dim
     _check(lib().irt_kv4_read(cache.device, _dtype_code[dtype], cache._c, row_start, n,
-                              _Rows(k.data_ptr(), row, cache.head_dim), _Rows(v.data_ptr(), row, cache.head_dim), handle))
+                              _ROWS.pack(k.data_ptr(), row, cache.head_dim),
+                              _ROWS.pack(v.data_ptr(), row, cache.head_dim), handle))
     _keep(side, *cache.buffers)
     return k, v
 
@@ -252,26 +247,24 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
     dev, dtype = q.get_device(), q.dtype
     handle, side = _stream(stream, dev)
     if out is None:
-        out = _empty(side, shape, dtype, dev)
-        out_rows = _Rows(out.data_ptr(), h * d, d)
-    else:
-        out_rows = _heads("out", out, dev, dtype, shape)
+        out = _empty_like(side, q)
+    out_p, out_row, out_head = _heads("out", out, dev, dtype, shape)
     lse = _empty(side, (n, h), torch.float32, dev) if return_lse else None
     if seqs is None:
-        nseq, tab = (n // max_q_len if max_q_len > 0 else 0), None
+        nseq, tab = (n // max_q_len if max_q_len > 0 else 0), 0
         if nseq * max_q_len != n or nseq * max_k_len != k_rows:
             raise IrodoriError(2, f"Shape mismatch: without a table {n} query rows and {k_rows} context rows must be "
                                   f"the same number of sequences of {max_q_len} and {max_k_len}")
     else:
         nseq = seqs.shape[0] if isinstance(seqs, torch.Tensor) and seqs.dim() == 2 else -1
         tab = _plain("seqs", seqs, dev, _INT32, (nseq, 4))
-    mask = None
+    mask = 0
     if key_mask is not None:
         mask = _plain("key_mask", key_mask, dev, _MASKS, (k_rows,))
-    a = _AttnArgs(dev, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
-                  d ** -0.5 if scale is None else scale, n, tab, _heads("q", q, dev, dtype, shape),
-                  _NO_ROWS if gate is None else _heads("gate", gate, dev, dtype, shape), out_rows, mask,
-                  None if lse is None else lse.data_ptr())
+    g = (0, 0, 0) if gate is None else _heads("gate", gate, dev, dtype, shape)
+    a = _ATTN.pack(dev, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
+                   d ** -0.5 if scale is None else scale, n, tab, *_heads("q", q, dev, dtype, shape), *g, out_p, out_row,
+                   out_head, mask, 0 if lse is None else lse.data_ptr())
     status = call(a, *context, handle)
     if status:
         _check(status)
@@ -303,7 +296,7 @@ def cross_attention(q, k, v, seqs, max_q_len: int, max_k_len: int, key_mask=None
     n = k.shape[0]
     shape = (n, k.shape[1], q.shape[2])
     dev = q.get_device()
-    context = (_heads("k", k, dev, q.dtype, shape), _heads("v", v, dev, q.dtype, shape), n)
+    context = (_ROWS.pack(*_heads("k", k, dev, q.dtype, shape)), _ROWS.pack(*_heads("v", v, dev, q.dtype, shape)), n)
     return _attention(lib().irt_cross_attention, q, shape[1], n, seqs, max_q_len, max_k_len, key_mask, gate, scale,
                       out, return_lse, stream, context, (k, v))
 
@@ -320,8 +313,8 @@ def kv4_attention(q, cache: Kv4Cache, seqs, max_q_len: int, max_k_len: int, k_se
     if cache.device != dev:
         raise IrodoriError(22, f"the cache must be on cuda:{dev}, got cuda:{cache.device}")
     shape = (q.shape[0], cache.kv_heads, q.shape[2])
-    kr = None if k_self is None else _heads("k_self", k_self, dev, q.dtype, shape)
-    vr = None if v_self is None else _heads("v_self", v_self, dev, q.dtype, shape)
+    kr = None if k_self is None else _ROWS.pack(*_heads("k_self", k_self, dev, q.dtype, shape))
+    vr = None if v_self is None else _ROWS.pack(*_heads("v_self", v_self, dev, q.dtype, shape))
     return _attention(lib().irt_kv4_attention, q, cache.kv_heads, cache.rows, seqs, max_q_len, max_k_len, key_mask,
                       gate, scale, out, return_lse, stream, (cache._c, kr, vr),
                       (k_self, v_self, *cache.buffers))

@@ -9,6 +9,26 @@ import pytest
 torch = pytest.importorskip("torch")
 
 
+class Rows(ctypes.Structure):  # irt_rows
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class AttnArgs(ctypes.Structure):  # irt_attn_args
+    _fields_ = [
+        ("device", ctypes.c_int32), ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("num_seqs", ctypes.c_int32), ("max_q_len", ctypes.c_int32),
+        ("max_k_len", ctypes.c_int32), ("scale", ctypes.c_float), ("q_rows", ctypes.c_int64),
+        ("seqs", ctypes.c_void_p), ("q", Rows), ("gate", Rows), ("out", Rows), ("key_mask", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+class Cache(ctypes.Structure):  # irt_kv4_cache
+    _fields_ = [("rows", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p)]
+
+
 @pytest.fixture()
 def ops(pkg):
     if not pkg.LIB_PATH.exists():
@@ -20,9 +40,9 @@ def ops(pkg):
 
 def attn_args(o, **kw):
     """A valid call's arguments over made-up addresses (never read: each test breaks one of them)."""
-    a = o._AttnArgs(device=0, dtype=0, heads=4, kv_heads=2, head_dim=128, num_seqs=2, max_q_len=3, max_k_len=5,
-                    scale=0.1, q_rows=6, seqs=None, q=o._Rows(0x10000000, 512, 128), gate=o._Rows(),
-                    out=o._Rows(0x20000000, 512, 128), key_mask=None, lse=None)
+    a = AttnArgs(device=0, dtype=0, heads=4, kv_heads=2, head_dim=128, num_seqs=2, max_q_len=3, max_k_len=5,
+                    scale=0.1, q_rows=6, seqs=None, q=Rows(0x10000000, 512, 128), gate=Rows(),
+                    out=Rows(0x20000000, 512, 128), key_mask=None, lse=None)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -67,15 +87,15 @@ BAD = [
 
 @pytest.mark.parametrize("kw,kind,msg", BAD)
 def test_cross_attention_refusals_through_the_c_abi(pkg, ops, kw, kind, msg):
-    a = attn_args(ops, **{k: ops._Rows(*v) if isinstance(v, tuple) else v for k, v in kw.items()})
-    k, v = ops._Rows(*K), ops._Rows(*V)
+    a = attn_args(ops, **{k: Rows(*v) if isinstance(v, tuple) else v for k, v in kw.items()})
+    k, v = Rows(*K), Rows(*V)
     rc = pkg.lib().irt_cross_attention(ctypes.byref(a), ctypes.byref(k), ctypes.byref(v), 10, None)
     got, text = status(pkg, rc)
     assert got == kind and msg in text, (got, text)
 
 
 def cache_struct(ops, **kw):
-    c = ops._Cache(10, 2, 128, 0x50000000, 0x51000000, 0x52000000, 0x53000000)
+    c = Cache(10, 2, 128, 0x50000000, 0x51000000, 0x52000000, 0x53000000)
     for k, v in kw.items():
         setattr(c, k, v)
     return c
@@ -96,7 +116,7 @@ def test_kv4_attention_refusals_through_the_c_abi(pkg, ops, kw, kind, msg):
 
 
 def test_kv4_attention_needs_both_own_tensors(pkg, ops):
-    a, c, r = attn_args(ops), cache_struct(ops), ops._Rows(*K)
+    a, c, r = attn_args(ops), cache_struct(ops), Rows(*K)
     rc = pkg.lib().irt_kv4_attention(ctypes.byref(a), ctypes.byref(c), ctypes.byref(r), None, None)
     got, text = status(pkg, rc)
     assert got == "MissingInput" and "go together" in text
@@ -109,21 +129,30 @@ def test_kv4_attention_needs_both_own_tensors(pkg, ops):
     (0, 3, -1, "Shape", "source rows"),
 ])
 def test_kv4_append_refusals_through_the_c_abi(pkg, ops, start, n, src, kind, msg):
-    c, k, v = cache_struct(ops), ops._Rows(*K), ops._Rows(*V)
+    c, k, v = cache_struct(ops), Rows(*K), Rows(*V)
     rc = pkg.lib().irt_kv4_append(0, 0, ctypes.byref(c), start, n, ctypes.byref(k), ctypes.byref(v), src, None, None)
     got, text = status(pkg, rc)
     assert got == kind and msg in text, (got, text)
 
 
 def test_kv4_read_refuses_outputs_that_overlap(pkg, ops):
-    c, k, v = cache_struct(ops), ops._Rows(0x30000000, 128, 128), ops._Rows(*V)
+    c, k, v = cache_struct(ops), Rows(0x30000000, 128, 128), Rows(*V)
     rc = pkg.lib().irt_kv4_read(0, 0, ctypes.byref(c), 0, 5, ctypes.byref(k), ctypes.byref(v), None)
     got, text = status(pkg, rc)
     assert got == "Shape" and "overlap one another" in text
 
 
+def test_the_python_calls_pack_the_headers_structures(ops):
+    assert (ops._ROWS.size, ops._ATTN.size, ops._CACHE.size) == tuple(map(ctypes.sizeof, (Rows, AttnArgs, Cache)))
+    a = AttnArgs.from_buffer_copy(ops._ATTN.pack(*range(1, 9), 0.5, *range(10, 23)))
+    assert (a.device, a.max_k_len, a.scale, a.q_rows, a.seqs, a.q.data, a.q.head_stride, a.gate.data, a.out.data,
+            a.out.row_stride, a.key_mask, a.lse) == (1, 8, 0.5, 10, 11, 12, 14, 15, 18, 19, 21, 22)
+    c = Cache.from_buffer_copy(ops._CACHE.pack(*range(1, 8)))
+    assert (c.rows, c.kv_heads, c.head_dim, c.k_codes, c.v_scales) == (1, 2, 3, 4, 7)
+
+
 def test_null_arguments(pkg, ops):
-    L, a, r, c = pkg.lib(), attn_args(ops), ops._Rows(*K), cache_struct(ops)
+    L, a, r, c = pkg.lib(), attn_args(ops), Rows(*K), cache_struct(ops)
     assert L.irt_cross_attention(None, ctypes.byref(r), ctypes.byref(r), 10, None) == 22
     assert L.irt_cross_attention(ctypes.byref(a), None, ctypes.byref(r), 10, None) == 22
     assert L.irt_kv4_attention(ctypes.byref(a), None, None, None, None) == 22
