@@ -147,13 +147,6 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
   merge_partials<BF, R, ROW_WARPS>(p, sd, split, rank, hk, row0, sm, a.out_vec);
 }
 
-int device_sms() {
-  int dev = 0, n = 0;
-  IRT_CUDA(cudaGetDevice(&dev));
-  IRT_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-  return n;
-}
-
 template <bool BF, bool CTX4, int R, int U>
 void launch_rows(const CtxAttnParams& p, cudaStream_t s) {
   RowArgs a{};

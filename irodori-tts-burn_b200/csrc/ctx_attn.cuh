@@ -105,6 +105,28 @@ __device__ __forceinline__ void kv4_unpack8(uint32_t w, uint16_t sb, float (&x)[
   }
 }
 
+// SMs of the current device, looked up once per device.
+inline int device_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  IRT_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  IRT_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+// Lets a kernel use `bytes` of dynamic shared memory on the current device;
+// `done` is the kernel's own mask of the devices it has been told on.
+template <class K>
+void allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  IRT_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit & done.load(std::memory_order_relaxed)) return;
+  IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 // Four values of a row of the output (or gate).
 template <bool BF>
 __device__ __forceinline__ float4 load4(const void* base, long off, bool vec) {

@@ -468,9 +468,7 @@ void launch(void (*kernel)(Kv4RowArgs), const CtxAttnParams& p, cudaStream_t s) 
   a.p = p;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.out_vec = rows_vec(p.out, 1) && (!p.gate.data || rows_vec(p.gate, 1));
-  int dev = 0, sms = 0;
-  IRT_CUDA(cudaGetDevice(&dev));
-  IRT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int sms = device_sms();
   const long blocks = ((long)p.max_q * p.G + R - 1) / R;
   const long ctas = blocks * p.Hkv * p.nseq;
   // Keys are split over a cluster up to four times the two CTAs an SM holds,
@@ -479,7 +477,8 @@ void launch(void (*kernel)(Kv4RowArgs), const CtxAttnParams& p, cudaStream_t s) 
   // frame over 576 rows: 9.1 / 8.2 / 6.8 / 7.4 us at 1 / 2 / 4 / 8).
   a.split = 1;
   while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 8L * sms && p.max_k >= (long)a.split * WARPS * KEYS) a.split *= 2;
-  IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> told{0};
+  allow_smem(kernel, smem, told);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
   cfg.blockDim = dim3(32 * WARPS);

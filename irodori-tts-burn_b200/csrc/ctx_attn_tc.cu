@@ -62,7 +62,7 @@ struct Cfg {
 struct TcArgs {
   CtxAttnParams p;
   float scale_log2;
-  int Gp;     // heads packed into a query tile
+  int log_gp; // heads packed into a query tile, a power of two
   int split;  // CTAs of the cluster
 };
 
@@ -115,16 +115,23 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
                        const __grid_constant__ TcArgs a) {
   using C = Cfg<HDT, CTX4>;
+  if (threadIdx.x == 128) {  // the TMA thread's first descriptors, while the predecessor may still run
+    prefetch_map(&tmQ);
+    if (!CTX4) {
+      prefetch_map(&tmK);
+      prefetch_map(&tmV);
+    }
+  }
   pdl_wait();
   pdl_trigger();
   const CtxAttnParams& p = a.p;
   irt_attn_seq sd;
   if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
-  const int split = a.split, rank = blockIdx.x % split, Gp = a.Gp;
-  const int q0 = (blockIdx.x / split) * (QT / Gp);  // first query of the tile
+  const int split = a.split, rank = blockIdx.x % split, lg = a.log_gp, gmask = (1 << lg) - 1;
+  const int q0 = (blockIdx.x / split) * (QT >> lg);  // first query of the tile
   if (q0 >= sd.q_len) return;                       // the whole cluster
-  const int head0 = blockIdx.y * Gp, hk = head0 / p.G;
-  const int rows = min(QT, (sd.q_len - q0) * Gp);  // packed query rows of the tile
+  const int head0 = blockIdx.y << lg, hk = head0 / p.G;
+  const int rows = min(QT, (sd.q_len - q0) << lg);  // packed query rows of the tile
   const int n_self = p.ks.data ? (sd.q_len + KT - 1) / KT : 0;
   const int n_all = n_self + (sd.k_len + KT - 1) / KT;
   const int t0 = (int)((long)n_all * rank / split), nt = (int)((long)n_all * (rank + 1) / split) - t0;
@@ -145,7 +152,38 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sm_warps = (rows + 31) / 32;  // softmax warps that have a query row
-  if (threadIdx.x == 0) {
+  const uint32_t sQ = smem_u32(sm);
+  auto sK = [&](int s) { return smem_u32(sm + C::OFF_K + s * C::TILE); };
+  auto sV = [&](int s) { return smem_u32(sm + C::OFF_V + s * C::TILE); };
+  // first row and valid keys of local tile j
+  auto row_of = [&](int j) {
+    const int t = t0 + j;
+    return t < n_self ? sd.q_start + t * KT : sd.k_start + (t - n_self) * KT;
+  };
+  auto keys_of = [&](int j) {
+    const int t = t0 + j;
+    return min(KT, t < n_self ? sd.q_len - t * KT : sd.k_len - (t - n_self) * KT);
+  };
+
+  // K (V) rows of local tile j, by the TMA thread
+  auto load = [&](int j, uint32_t full, uint32_t empty, uint32_t dst, const CUtensorMap* self, const CUtensorMap* ctx) {
+    mbar_wait(empty, ((j / NKV) & 1) ^ 1);
+    const bool own = t0 + j < n_self;
+    if (CTX4 && !own) {  // the code warps fill this one
+      mbar_arrive(full);
+      return;
+    }
+    mbar_expect_tx(full, C::TILE);
+    const CUtensorMap* m = own ? self : ctx;
+#pragma unroll
+    for (int h = 0; h < HDT / 64; ++h) tma_load_3d(dst + h * C::HALF, m, full, 64 * h, hk, row_of(j));
+  };
+  auto load_k = [&](int j) { load(j, K_FULL(j % NKV), K_EMPTY(j % NKV), sK(j % NKV), &tmKS, &tmK); };
+  auto load_v = [&](int j) { load(j, V_FULL(j % NKV), V_EMPTY(j % NKV), sV(j % NKV), &tmVS, &tmV); };
+
+  // The TMA thread sets up the barriers and starts the first loads; TMEM is
+  // allocated meanwhile.
+  if (threadIdx.x == 128) {
     mbar_init(Q_FULL, 1);
     mbar_init(O_DONE, 1);
     mbar_init(O_FINAL, 1);
@@ -161,52 +199,31 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       mbar_init(P_FULL(b), sm_warps);
     }
     mbar_fence_init();
+    fence_proxy_async();
+    if (nt > 0) {
+      mbar_expect_tx(Q_FULL, C::Q_BYTES);
+#pragma unroll
+      for (int h = 0; h < HDT / 64; ++h) tma_load_3d(sQ + h * C::Q_HALF, &tmQ, Q_FULL, 64 * h, head0, sd.q_start + q0);
+      load_k(0);
+      if (nt > 1) load_k(1);
+      load_v(0);
+    }
   }
+  __syncwarp();
   if (warp == 5) tmem_alloc(smem_u32(tmem_slot), C::TM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t sQ = smem_u32(sm);
-  auto sK = [&](int s) { return smem_u32(sm + C::OFF_K + s * C::TILE); };
-  auto sV = [&](int s) { return smem_u32(sm + C::OFF_V + s * C::TILE); };
-  // first row and valid keys of local tile j
-  auto row_of = [&](int j) {
-    const int t = t0 + j;
-    return t < n_self ? sd.q_start + t * KT : sd.k_start + (t - n_self) * KT;
-  };
-  auto keys_of = [&](int j) {
-    const int t = t0 + j;
-    return min(KT, t < n_self ? sd.q_len - t * KT : sd.k_len - (t - n_self) * KT);
-  };
 
   float m_run = -INFINITY, l_run = 0.f;
   if (nt > 0) {
     if (warp == 4) {
       // ---------------- TMA ----------------
       if (lane == 0) {
-        mbar_expect_tx(Q_FULL, C::Q_BYTES);
-#pragma unroll
-        for (int h = 0; h < HDT / 64; ++h) tma_load_3d(sQ + h * C::Q_HALF, &tmQ, Q_FULL, 64 * h, head0, sd.q_start + q0);
-        auto load = [&](int j, uint32_t full, uint32_t empty, uint32_t dst, const CUtensorMap* self, const CUtensorMap* ctx) {
-          mbar_wait(empty, ((j / NKV) & 1) ^ 1);
-          const bool own = t0 + j < n_self;
-          if (CTX4 && !own) {  // the code warps fill this one
-            mbar_arrive(full);
-            return;
-          }
-          mbar_expect_tx(full, C::TILE);
-          const CUtensorMap* m = own ? self : ctx;
-#pragma unroll
-          for (int h = 0; h < HDT / 64; ++h) tma_load_3d(dst + h * C::HALF, m, full, 64 * h, hk, row_of(j));
-        };
-        auto load_k = [&](int j) { load(j, K_FULL(j % NKV), K_EMPTY(j % NKV), sK(j % NKV), &tmKS, &tmK); };
-        auto load_v = [&](int j) { load(j, V_FULL(j % NKV), V_EMPTY(j % NKV), sV(j % NKV), &tmVS, &tmV); };
-        load_k(0);
-        if (nt > 1) load_k(1);
-        for (int j = 0; j < nt; ++j) {
-          load_v(j);
+        for (int j = 0; j + 1 < nt; ++j) {  // K two tiles ahead of V, as the products are issued
           if (j + 2 < nt) load_k(j + 2);
+          load_v(j + 1);
         }
         if (split == 1 && p.gate.data) {  // the gate takes Q's place once the last scores are done
           mbar_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1);
@@ -331,6 +348,16 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     } else if (warp < sm_warps) {
       // ---------------- softmax ----------------
       const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
+      // mask bytes of keys lane and lane + 32 of a tile, read a tile ahead
+      uint8_t next0 = 1, next1 = 1;
+      auto fetch_mask = [&](int j) {
+        if (!p.mask || j >= nt || t0 + j < n_self) return;
+        const uint8_t* mk = p.mask + row_of(j) + lane;
+        const int n = keys_of(j) - lane;
+        next0 = n > 0 ? mk[0] : 0;
+        next1 = n > 32 ? mk[32] : 0;
+      };
+      fetch_mask(0);
       for (int j = 0; j < nt; ++j) {
         const int b = j & 1;
         const bool own = t0 + j < n_self;
@@ -339,10 +366,10 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         uint32_t on0 = nkeys >= 32 ? 0xffffffffu : (1u << nkeys) - 1;
         uint32_t on1 = nkeys >= 64 ? 0xffffffffu : nkeys > 32 ? (1u << (nkeys - 32)) - 1 : 0u;
         if (p.mask && !own) {
-          const uint8_t* mk = p.mask + row_of(j);
-          on0 &= __ballot_sync(0xffffffffu, lane < nkeys && mk[lane]);
-          on1 &= __ballot_sync(0xffffffffu, lane + 32 < nkeys && mk[lane + 32]);
+          on0 &= __ballot_sync(0xffffffffu, next0);
+          on1 &= __ballot_sync(0xffffffffu, next1);
         }
+        fetch_mask(j + 1);
         const bool partial = (on0 & on1) != 0xffffffffu;
         mbar_wait(S_FULL(b), (j >> 1) & 1);
         tc_fence_after();
@@ -482,7 +509,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         }
       }
       if (qrow < rows && p.lse)
-        p.lse[((long)sd.q_start + q0 + qrow / Gp) * p.H + head0 + qrow % Gp] =
+        p.lse[((long)sd.q_start + q0 + (qrow >> lg)) * p.H + head0 + (qrow & gmask)] =
             l_run == 0.f ? -INFINITY : fmaf(m_run, LN2, logf(l_run));
       __syncwarp();
       constexpr int LPR = HDT / 8;  // lanes of a row
@@ -495,8 +522,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
           if (row >= rows) break;
           uint32_t v[4];
           ld_shared16(sQ + (chunk >> 3) * C::Q_HALF + row * 128 + (((chunk & 7) ^ (row & 7)) << 4), v);
-          *reinterpret_cast<uint4*>(out + ((long)sd.q_start + q0 + row / Gp) * p.out.row_stride +
-                                    (head0 + row % Gp) * p.out.head_stride) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(out + ((long)sd.q_start + q0 + (row >> lg)) * p.out.row_stride +
+                                    (head0 + (row & gmask)) * p.out.head_stride) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
     }
@@ -547,8 +574,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       }
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
       x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
-      const long row = (long)sd.q_start + q0 + r / Gp;
-      const int head = head0 + r % Gp;
+      const long row = (long)sd.q_start + q0 + (r >> lg);
+      const int head = head0 + (r & gmask);
       if (p.gate.data) {
         const uint2 g = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(p.gate.data) +
                                                         row * p.gate.row_stride + head * p.gate.head_stride + d);
@@ -591,31 +618,31 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
   TcArgs a{};
   a.p = p;
   a.scale_log2 = p.scale * 1.4426950408889634f;
-  a.Gp = QT % p.G == 0 ? p.G : 1;
+  const int gp = QT % p.G == 0 ? p.G : 1;
+  while ((1 << a.log_gp) < gp) ++a.log_gp;
   CUtensorMap q, ks, vs, k, v, g;
-  if (!rows_map(q, p.q, p.q_rows, p.H, p.hd, a.Gp, QT / a.Gp)) return false;
+  if (!rows_map(q, p.q, p.q_rows, p.H, p.hd, gp, QT / gp)) return false;
   ks = vs = k = v = g = q;
-  if (p.gate.data && !rows_map(g, p.gate, p.q_rows, p.H, p.hd, a.Gp, QT / a.Gp)) return false;
+  if (p.gate.data && !rows_map(g, p.gate, p.q_rows, p.H, p.hd, gp, QT / gp)) return false;
   if (p.ks.data && (!rows_map(ks, p.ks, p.q_rows, p.Hkv, p.hd, 1, KT) ||
                     !rows_map(vs, p.vs, p.q_rows, p.Hkv, p.hd, 1, KT)))
     return false;
   if (p.k.data && p.k_rows > 0 &&
       (!rows_map(k, p.k, p.k_rows, p.Hkv, p.hd, 1, KT) || !rows_map(v, p.v, p.k_rows, p.Hkv, p.hd, 1, KT)))
     return false;
-  int dev = 0, sms = 0;
-  IRT_CUDA(cudaGetDevice(&dev));
-  IRT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const long qtiles = ((long)p.max_q * a.Gp + QT - 1) / QT;
-  const long ctas = qtiles * (p.H / a.Gp) * p.nseq;
+  const int sms = device_sms();
+  const long qtiles = ((long)p.max_q * gp + QT - 1) / QT;
+  const long ctas = qtiles * (p.H / gp) * p.nseq;
   const long ktiles = (p.max_k + KT - 1L) / KT + (p.ks.data ? (p.max_q + KT - 1L) / KT : 0);
   // Key tiles are shared by a cluster while half the CTA slots (two per SM)
   // would stay empty.
   a.split = 1;
   while (a.split < 8 && ctas * a.split * 2 <= 2L * sms && a.split * 2 <= ktiles) a.split *= 2;
   auto kernel = ctx_attn_tc_kernel<HDT, CTX4>;
-  IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+  static std::atomic<uint64_t> told{0};
+  allow_smem(kernel, C::SMEM, told);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(qtiles * a.split), p.H / a.Gp, p.nseq);
+  cfg.gridDim = dim3((unsigned)(qtiles * a.split), p.H / gp, p.nseq);
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;

@@ -337,9 +337,7 @@ void launch(const CtxAttnParams& p, cudaStream_t s) {
   a.ks_vec = rows_vec(p.ks, BF);
   a.vs_vec = rows_vec(p.vs, BF);
   a.out_vec = rows_vec(p.out, BF) && (!p.gate.data || rows_vec(p.gate, BF));
-  int dev = 0, sms = 0;
-  IRT_CUDA(cudaGetDevice(&dev));
-  IRT_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int sms = device_sms();
   const long blocks = ((long)p.max_q * p.G + QT - 1) / QT;
   const long ctas = blocks * p.Hkv * p.nseq;
   const long ktiles = (p.max_k + KT - 1L) / KT + (p.ks.data ? (p.max_q + KT - 1L) / KT : 0);
@@ -347,7 +345,8 @@ void launch(const CtxAttnParams& p, cudaStream_t s) {
   while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 2L * sms && a.split * 2 <= ktiles) a.split *= 2;
   constexpr size_t smem = Smem<HDT>::FLOATS * sizeof(float);
   auto kernel = ctx_attn_tile_kernel<BF, CTX4, HDT>;
-  IRT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> told{0};
+  allow_smem(kernel, smem, told);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
   cfg.blockDim = dim3(THREADS);
