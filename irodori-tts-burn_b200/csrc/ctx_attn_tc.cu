@@ -2,7 +2,7 @@
 //
 // One CTA = one (sequence, head group, tile of 128 packed query rows); with
 // grouped heads the rows of a tile are query x head of the group (row r =
-// query r / Gp, head r % Gp), so the group's K and V are read once.  Two CTAs
+// query r / Gp, head r % Gp; Gp a power of two), so the group's K and V are read once.  Two CTAs
 // share an SM.  Key tiles of 64: a sequence's own rows first, then its context
 // rows.  Warps:
 //   0..3  softmax: thread = query row.  Per tile: scores from TMEM, masked
@@ -56,7 +56,7 @@ struct Cfg {
   static constexpr uint32_t FULL_COUNT = 1 + CODE_WARPS / 2;
   // cluster merge: f32 O rows (padded against bank conflicts), m and l
   static constexpr int OLD = HDT + 4;
-  static_assert((uint32_t)QT * OLD * 4 + 2 * QT * 4 <= OFF_BAR, "merge buffers fit the tiles");
+  static_assert((uint32_t)QT * (OLD + 2 + MAX_SPLIT) * 4 <= OFF_BAR, "merge buffers fit the tiles");
 };
 
 struct TcArgs {
@@ -554,39 +554,59 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     cg::cluster_group cluster = cg::this_cluster();
     __syncwarp();
     cluster.sync();
-    const int per_row = p.hd / 4;
-    for (int e = threadIdx.x; e < ((rows - rank + split - 1) / split) * per_row; e += C::THREADS) {
-      const int r = (e / per_row) * split + rank, d = (e % per_row) * 4;  // rows dealt out to the CTAs
-      float mt = -INFINITY;
-      for (int c = 0; c < split; ++c) mt = fmaxf(mt, cluster.map_shared_rank(sml, c)[r]);
+    // weights of the CTAs' states for the rows dealt out to this one
+    float* wt = sml + 2 * QT;  // [row of this CTA][MAX_SPLIT]
+    const int mine = (rows - rank + split - 1) / split;
+    for (int i = threadIdx.x; i < mine; i += C::THREADS) {
+      const int r = i * split + rank;
+      float m[MAX_SPLIT], l[MAX_SPLIT], mt = -INFINITY, lt = 0.f;
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c)
+        if (c < split) {
+          const float* o = cluster.map_shared_rank(sml, c);
+          m[c] = o[r];
+          l[c] = o[QT + r];
+          mt = fmaxf(mt, m[c]);
+        }
       const float base = mt == -INFINITY ? 0.f : mt;
-      float lt = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = 0; c < split; ++c) {
-        const float* om = cluster.map_shared_rank(sml, c);
-        const float f = ex2(om[r] - base);
-        const float4 o = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, c) + r * C::OLD + d);
-        lt = fmaf(om[QT + r], f, lt);
-        x.x = fmaf(o.x, f, x.x);
-        x.y = fmaf(o.y, f, x.y);
-        x.z = fmaf(o.z, f, x.z);
-        x.w = fmaf(o.w, f, x.w);
-      }
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c)
+        if (c < split) {
+          m[c] = ex2(m[c] - base);
+          lt = fmaf(l[c], m[c], lt);
+        }
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
-      x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c)
+        if (c < split) wt[i * MAX_SPLIT + c] = m[c] * inv;
+      if (p.lse)
+        p.lse[((long)sd.q_start + q0 + (r >> lg)) * p.H + head0 + (r & gmask)] =
+            lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
+    }
+    __syncthreads();
+    const int per_row = p.hd / 4;
+    for (int e = threadIdx.x; e < mine * per_row; e += C::THREADS) {
+      const int i = e / per_row, d = (e - i * per_row) * 4, r = i * split + rank;
+      float4 o[MAX_SPLIT], x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c)
+        if (c < split) o[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, c) + r * C::OLD + d);
+#pragma unroll
+      for (int c = 0; c < MAX_SPLIT; ++c)
+        if (c < split) {
+          const float f = wt[i * MAX_SPLIT + c];
+          x.x = fmaf(o[c].x, f, x.x);
+          x.y = fmaf(o[c].y, f, x.y);
+          x.z = fmaf(o[c].z, f, x.z);
+          x.w = fmaf(o[c].w, f, x.w);
+        }
       const long row = (long)sd.q_start + q0 + (r >> lg);
       const int head = head0 + (r & gmask);
       if (p.gate.data) {
-        const uint2 g = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(p.gate.data) +
-                                                        row * p.gate.row_stride + head * p.gate.head_stride + d);
-        x.x *= __uint_as_float(g.x << 16);
-        x.y *= __uint_as_float(g.x & 0xffff0000u);
-        x.z *= __uint_as_float(g.y << 16);
-        x.w *= __uint_as_float(g.y & 0xffff0000u);
+        const float4 g = load4<true>(p.gate.data, row * p.gate.row_stride + head * p.gate.head_stride + d, true);
+        x.x *= g.x; x.y *= g.y; x.z *= g.z; x.w *= g.w;
       }
-      *reinterpret_cast<uint2*>(static_cast<bf16*>(p.out.data) + row * p.out.row_stride + head * p.out.head_stride +
-                                d) = make_uint2(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w));
-      if (p.lse && d == 0) p.lse[row * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
+      store4<true>(p.out.data, row * p.out.row_stride + head * p.out.head_stride + d, true, x);
     }
     __syncwarp();
     cluster.sync();  // the others may still read this CTA's part
@@ -634,10 +654,22 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
   const long qtiles = ((long)p.max_q * gp + QT - 1) / QT;
   const long ctas = qtiles * (p.H / gp) * p.nseq;
   const long ktiles = (p.max_k + KT - 1L) / KT + (p.ks.data ? (p.max_q + KT - 1L) / KT : 0);
-  // Key tiles are shared by a cluster while half the CTA slots (two per SM)
-  // would stay empty.
-  a.split = 1;
-  while (a.split < 8 && ctas * a.split * 2 <= 2L * sms && a.split * 2 <= ktiles) a.split *= 2;
+  // Key tiles are shared by a cluster where that pays: the least of
+  //   5 + 0.82 (tiles of a CTA) (1.6 where CTAs share SMs) + 1 + 2.2 rows / 128
+  // microseconds, the last two for the merge; at most two CTAs per SM.  One
+  // sequence of 16 heads, 1 / 2 / 4 / 8 CTAs: 1 query over 576 keys 11.3 / 9.3
+  // / 8.1 / 7.9 us; 128 over 2048 31.4 / 21.9 / 14.8 / 14.3; 750 over 576 13.2
+  // / 16.1 / 22.9 / 36.3; 750 over 2048 32.5 / 26.8 / 32.3 / 44.8.
+  const float rows = (float)std::min(128L, (long)p.max_q * gp);
+  float best = 0.f;
+  for (int n = 1; n <= MAX_SPLIT && (n == 1 || (ctas * n <= 2L * sms && n <= ktiles)); n *= 2) {
+    const float share = ctas * n > sms ? 1.6f : 1.f;
+    const float t = 5.f + 0.82f * ((ktiles + n - 1) / n) * share + (n > 1 ? 1.f + 2.2f / 128.f * rows : 0.f);
+    if (n == 1 || t < best) {
+      best = t;
+      a.split = n;
+    }
+  }
   auto kernel = ctx_attn_tc_kernel<HDT, CTX4>;
   static std::atomic<uint64_t> told{0};
   allow_smem(kernel, C::SMEM, told);
