@@ -166,6 +166,16 @@ IRT_API int irt_engine_destroy(irt_engine* e);
 /* with_sampling(params) (src/inference.rs:151-155, :166-172, :231-233):
  * validates and stores the parameters; Loaded/Ready -> Ready. */
 IRT_API int irt_engine_set_sampling(irt_engine* e, const irt_sampler_params* p);
+/* Extension of the reference's context K/V cache (src/model/attention.rs:431-501):
+ * how the engine keeps a request's text and speaker / caption K and V.
+ * IRT_CTX_CACHE_NATIVE (default): in the engine's precision.
+ * IRT_CTX_CACHE_4BIT: in 4.5 bits a value (irt_kv4_cache), 0.28 of the bf16
+ * bytes, projected and quantised a layer at a time; for batches whose context
+ * rows bound the utterances in flight.  The context's values are rounded
+ * (relative error about 0.1 each), the latents change accordingly.  Takes
+ * effect with the next irt_engine_sample. */
+typedef enum irt_ctx_cache { IRT_CTX_CACHE_NATIVE = 0, IRT_CTX_CACHE_4BIT = 1 } irt_ctx_cache;
+IRT_API int irt_engine_set_context_cache(irt_engine* e, int mode);
 /* with_default_sampling() (src/inference.rs:158-164). */
 IRT_API int irt_engine_set_default_sampling(irt_engine* e);
 /* sampling_params() (src/inference.rs:240-243). IRT_E_STATE before set_sampling. */

@@ -38,6 +38,7 @@ STATUS_NAMES = {
 PREC = {"bf16": 0, "f32": 1}
 METHODS = {"euler": 0, "heun": 1, "plms4": 2}
 MODES = {"independent": 0, "joint": 1, "alternating": 2}
+CTX_CACHES = {"native": 0, "4bit": 1}
 MEM_HOST, MEM_DEVICE = 0, 1
 
 
@@ -102,6 +103,7 @@ _SIGNATURES = {
                                                       ctypes.POINTER(ctypes.c_void_p)]),
     "irt_engine_destroy": (ctypes.c_int, [ctypes.c_void_p]),
     "irt_engine_set_sampling": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_Params)]),
+    "irt_engine_set_context_cache": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int]),
     "irt_engine_set_default_sampling": (ctypes.c_int, [ctypes.c_void_p]),
     "irt_engine_get_sampling": (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(_Params)]),
     "irt_engine_get_config": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t,
@@ -386,8 +388,19 @@ class ReadyBuilder:
         _check(lib().irt_engine_set_sampling(self._h.h, ctypes.byref(p)))
         return self
 
+    def with_context_cache(self, mode: str) -> "ReadyBuilder":
+        """``InferenceEngine.with_context_cache``."""
+        _set_context_cache(self._h, mode)
+        return self
+
     def build(self) -> "InferenceEngine":
         return InferenceEngine(self._h, self._device, self._precision)
+
+
+def _set_context_cache(h: _Handle, mode: str) -> None:
+    if mode not in CTX_CACHES:
+        raise IrodoriError(22, f"unknown context cache {mode!r}; expected native or 4bit")
+    _check(lib().irt_engine_set_context_cache(h.h, CTX_CACHES[mode]))
 
 
 def _engine_config(h: _Handle) -> dict:
@@ -432,6 +445,13 @@ class InferenceEngine:
     def with_sampling(self, params: SamplerParams) -> "InferenceEngine":
         p = params._to_c()
         _check(lib().irt_engine_set_sampling(self._h.h, ctypes.byref(p)))
+        return self
+
+    def with_context_cache(self, mode: str) -> "InferenceEngine":
+        """How a request's text and speaker / caption K and V are kept
+        (``irt_engine_set_context_cache``): "native", in the engine's precision,
+        or "4bit", in 0.28 of the bf16 bytes with rounded values."""
+        _set_context_cache(self._h, mode)
         return self
 
     def last_stats(self):

@@ -111,6 +111,18 @@ int irt_engine_set_sampling(irt_engine* e, const irt_sampler_params* p) {
   });
 }
 
+int irt_engine_set_context_cache(irt_engine* e, int mode) {
+  return guard([&] {
+    need(e, "engine");
+    if (mode != IRT_CTX_CACHE_NATIVE && mode != IRT_CTX_CACHE_4BIT)
+      throw irt::Error(IRT_E_INVALID_ARG, "mode must be an irt_ctx_cache");
+    std::lock_guard<std::mutex> lk(e->e->mu);
+    if (mode == IRT_CTX_CACHE_4BIT && (e->e->hd % 8 || e->e->hd > 256))
+      throw irt::unsupported("the 4-bit context cache needs a head_dim that is a multiple of 8, at most 256");
+    e->e->ctx_cache = mode;
+  });
+}
+
 int irt_engine_set_default_sampling(irt_engine* e) {
   irt_sampler_params p;
   irt_sampler_params_default(&p);

@@ -1,6 +1,7 @@
 // Engine implementation: checkpoint upload + packing, condition encoders,
 // context KV cache, precomputed adaLN tables, DiT forward and the RF sampler.
 #include "engine.hpp"
+#include "ctx_attn.hpp"
 #include "lora.hpp"
 
 #include <algorithm>
@@ -367,27 +368,29 @@ void Engine::load(const std::string& path, const std::string& adapter_dir) {
 // GEMM dispatch: tcgen05 kernel for bf16 operands when the shape allows it,
 // else the SIMT kernel + standalone epilogue.
 // ---------------------------------------------------------------------------
-void Engine::gemm(const void* A, long lda, const DevBuf& W, int M, int N, int K, EpiParams p, cudaStream_t s) {
+void Engine::gemm(const void* A, long lda, const DevBuf& W, int M, int N, int K, EpiParams p, cudaStream_t s,
+                  long w_row0) {
   p.M = M;
   p.N = N;
   if (M <= 0 || N <= 0) return;
-  if (bf && gemm_tc_supported(p, K, lda, K, A, W.p)) {
-    gemm_tc(reinterpret_cast<const bf16*>(A), lda, W.as<bf16>(), K, M, N, K, p, s);
+  const void* w = W.as<uint8_t>() + (size_t)w_row0 * K * esz();
+  if (bf && gemm_tc_supported(p, K, lda, K, A, w)) {
+    gemm_tc(reinterpret_cast<const bf16*>(A), lda, static_cast<const bf16*>(w), K, M, N, K, p, s);
     return;
   }
   if (tf32) {
     const auto it = w_tf32.find(W.p);
     const int Kp = tf32_kpad(K);
     if (it != w_tf32.end() && (lda % 4) == 0 && (reinterpret_cast<uintptr_t>(A) & 15) == 0 &&
-        gemm_tc_supported(p, Kp, 2L * Kp, 2L * Kp, A, it->second.p)) {
+        gemm_tc_supported(p, Kp, 2L * Kp, 2L * Kp, A, it->second.as<float>() + w_row0 * 2 * Kp)) {
       ws.a2.ensure((size_t)M * 2 * Kp * 4);
       split_tf32(static_cast<const float*>(A), lda, M, K, ws.a2.as<float>(), Kp, s);
-      gemm_tc_tf32x3(ws.a2.as<float>(), 2L * Kp, it->second.as<float>(), 2L * Kp, M, N, Kp, p, s);
+      gemm_tc_tf32x3(ws.a2.as<float>(), 2L * Kp, it->second.as<float>() + w_row0 * 2 * Kp, 2L * Kp, M, N, Kp, p, s);
       return;
     }
   }
   ws.raw.ensure((size_t)M * N * 4);
-  gemm_simt(A, bf, lda, 0, W.p, bf, K, 0, ws.raw.as<float>(), N, 0, M, N, K, 1, s);
+  gemm_simt(A, bf, lda, 0, w, bf, K, 0, ws.raw.as<float>(), N, 0, M, N, K, 1, s);
   epilogue_apply(p, ws.raw.as<float>(), N, 0, 1, s);
 }
 
@@ -492,14 +495,14 @@ void Engine::run_encoder(EncoderW& e, int B, int T, const void* input, bool from
 // One DiT forward over M packed rows (src/model/dit/model.rs:354-393):
 // input ws.xin [M, P] (operand type), output ws.vout [M, P] f32.
 // ---------------------------------------------------------------------------
-void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, int t_index, int nrows_ctx,
-                          cudaStream_t s) {
+void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, int max_ctx, int t_index,
+                          int nrows_ctx, cudaStream_t s) {
   const size_t ada_bytes = (size_t)L * 6 * D * 4;
   ada_cur.ensure(ada_bytes);
   IRT_CUDA(cudaMemcpyAsync(ada_cur.p, ws.ada.as<uint8_t>() + (size_t)t_index * ada_bytes, ada_bytes,
                            cudaMemcpyDeviceToDevice, s));
   if (!use_graphs || dump_layers) {
-    dit_forward(M, d_seqs, nseq, max_len, ada_cur.as<float>(), nrows_ctx, s);
+    dit_forward(M, d_seqs, nseq, max_len, max_ctx, ada_cur.as<float>(), nrows_ctx, s);
     return;
   }
   std::vector<uintptr_t> key = {
@@ -507,14 +510,15 @@ void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, i
       (uintptr_t)ws.x.p, (uintptr_t)ws.h.p, (uintptr_t)ws.q.p, (uintptr_t)ws.k.p, (uintptr_t)ws.v.p,
       (uintptr_t)ws.g.p, (uintptr_t)ws.attn.p, (uintptr_t)ws.hm.p, (uintptr_t)ws.xin.p, (uintptr_t)ws.vout.p,
       (uintptr_t)ws.raw.p, (uintptr_t)ws.tokpos.p, (uintptr_t)ws.cache_k.p, (uintptr_t)ws.cache_v.p,
-      (uintptr_t)ws.rope_cos.p, (uintptr_t)ws.rope_sin.p, (uintptr_t)ada_cur.p, (uintptr_t)ws.a2.p};
+      (uintptr_t)ws.rope_cos.p, (uintptr_t)ws.rope_sin.p, (uintptr_t)ada_cur.p, (uintptr_t)ws.a2.p,
+      (uintptr_t)ctx_cache, (uintptr_t)(ctx_cache ? max_ctx : 0), (uintptr_t)ws.cache4.p};
   auto it = graphs.find(key);
   if (it == graphs.end()) {
     // keys seen once and never again (a server sees many ragged shapes) must
     // not accumulate: the table of first uses is bounded like the graphs
     if (graph_seen.size() > 256) graph_seen.clear();
     if (graph_seen[key]++ == 0) {  // first use: eager (allocations happen here)
-      dit_forward(M, d_seqs, nseq, max_len, ada_cur.as<float>(), nrows_ctx, s);
+      dit_forward(M, d_seqs, nseq, max_len, max_ctx, ada_cur.as<float>(), nrows_ctx, s);
       return;
     }
     cudaGraph_t g = nullptr;
@@ -522,7 +526,7 @@ void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, i
     const long long before = launch_counter().load();
     IRT_CUDA(cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal));
     try {
-      dit_forward(M, d_seqs, nseq, max_len, ada_cur.as<float>(), nrows_ctx, s);
+      dit_forward(M, d_seqs, nseq, max_len, max_ctx, ada_cur.as<float>(), nrows_ctx, s);
     } catch (...) {
       cudaStreamEndCapture(s, &g);
       if (g) cudaGraphDestroy(g);
@@ -547,8 +551,22 @@ void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, i
   launch_counter().fetch_add(graph_kernels[key]);
 }
 
-void Engine::dit_forward(int M, const SeqDesc* d_seqs, int nseq, int max_len, const float* ada_t, int nrows_ctx,
-                         cudaStream_t s) {
+size_t Engine::cache4_layer_bytes(long rows) const {
+  // codes, then scales, of K and of V; each part starts on a 256-byte border
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  return 2 * (up((size_t)H * rows * (hd / 2)) + up((size_t)H * rows * kv4_groups(hd) * 2));
+}
+
+irt_kv4_cache Engine::cache4_layer(int l, long rows) const {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  const size_t codes = up((size_t)H * rows * (hd / 2)), half = cache4_layer_bytes(rows) / 2;
+  uint8_t* p = ws.cache4.as<uint8_t>() + (size_t)l * 2 * half;
+  return {rows, H, hd, p, reinterpret_cast<uint16_t*>(p + codes), p + half,
+          reinterpret_cast<uint16_t*>(p + half + codes)};
+}
+
+void Engine::dit_forward(int M, const SeqDesc* d_seqs, int nseq, int max_len, int max_ctx, const float* ada_t,
+                         int nrows_ctx, cudaStream_t s) {
   const float eps = (float)cfg.norm_eps;
   float* x = ws.x.as<float>();
   {
@@ -591,7 +609,35 @@ void Engine::dit_forward(int M, const SeqDesc* d_seqs, int nseq, int max_len, co
     ap.out = ws.attn.p;
     ap.rows = M;
     ap.ctx_rows = nrows_ctx;
-    attention(ap, bf, s);
+    if (ctx_cache == IRT_CTX_CACHE_4BIT && nrows_ctx) {
+      static_assert(sizeof(SeqDesc) == sizeof(irt_attn_seq), "one table for both attentions");
+      const irt_kv4_cache c4 = cache4_layer(l, nrows_ctx);
+      CtxAttnParams cp{};
+      cp.bf16_io = bf;
+      cp.H = cp.Hkv = H;
+      cp.hd = hd;
+      cp.G = 1;
+      cp.nseq = nseq;
+      cp.max_q = max_len;
+      cp.max_k = max_ctx;
+      cp.scale = ap.scale;
+      cp.q_rows = M;
+      cp.k_rows = nrows_ctx;
+      cp.seqs = reinterpret_cast<const irt_attn_seq*>(d_seqs);
+      auto rows = [&](DevBuf& b) { return irt_rows{b.p, D, hd}; };
+      cp.q = rows(ws.q);
+      cp.ks = rows(ws.k);
+      cp.vs = rows(ws.v);
+      cp.gate = rows(ws.g);
+      cp.out = rows(ws.attn);
+      cp.kc = c4.k_codes;
+      cp.vc = c4.v_codes;
+      cp.kscale = reinterpret_cast<const bf16*>(c4.k_scales);
+      cp.vscale = reinterpret_cast<const bf16*>(c4.v_scales);
+      ctx_attention(cp, s);
+    } else {
+      attention(ap, bf, s);
+    }
     EpiParams r;
     r.mode = EPI_RESID;
     r.x = x;
@@ -861,47 +907,63 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
   }
   const int nctx = base[B];
   const size_t lstride_el = (size_t)nctx * D;
+  const bool kv4 = ctx_cache == IRT_CTX_CACHE_4BIT;
   if (nctx > 0) {
-    ws.cache_k.ensure((size_t)L * lstride_el * esz());
-    ws.cache_v.ensure((size_t)L * lstride_el * esz());
+    const int lp = kv4 ? 1 : L;  // layers that cache_k / cache_v hold
+    ws.cache_k.ensure((size_t)lp * lstride_el * esz());
+    ws.cache_v.ensure((size_t)lp * lstride_el * esz());
+    if (kv4) ws.cache4.ensure((size_t)L * cache4_layer_bytes(nctx));
     to_device(ws.rowmap_t, map_t.data(), map_t.size(), IRT_MEM_HOST, s);
-    EpiParams c;
-    c.mode = EPI_CTXKV;
-    c.out_bf16 = bf;
-    c.ck = ws.cache_k.p;
-    c.cv = ws.cache_v.p;
-    c.layer_stride = (long)lstride_el;
-    c.Dq = D;
-    c.hd = hd;
-    c.H = H;
-    c.kn_w = kn_all.as<float>();
-    c.eps = (float)cfg.norm_eps;
-    c.row_map = ws.rowmap_t.as<int>();
-    if (B * Tt > 0) gemm(text_t.p, td, ctx_text_w, B * Tt, L * 2 * D, td, c, s);
-    if (aux_in) {
-      to_device(ws.rowmap_a, map_a.data(), map_a.size(), IRT_MEM_HOST, s);
+    if (aux_in) to_device(ws.rowmap_a, map_a.data(), map_a.size(), IRT_MEM_HOST, s);
+    const int nl = !skv_cfg ? 0 : pr.speaker_kv_max_layers < 0 ? L : std::min(pr.speaker_kv_max_layers, L);
+    int nscaled = 0;  // rows of the scaled speaker copies (SpeakerKvConfig, src/rf/kv_scaling.rs:10-60)
+    if (skv_cfg) {
+      to_device(ws.rowmap_as, map_as.data(), map_as.size(), IRT_MEM_HOST, s);
+      std::vector<int> rows;
+      for (int b = 0; b < B; ++b)
+        for (int i = 0; i < sc[b]; ++i) rows.push_back(base[b] + i);
+      to_device(ws.rows, rows.data(), rows.size(), IRT_MEM_HOST, s);
+      nscaled = (int)rows.size();
+      IRT_CUDA(cudaStreamSynchronize(s));
+    }
+    // K and V of layers [l0, l0 + n) into cache_k / cache_v from layer 0 on
+    auto project = [&](int l0, int n) {
+      EpiParams c;
+      c.mode = EPI_CTXKV;
+      c.out_bf16 = bf;
+      c.ck = ws.cache_k.p;
+      c.cv = ws.cache_v.p;
+      c.layer_stride = (long)lstride_el;
+      c.Dq = D;
+      c.hd = hd;
+      c.H = H;
+      c.kn_w = kn_all.as<float>() + (size_t)l0 * D;
+      c.eps = (float)cfg.norm_eps;
+      c.row_map = ws.rowmap_t.as<int>();
+      const long w0 = (long)l0 * 2 * D;
+      if (B * Tt > 0) gemm(text_t.p, td, ctx_text_w, B * Tt, n * 2 * D, td, c, s, w0);
+      if (!aux_in) return;
       c.row_map = ws.rowmap_a.as<int>();
-      gemm(ws.aux_state_t.p, aux_dim, ctx_aux_w, B * Ta, L * 2 * D, aux_dim, c, s);
-      if (skv_cfg) {
-        // scaled copy of the speaker rows (SpeakerKvConfig, src/rf/kv_scaling.rs:10-60)
-        to_device(ws.rowmap_as, map_as.data(), map_as.size(), IRT_MEM_HOST, s);
-        c.row_map = ws.rowmap_as.as<int>();
-        gemm(ws.aux_state_t.p, aux_dim, ctx_aux_w, B * Ta, L * 2 * D, aux_dim, c, s);
-        int nl = pr.speaker_kv_max_layers < 0 ? L : std::min(pr.speaker_kv_max_layers, L);
-        std::vector<int> rows;
-        for (int b = 0; b < B; ++b)
-          for (int i = 0; i < sc[b]; ++i) rows.push_back(base[b] + i);
-        DevBuf& rows_d = ws.rows;
-        to_device(rows_d, rows.data(), rows.size(), IRT_MEM_HOST, s);
-        for (int l = 0; l < nl; ++l) {
-          uint8_t* kl = ws.cache_k.as<uint8_t>() + (size_t)l * lstride_el * esz();
-          uint8_t* vl = ws.cache_v.as<uint8_t>() + (size_t)l * lstride_el * esz();
-          scale_rows_bf16_or_f32(kl, bf, D, rows_d.as<int>(), (int)rows.size(), pr.speaker_kv_scale, s);
-          scale_rows_bf16_or_f32(vl, bf, D, rows_d.as<int>(), (int)rows.size(), pr.speaker_kv_scale, s);
-        }
-        IRT_CUDA(cudaStreamSynchronize(s));
+      gemm(ws.aux_state_t.p, aux_dim, ctx_aux_w, B * Ta, n * 2 * D, aux_dim, c, s, w0);
+      if (!skv_cfg) return;
+      c.row_map = ws.rowmap_as.as<int>();
+      gemm(ws.aux_state_t.p, aux_dim, ctx_aux_w, B * Ta, n * 2 * D, aux_dim, c, s, w0);
+      for (int l = l0; l < std::min(nl, l0 + n); ++l) {
+        uint8_t* kl = ws.cache_k.as<uint8_t>() + (size_t)(l - l0) * lstride_el * esz();
+        uint8_t* vl = ws.cache_v.as<uint8_t>() + (size_t)(l - l0) * lstride_el * esz();
+        scale_rows_bf16_or_f32(kl, bf, D, ws.rows.as<int>(), nscaled, pr.speaker_kv_scale, s);
+        scale_rows_bf16_or_f32(vl, bf, D, ws.rows.as<int>(), nscaled, pr.speaker_kv_scale, s);
+      }
+    };
+    if (!kv4) {
+      project(0, L);
+    } else {
+      for (int l = 0; l < L; ++l) {
+        project(l, 1);
+        kv4_append(cache4_layer(l, nctx), bf, 0, nctx, {ws.cache_k.p, D, hd}, {ws.cache_v.p, D, hd}, nctx, nullptr, s);
       }
     }
+    if (skv_cfg) IRT_CUDA(cudaStreamSynchronize(s));
   }
 
   // ---- timestep schedule, embeddings, cond_module, adaLN tables ----
@@ -1052,6 +1114,8 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
       int nalt = (uc && pr.cfg_mode == IRT_CFG_ALTERNATING) ? (int)enabled.size() : 1;
       for (int a = 0; a < nalt; ++a) table_for(groups_for(uc, sk, a));
     }
+  int max_ctx = 0;
+  for (const SeqDesc& d : all_desc) max_ctx = std::max(max_ctx, d.ctx_len);
   ws.seqs.ensure(all_desc.size() * sizeof(SeqDesc) + 16);
   IRT_CUDA(cudaMemcpyAsync(ws.seqs.p, all_desc.data(), all_desc.size() * sizeof(SeqDesc), cudaMemcpyHostToDevice, s));
   IRT_CUDA(cudaStreamSynchronize(s));
@@ -1101,7 +1165,7 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
       if (bf) gather_split_rows(xin_f32, reinterpret_cast<bf16*>(dst), ntok, P, Pk, s);
       else gather_rows(xin_f32, nullptr, dst, 0, ntok, P, s, Pk);
     }
-    forward_step(G * ntok, ws.seqs.as<SeqDesc>() + toff, G * B, Smax, t_index, nctx, s);
+    forward_step(G * ntok, ws.seqs.as<SeqDesc>() + toff, G * B, Smax, max_ctx, t_index, nctx, s);
     last_row_forwards += (long long)G * B;
     if (G == 1) {
       IRT_CUDA(cudaMemcpyAsync(v_out, ws.vout.p, nel * 4, cudaMemcpyDeviceToDevice, s));
@@ -1205,7 +1269,7 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
     IRT_CUDA(cudaMemcpyAsync(out, xs, nel * 4, okind, s));
   }
   IRT_CUDA(cudaStreamSynchronize(s));
-  if (read_and_clear_kernel_error() | read_and_clear_attn_error())
+  if (read_and_clear_kernel_error() | read_and_clear_attn_error() | read_and_clear_ctx_attn_error())
     throw Error(IRT_E_CUDA, "a GEMM pipeline wait timed out (device watchdog); results are invalid");
   last_launches = launch_counter().load() - launches0;
 }

@@ -44,6 +44,10 @@ struct Engine {
   bool has_params = false;
   irt_sampler_params params{};
   std::mutex mu;
+  // IRT_CTX_CACHE_4BIT: the text / speaker K and V of a request are kept in 4
+  // bits (kv4.cu), projected and quantised one layer at a time, so that no
+  // full-precision copy of the cache exists.
+  int ctx_cache = IRT_CTX_CACHE_NATIVE;
 
   // dimensions
   int D = 0, L = 0, H = 0, hd = 0, P = 0, F = 0, Fp = 0, R = 0, Temb = 0;
@@ -86,6 +90,7 @@ struct Engine {
     DevBuf x, h, q, k, v, g, attn, hm, xin, vout, raw, tokpos, seqs, vcomb, xpred, v1, hist[4], xstate, scal;
     DevBuf ex, eh, eq, ek, ev, eg, eattn, ehm, estate, estate2, emask, eseq, etok;  // encoders
     DevBuf cache_k, cache_v, rowmap_t, rowmap_a, rowmap_as, amask, aux_state_t;
+    DevBuf cache4;  // 4-bit context cache, all layers; cache_k / cache_v then hold one layer's rows
     DevBuf ada, temb, ce, su, dn;
     DevBuf ids, tmask, ref, rmask, cids, cmask, noise, out;
     DevBuf rope_cos, rope_sin;
@@ -111,7 +116,7 @@ struct Engine {
   std::map<std::vector<uintptr_t>, int> graph_seen;
   std::map<std::vector<uintptr_t>, long long> graph_kernels;
   DevBuf ada_cur;  // adaLN parameters of the current step, read by the graph
-  void forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, int t_index, int nrows_ctx,
+  void forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, int max_ctx, int t_index, int nrows_ctx,
                     cudaStream_t s);
 
   // adapter_dir: optional PEFT LoRA adapter merged into the weights at load
@@ -123,11 +128,16 @@ struct Engine {
 
   // helpers
   size_t esz() const { return bf ? 2 : 4; }
-  void gemm(const void* A, long lda, const DevBuf& W, int M, int N, int K, EpiParams p, cudaStream_t s);
+  // w_row0: first row of W that the product uses
+  void gemm(const void* A, long lda, const DevBuf& W, int M, int N, int K, EpiParams p, cudaStream_t s,
+            long w_row0 = 0);
+  // layer l of the 4-bit context cache of `rows` rows inside ws.cache4
+  irt_kv4_cache cache4_layer(int l, long rows) const;
+  size_t cache4_layer_bytes(long rows) const;
   void run_encoder(EncoderW& e, int B, int T, const void* input_rows_T, bool from_ids, const uint8_t* d_mask,
                    const float* d_maskf, void* out_state_f32, cudaStream_t s);
-  void dit_forward(int M, const SeqDesc* d_seqs, int nseq, int max_len, const float* ada_t, int nrows_ctx,
-                   cudaStream_t s);
+  void dit_forward(int M, const SeqDesc* d_seqs, int nseq, int max_len, int max_ctx, const float* ada_t,
+                   int nrows_ctx, cudaStream_t s);
 
  private:
   void load(const std::string& path, const std::string& adapter_dir);
