@@ -3,8 +3,8 @@
 // bases that are not multiples of 16 bytes, a scale that is not positive).
 // head_dim <= 128.
 //
-// One CTA = 64 packed query rows (query x grouped head) of one KV head, in
-// tiles of 64 keys; 256 threads as 16 x 16, each with 4 x 4 scores (rows
+// One CTA = 64 (32) packed query rows (query x grouped head) of one KV head, in
+// tiles of 64 keys; 256 threads as 16 x 16, each with 4 x 4 (2 x 4) scores (rows
 // r + 16 i, keys c + 16 j) and 4 x HDT / 16 outputs, so both products run from
 // registers at 16 multiply-adds for each 16-byte shared-memory load, as packed
 // f32 pairs along the head dimension (half the instructions of scalar ones).
@@ -15,6 +15,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ctx_attn.cuh"
 #include "tc_common.cuh"
@@ -29,7 +30,7 @@ using tcx::f2_fma;
 using tcx::f2_unpack;
 using tcx::smem_u32;
 
-constexpr int QT = 64, KT = 64, THREADS = 256;
+constexpr int KT = 64, THREADS = 256;
 constexpr float LN2 = 0.6931471805599453f;
 
 struct TileArgs {
@@ -38,13 +39,15 @@ struct TileArgs {
   int q_vec, k_vec, v_vec, ks_vec, vs_vec, out_vec;
 };
 
-template <int HDT>
+template <int HDT, int RT>
 struct Smem {
+  static constexpr int QT = 16 * RT;  // query rows of a CTA
   static constexpr int CH = HDT / 4;  // 16-byte chunks of a row
   static constexpr int OFF_K = QT * HDT, OFF_V = OFF_K + KT * HDT, OFF_P = OFF_V + KT * HDT, OFF_B = OFF_P + KT * QT;
   static constexpr int FLOATS = OFF_B + KT;
-  // cluster merge over the tiles: O rows, then m and l
-  static_assert(QT * HDT + 2 * QT <= OFF_P, "merge state fits K and V");
+  // cluster merge over the tiles: O rows (padded against bank conflicts), m, l and weights
+  static constexpr int OLD = HDT + 4;
+  static_assert(QT * (OLD + 2 + MAX_SPLIT) <= OFF_P, "merge state fits Q, K and V");
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
@@ -59,10 +62,11 @@ __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
   return tcx::f2_pack(__float_as_uint(lo), __float_as_uint(hi));
 }
 
-template <bool BF, bool CTX4, int HDT>
+// RT: query rows of a thread.
+template <bool BF, bool CTX4, int HDT, int RT>
 __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_constant__ TileArgs a) {
-  using S = Smem<HDT>;
-  constexpr int CH = S::CH, OC = HDT / 8, NV = HDT / 64;  // NV: output chunks of four values per thread and row
+  using S = Smem<HDT, RT>;
+  constexpr int QT = S::QT, CH = S::CH, OC = HDT / 8, NV = HDT / 64;  // NV: output chunks of four values per thread and row
   const CtxAttnParams& p = a.p;
   irt_attn_seq sd;
   if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
@@ -146,10 +150,10 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
     }
   };
 
-  uint64_t acc[4][2 * NV];
-  float m[4], l[4];
+  uint64_t acc[RT][2 * NV];
+  float m[RT], l[RT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < RT; ++i) {
 #pragma unroll
     for (int d = 0; d < 2 * NV; ++d) acc[i][d] = 0;
     m[i] = -INFINITY;
@@ -164,24 +168,24 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
   for (int j = 0; j < nt; ++j) {
     cp_wait<1>();  // K of this tile (its V may still fly)
     __syncthreads();
-    float s[4][4];
+    float s[RT][4];
     {
-      uint64_t s2[4][4];
+      uint64_t s2[RT][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int n = 0; n < 4; ++n) s2[i][n] = 0;
       const ulonglong2* q2 = reinterpret_cast<const ulonglong2*>(sq);
       const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(sk);
 #pragma unroll 4
       for (int ch = 0; ch < CH; ++ch) {
-        ulonglong2 qa[4], kb[4];
+        ulonglong2 qa[RT], kb[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) qa[i] = q2[(r + 16 * i) * CH + (ch ^ (r & 7))];
+        for (int i = 0; i < RT; ++i) qa[i] = q2[(r + 16 * i) * CH + (ch ^ (r & 7))];
 #pragma unroll
         for (int n = 0; n < 4; ++n) kb[n] = k2[(c + 16 * n) * CH + (ch ^ (c & 7))];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int n = 0; n < 4; ++n) s2[i][n] = f2_fma(qa[i].y, kb[n].y, f2_fma(qa[i].x, kb[n].x, s2[i][n]));
       }
@@ -189,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
       for (int n = 0; n < 4; ++n) {
         const bool off = sb[c + 16 * n] != 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) {
           float x, y;
           f2_unpack(s2[i][n], x, y);
           s[i][n] = off ? -INFINITY : x + y;
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
 
     // online softmax: a row's scores are in the 16 threads of a half warp
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
       float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
@@ -221,25 +225,28 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
 #pragma unroll
       for (int d = 0; d < 2 * NV; ++d) acc[i][d] = f2_fma(acc[i][d], c2, 0);
     }
-    // P transposed: the four rows of a thread are one chunk of a key
-    float4* p4 = reinterpret_cast<float4*>(sp);
+    // P transposed: the rows of a thread are one chunk of a key
+    using Chunk = typename std::conditional<RT == 4, float4, float2>::type;
+    Chunk* pc = reinterpret_cast<Chunk*>(sp);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int key = c + 16 * n;
-      p4[key * 16 + (r ^ (key & 15))] = make_float4(s[0][n], s[1][n], s[2][n], s[3][n]);
+      float* t = reinterpret_cast<float*>(&pc[key * 16 + (r ^ (key & 15))]);
+      if constexpr (RT == 4) *reinterpret_cast<float4*>(t) = make_float4(s[0][n], s[1][n], s[2][n], s[3][n]);
+      else *reinterpret_cast<float2*>(t) = make_float2(s[0][n], s[1][n]);
     }
     cp_wait<1>();  // V of this tile (K of the next may still fly)
     __syncthreads();
     const ulonglong2* v2 = reinterpret_cast<const ulonglong2*>(sv);
 #pragma unroll 4
     for (int key = 0; key < KT; ++key) {
-      const float4 pr = p4[key * 16 + (r ^ (key & 15))];
+      const Chunk pr = pc[key * 16 + (r ^ (key & 15))];
       ulonglong2 v[NV];
 #pragma unroll
       for (int u = 0; u < NV; ++u) v[u] = v2[key * CH + ((c + 16 * u) ^ (key & 7))];
-      const float pv[4] = {pr.x, pr.y, pr.z, pr.w};
+      const float* pv = reinterpret_cast<const float*>(&pr);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < RT; ++i) {
         const uint64_t pp = pack2(pv[i], pv[i]);
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
@@ -255,11 +262,10 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
   cp_wait<0>();
 
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
-  auto write = [&](int row, int d, float4 x, float ms, float ls) {  // four values from d of a row of the block
-    const float inv = ls == 0.f ? 0.f : 1.f / ls;
+  auto write = [&](int row, int d, float4 x, float inv) {  // four values from d of a row of the block
     x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
     const int pr = row0 + row;
     const long q = (long)sd.q_start + pr / G;
@@ -269,20 +275,26 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
       x.x *= g.x; x.y *= g.y; x.z *= g.z; x.w *= g.w;
     }
     store4<BF>(p.out.data, q * p.out.row_stride + head * p.out.head_stride + d, a.out_vec, x);
-    if (p.lse && d == 0) p.lse[q * p.H + head] = ls == 0.f ? -INFINITY : fmaf(ms, LN2, logf(ls));
+  };
+  auto write_lse = [&](int row, float ms, float ls) {
+    const int pr = row0 + row;
+    if (p.lse)
+      p.lse[((long)sd.q_start + pr / G) * p.H + hk * G + pr % G] = ls == 0.f ? -INFINITY : fmaf(ms, LN2, logf(ls));
   };
   if (split == 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
       const int row = r + 16 * i;
       if (row0 + row >= nrows) continue;
+      const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+      if (c == 0) write_lse(row, m[i], l[i]);
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
         const int d = 4 * (c + 16 * u);
         float4 x;
         f2_unpack(acc[i][2 * u], x.x, x.y);
         f2_unpack(acc[i][2 * u + 1], x.z, x.w);
-        if (d < hd) write(row, d, x, m[i], l[i]);
+        if (d < hd) write(row, d, x, inv);
       }
     }
     return;
@@ -290,13 +302,15 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
   // this CTA's rows for the others, over its tiles
   __syncthreads();
   float* so = sm;
-  float* sml = sm + QT * HDT;
+  float* sml = sm + QT * S::OLD;
+  float* wt = sml + 2 * QT;  // [row of this CTA][MAX_SPLIT]
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < RT; ++i) {
     const int row = r + 16 * i;
 #pragma unroll
     for (int u = 0; u < NV; ++u)
-      *reinterpret_cast<ulonglong2*>(so + row * HDT + 4 * (c + 16 * u)) = make_ulonglong2(acc[i][2 * u], acc[i][2 * u + 1]);
+      *reinterpret_cast<ulonglong2*>(so + row * S::OLD + 4 * (c + 16 * u)) =
+          make_ulonglong2(acc[i][2 * u], acc[i][2 * u + 1]);
     if (c == 0) {
       sml[row] = m[i];
       sml[QT + row] = l[i];
@@ -305,29 +319,53 @@ __global__ void __launch_bounds__(THREADS, 2) ctx_attn_tile_kernel(const __grid_
   cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
   const int valid = min(QT, nrows - row0), per_row = hd / 4;
-  for (int e = tid; e < ((valid - rank + split - 1) / split) * per_row; e += THREADS) {
-    const int row = (e / per_row) * split + rank, d = (e % per_row) * 4;  // rows dealt out to the CTAs
-    float mt = -INFINITY;
-    for (int u = 0; u < split; ++u) mt = fmaxf(mt, cluster.map_shared_rank(sml, u)[row]);
+  const int mine = (valid - rank + split - 1) / split;  // rows dealt out to this CTA
+  for (int i = tid; i < mine; i += THREADS) {
+    const int row = i * split + rank;
+    float mc[MAX_SPLIT], lc[MAX_SPLIT], mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int u = 0; u < MAX_SPLIT; ++u)
+      if (u < split) {
+        const float* o = cluster.map_shared_rank(sml, u);
+        mc[u] = o[row];
+        lc[u] = o[QT + row];
+        mt = fmaxf(mt, mc[u]);
+      }
     const float base = mt == -INFINITY ? 0.f : mt;
-    float lt = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int u = 0; u < split; ++u) {
-      const float* om = cluster.map_shared_rank(sml, u);
-      const float f = exp2f(om[row] - base);
-      const float4 o = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, u) + row * HDT + d);
-      lt = fmaf(om[QT + row], f, lt);
-      x.x = fmaf(o.x, f, x.x);
-      x.y = fmaf(o.y, f, x.y);
-      x.z = fmaf(o.z, f, x.z);
-      x.w = fmaf(o.w, f, x.w);
-    }
-    write(row, d, x, mt, lt);
+#pragma unroll
+    for (int u = 0; u < MAX_SPLIT; ++u)
+      if (u < split) {
+        mc[u] = exp2f(mc[u] - base);
+        lt = fmaf(lc[u], mc[u], lt);
+      }
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+#pragma unroll
+    for (int u = 0; u < MAX_SPLIT; ++u)
+      if (u < split) wt[i * MAX_SPLIT + u] = mc[u] * inv;
+    write_lse(row, mt, lt);
+  }
+  __syncthreads();
+  for (int e = tid; e < mine * per_row; e += THREADS) {
+    const int i = e / per_row, d = (e - i * per_row) * 4, row = i * split + rank;
+    float4 o[MAX_SPLIT], x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < MAX_SPLIT; ++u)
+      if (u < split) o[u] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(so, u) + row * S::OLD + d);
+#pragma unroll
+    for (int u = 0; u < MAX_SPLIT; ++u)
+      if (u < split) {
+        const float f = wt[i * MAX_SPLIT + u];
+        x.x = fmaf(o[u].x, f, x.x);
+        x.y = fmaf(o[u].y, f, x.y);
+        x.z = fmaf(o[u].z, f, x.z);
+        x.w = fmaf(o[u].w, f, x.w);
+      }
+    write(row, d, x, 1.f);
   }
   cluster.sync();  // the others may still read this CTA's rows
 }
 
-template <bool BF, bool CTX4, int HDT>
+template <bool BF, bool CTX4, int HDT, int RT>
 void launch(const CtxAttnParams& p, cudaStream_t s) {
   TileArgs a{};
   a.p = p;
@@ -338,13 +376,14 @@ void launch(const CtxAttnParams& p, cudaStream_t s) {
   a.vs_vec = rows_vec(p.vs, BF);
   a.out_vec = rows_vec(p.out, BF) && (!p.gate.data || rows_vec(p.gate, BF));
   const int sms = device_sms();
+  constexpr int QT = Smem<HDT, RT>::QT;
   const long blocks = ((long)p.max_q * p.G + QT - 1) / QT;
   const long ctas = blocks * p.Hkv * p.nseq;
   const long ktiles = (p.max_k + KT - 1L) / KT + (p.ks.data ? (p.max_q + KT - 1L) / KT : 0);
   a.split = 1;
   while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 2L * sms && a.split * 2 <= ktiles) a.split *= 2;
-  constexpr size_t smem = Smem<HDT>::FLOATS * sizeof(float);
-  auto kernel = ctx_attn_tile_kernel<BF, CTX4, HDT>;
+  constexpr size_t smem = Smem<HDT, RT>::FLOATS * sizeof(float);
+  auto kernel = ctx_attn_tile_kernel<BF, CTX4, HDT, RT>;
   static std::atomic<uint64_t> told{0};
   allow_smem(kernel, smem, told);
   cudaLaunchConfig_t cfg = {};
@@ -361,10 +400,17 @@ void launch(const CtxAttnParams& p, cudaStream_t s) {
   IRT_CHECK_LAUNCH();
 }
 
+// Blocks of 32 rows up to 32 (half the work of a key tile), of 64 beyond.
 template <bool BF, bool CTX4>
 void launch_hd(const CtxAttnParams& p, cudaStream_t s) {
-  if (p.hd <= 64) launch<BF, CTX4, 64>(p, s);
-  else launch<BF, CTX4, 128>(p, s);
+  const bool few = (long)p.max_q * p.G <= 32;
+  if (p.hd <= 64) {
+    if (few) launch<BF, CTX4, 64, 2>(p, s);
+    else launch<BF, CTX4, 64, 4>(p, s);
+  } else {
+    if (few) launch<BF, CTX4, 128, 2>(p, s);
+    else launch<BF, CTX4, 128, 4>(p, s);
+  }
 }
 
 }  // namespace
