@@ -218,9 +218,17 @@ __global__ void __launch_bounds__(KV4_READ_THREADS) kv4_read_kernel(const __grid
   for (int i = 0; i < N; ++i) {
     const int e = threadIdx.x + KV4_READ_THREADS * i, o = e % OCTS;
     const long r = r0 + e / OCTS;
-    float x[8];
-    kv4_unpack8(w[i], sb[i], x);
-    if (in[i]) store8<BF>(sd.x.data, r * sd.x.row_stride + h * sd.x.head_stride + 8 * o, sd.vec, x);
+    if (!in[i]) continue;
+    const long off = r * sd.x.row_stride + h * sd.x.head_stride + 8 * o;
+    if (BF && sd.vec) {  // the values as the tensor cores get them
+      const uint32_t s = (uint32_t)sb[i] << 16 | sb[i];
+      const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&s);
+      *reinterpret_cast<uint4*>(static_cast<bf16*>(sd.x.data) + off) = kv4_bf16x8<true>(w[i], s2, s2);
+    } else {
+      float x[8];
+      kv4_unpack8(w[i], sb[i], x);
+      store8<BF>(sd.x.data, off, sd.vec, x);
+    }
   }
 }
 
