@@ -275,7 +275,7 @@ int irt_kv4_append(int device, int dtype, const irt_kv4_cache* cache, int64_t ro
     need(cache, "cache");
     need(k, "k");
     need(v, "v");
-    irt::kv4_check_rows(*cache, dtype, row_start, n, *k, *v, src_rows, false);
+    irt::kv4_check_rows(*cache, dtype, row_start, n, *k, *v, src_rows, src_index, false);
     if (!src_index && n > src_rows)
       throw irt::shape_error("n " + std::to_string(n) + " exceeds the source's " + std::to_string(src_rows) + " rows");
     irt::DeviceGuard dg(device);
@@ -290,7 +290,7 @@ int irt_kv4_read(int device, int dtype, const irt_kv4_cache* cache, int64_t row_
     need(cache, "cache");
     need(k, "k");
     need(v, "v");
-    irt::kv4_check_rows(*cache, dtype, row_start, n, *k, *v, n, true);
+    irt::kv4_check_rows(*cache, dtype, row_start, n, *k, *v, n, nullptr, true);
     irt::DeviceGuard dg(device);
     irt::kv4_read(*cache, dtype == IRT_PREC_BF16, row_start, n, *k, *v, reinterpret_cast<cudaStream_t>(stream));
   });

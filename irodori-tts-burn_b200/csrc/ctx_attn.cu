@@ -203,16 +203,28 @@ constexpr long MAX_ROWS = (1L << 30) - 1;
 
 Error arg_error(const std::string& m) { return Error(IRT_E_INVALID_ARG, m); }
 
-// First and one-past-last byte of a tensor of rows (strides are not negative).
+// First and one-past-last byte of a tensor; for rows of heads also the bytes
+// from one row to the next and those that a row spans.
 struct Span {
-  uintptr_t lo, hi;
+  uintptr_t lo, hi, period, extent;
 };
 Span span_of(const irt_rows& r, long rows, int heads, int hd, int esz) {
   const uintptr_t lo = reinterpret_cast<uintptr_t>(r.data);
-  if (!r.data || rows <= 0) return {lo, lo};
-  return {lo, lo + (uintptr_t)((rows - 1) * r.row_stride + (heads - 1) * r.head_stride + hd) * esz};
+  if (!r.data || rows <= 0) return {lo, lo, 0, 0};
+  const uintptr_t extent = (uintptr_t)((heads - 1) * r.head_stride + hd) * esz, period = (uintptr_t)r.row_stride * esz;
+  return {lo, lo + (rows - 1) * period + extent, period, extent};
 }
-bool overlap(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+Span span_of(const void* data, long bytes) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(data);
+  return {lo, data ? lo + bytes : lo, 0, 0};
+}
+bool overlap(const Span& a, const Span& b) {
+  if (a.lo >= b.hi || b.lo >= a.hi) return false;
+  if (a.period == 0 || a.period != b.period) return true;
+  // columns of one tensor: rows of both in the same period, side by side
+  const uintptr_t d = b.lo >= a.lo ? (b.lo - a.lo) % a.period : (a.period - (a.lo - b.lo) % a.period) % a.period;
+  return d < a.extent || d + b.extent > a.period;
+}
 
 void check_rows(const char* name, const irt_rows& r, long rows, int heads, int esz) {
   if (!r.data && rows > 0) throw arg_error(std::string(name) + " is NULL");
@@ -255,8 +267,21 @@ void kv4_check_cache(const irt_kv4_cache& c) {
   }
 }
 
+namespace {
+
+constexpr const char* KV4_NAMES[4] = {"k_codes", "k_scales", "v_codes", "v_scales"};
+void kv4_spans(const irt_kv4_cache& c, Span (&s)[4]) {
+  const long n = c.rows * c.kv_heads, codes = n * (c.head_dim / 2), scales = n * kv4_groups(c.head_dim) * 2;
+  s[0] = span_of(c.k_codes, codes);
+  s[1] = span_of(c.k_scales, scales);
+  s[2] = span_of(c.v_codes, codes);
+  s[3] = span_of(c.v_scales, scales);
+}
+
+}  // namespace
+
 void kv4_check_rows(const irt_kv4_cache& c, int dtype, long row_start, long n, const irt_rows& k, const irt_rows& v,
-                    long ext_rows, bool written) {
+                    long ext_rows, const int* idx, bool written) {
   if (dtype != IRT_PREC_BF16 && dtype != IRT_PREC_F32) throw arg_error("dtype must be an irt_precision");
   kv4_check_cache(c);
   if (row_start < 0 || n < 0 || row_start > c.rows || n > c.rows - row_start)
@@ -270,6 +295,19 @@ void kv4_check_rows(const irt_kv4_cache& c, int dtype, long row_start, long n, c
     check_own("k", k, ext_rows, c.kv_heads, c.head_dim);
     check_own("v", v, ext_rows, c.kv_heads, c.head_dim);
   }
+  const Span sk = span_of(k, ext_rows, c.kv_heads, c.head_dim, esz), sv = span_of(v, ext_rows, c.kv_heads, c.head_dim, esz);
+  if (written && overlap(sk, sv)) throw arg_error("k overlaps v");
+  Span buf[4];
+  kv4_spans(c, buf);
+  const Span si = span_of(idx, 4 * n);
+  for (int i = 0; i < 4; ++i) {
+    const std::string name = std::string("the cache's ") + KV4_NAMES[i];
+    if (overlap(sk, buf[i])) throw arg_error("k overlaps " + name);
+    if (overlap(sv, buf[i])) throw arg_error("v overlaps " + name);
+    if (overlap(si, buf[i])) throw arg_error("the source index overlaps " + name);
+    for (int j = 0; j < i && !written; ++j)
+      if (overlap(buf[j], buf[i])) throw arg_error(std::string(KV4_NAMES[j]) + " overlaps " + name);
+  }
 }
 
 CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache, const irt_rows* k,
@@ -281,7 +319,8 @@ CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache
   if (a.q_rows < 0 || k_rows < 0 || a.q_rows > MAX_ROWS || k_rows > MAX_ROWS)
     throw shape_error("q_rows and the context rows must be in 0..2^30 - 1");
   if ((long)a.max_q_len * (a.heads / a.kv_heads) > (1L << 26)) throw shape_error("max_q_len is too large");
-  if (!(a.scale == a.scale) || a.scale - a.scale != 0.f) throw arg_error("scale must be finite");
+  const float s2 = a.scale * LOG2E;  // as the kernels use it
+  if (s2 - s2 != 0.f) throw arg_error("scale must be finite, and below 2^127");
   if (!a.seqs && ((long)a.num_seqs * a.max_q_len > a.q_rows || (long)a.num_seqs * a.max_k_len > k_rows))
     throw shape_error("without a sequence table q needs num_seqs * max_q_len rows and the context num_seqs * max_k_len");
   const bool bf = a.dtype == IRT_PREC_BF16;
@@ -308,10 +347,19 @@ CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache
   check_rows("out", a.out, a.q_rows, a.heads, esz);
   check_own("out", a.out, a.q_rows, a.heads, a.head_dim);
   if (a.gate.data) check_rows("gate", a.gate, a.q_rows, a.heads, esz);
-  const Span so = span_of(a.out, a.q_rows, a.heads, a.head_dim, esz);
-  auto apart = [&](const char* name, const irt_rows& r, long rows, int heads) {
-    if (overlap(so, span_of(r, rows, heads, a.head_dim, esz))) throw arg_error("out overlaps " + std::string(name));
+  const Span so = span_of(a.out, a.q_rows, a.heads, a.head_dim, esz), sl = span_of(a.lse, a.q_rows * a.heads * 4);
+  if (reinterpret_cast<uintptr_t>(a.lse) % 4 || reinterpret_cast<uintptr_t>(a.seqs) % 4)
+    throw arg_error("lse and seqs must be aligned to 4 bytes");
+  auto apart_span = [&](const char* name, const Span& x) {
+    if (overlap(so, x)) throw arg_error("out overlaps " + std::string(name));
+    if (overlap(sl, x)) throw arg_error("lse overlaps " + std::string(name));
   };
+  auto apart = [&](const char* name, const irt_rows& r, long rows, int heads) {
+    apart_span(name, span_of(r, rows, heads, a.head_dim, esz));
+  };
+  if (overlap(so, sl)) throw arg_error("out overlaps lse");
+  apart_span("key_mask", span_of(a.key_mask, k_rows));
+  apart_span("seqs", span_of(a.seqs, a.num_seqs * (long)sizeof(irt_attn_seq)));
   apart("q", a.q, a.q_rows, a.heads);
   apart("gate", a.gate, a.q_rows, a.heads);
   if (cache) {
@@ -320,6 +368,9 @@ CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache
       throw shape_error("the cache holds " + std::to_string(cache->kv_heads) + " heads of " +
                         std::to_string(cache->head_dim) + ", the call has " + std::to_string(a.kv_heads) + " of " +
                         std::to_string(a.head_dim));
+    Span buf[4];
+    kv4_spans(*cache, buf);
+    for (int i = 0; i < 4; ++i) apart_span(KV4_NAMES[i], buf[i]);
     p.kc = cache->k_codes;
     p.vc = cache->v_codes;
     p.kscale = reinterpret_cast<const bf16*>(cache->k_scales);

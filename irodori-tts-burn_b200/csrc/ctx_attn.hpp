@@ -69,9 +69,9 @@ CtxAttnParams ctx_attn_params(const irt_attn_args& a, const irt_kv4_cache* cache
                               const irt_rows* v, long k_rows, const irt_rows* k_self, const irt_rows* v_self);
 void kv4_check_cache(const irt_kv4_cache& c);
 // Cache rows [row_start, row_start + n) against `ext_rows` rows of k and v
-// (written: they are outputs).
+// (written: they are outputs) and n source indices (or null).
 void kv4_check_rows(const irt_kv4_cache& c, int dtype, long row_start, long n, const irt_rows& k, const irt_rows& v,
-                    long ext_rows, bool written);
+                    long ext_rows, const int* idx, bool written);
 
 // Sets the current device for one call and puts the caller's back.
 struct DeviceGuard {

@@ -15,7 +15,8 @@ the same attention to programs that keep queries and context rows themselves.
 Unlike ``InferenceEngine.sample`` the calls queue their work and return: with
 ``stream=None`` on torch's current stream of the tensors' GPU (whichever GPU is
 current), so they order like torch's own operators and can be captured into a
-CUDA graph.  They are forward only; a tensor that requires a gradient is
+CUDA graph.  On an explicit ``stream`` the caller orders the work before and
+after; the tensors' memory is kept until that stream is done with it.  They are forward only; a tensor that requires a gradient is
 refused while gradients are recorded.
 """
 
@@ -62,6 +63,8 @@ def _t():
 
 def _heads(name, t, device, dtype, shape):
     """(address, row stride, head stride) of a [rows, heads, head_dim] tensor (any strides, the last one 1)."""
+    if not isinstance(t, _torch.Tensor):
+        raise IrodoriError(22, f"{name} must be a torch CUDA tensor")
     if t.dtype is dtype and t.get_device() == device and t.shape == shape and not t.requires_grad:
         row, head, one = t.stride()
         if one == 1:
@@ -148,6 +151,11 @@ def attention_table(q_lens, k_lens, k_starts=None, device=0):
         raise IrodoriError(2, "Shape mismatch: q_lens, k_lens and k_starts must have one entry per sequence")
     if any(x < 0 for x in q_lens + k_lens):
         raise IrodoriError(2, "Shape mismatch: lengths must not be negative")
+    if sum(q_lens) >= 1 << 30 or max(k_lens, default=0) >= 1 << 30 or \
+            (sum(k_lens) if k_starts is None else max(map(int, k_starts), default=0)) >= 1 << 30:
+        raise IrodoriError(2, "Shape mismatch: the query rows and the context rows must stay below 2^30")
+    if k_starts is not None and min(map(int, k_starts), default=0) < 0:
+        raise IrodoriError(2, "Shape mismatch: k_starts must not be negative")
     rows, q, k = [], 0, 0
     for i, (a, b) in enumerate(zip(q_lens, k_lens)):
         rows.append([q, a, k if k_starts is None else int(k_starts[i]), b])
@@ -155,6 +163,13 @@ def attention_table(q_lens, k_lens, k_starts=None, device=0):
     if not rows:
         return torch.zeros((0, 4), dtype=torch.int32, device=torch.device("cuda", device))
     return torch.tensor(rows, dtype=torch.int32, device=torch.device("cuda", device))
+
+
+def _row_range(cache, row_start, n):
+    if not isinstance(cache, Kv4Cache):
+        raise IrodoriError(22, "cache must be a Kv4Cache")
+    if not 0 <= row_start <= cache.rows or not 0 <= n <= cache.rows - row_start:
+        raise IrodoriError(2, f"Shape mismatch: rows [{row_start}, {row_start} + {n}) are outside the cache's {cache.rows}")
 
 
 class Kv4Cache:
@@ -204,6 +219,8 @@ def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=
     ``src_rows`` (int32 tensor; an index outside the source leaves its cache
     row as it was)."""
     torch = _first("k", k)
+    if not isinstance(cache, Kv4Cache):
+        raise IrodoriError(22, "cache must be a Kv4Cache")
     n_src = k.shape[0]
     shape = (n_src, cache.kv_heads, cache.head_dim)
     kr = _ROWS.pack(*_heads("k", k, cache.device, k.dtype, shape))
@@ -212,6 +229,7 @@ def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=
     if src_rows is not None:
         n = src_rows.shape[0] if isinstance(src_rows, torch.Tensor) and src_rows.dim() == 1 else -1
         idx = _plain("src_rows", src_rows, cache.device, _INT32, (n,))
+    _row_range(cache, row_start, n)
     handle, side = _stream(stream, cache.device)
     _check(lib().irt_kv4_append(cache.device, _dtype_code[k.dtype], cache._c, row_start, n, kr, vr, n_src, idx, handle))
     _keep(side, k, v, src_rows, *cache.buffers)
@@ -226,8 +244,7 @@ def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=
     if dtype not in _dtype_code:
         raise IrodoriError(9, f"dtype must be bfloat16 or float32, got {dtype}")
     n = cache.rows - row_start if rows is None else rows
-    if n < 0:
-        raise IrodoriError(2, f"Shape mismatch: {n} rows from {row_start} of a cache of {cache.rows}")
+    _row_range(cache, row_start, n)
     handle, side = _stream(stream, cache.device)
     shape = (n, cache.kv_heads, cache.head_dim)
     k = _empty(side, shape, dtype, cache.device)
@@ -248,7 +265,10 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
     handle, side = _stream(stream, dev)
     if out is None:
         out = _empty_like(side, q)
-    out_p, out_row, out_head = _heads("out", out, dev, dtype, shape)
+        out_row, out_head, _ = out.stride()
+        out_p = out.data_ptr()
+    else:
+        out_p, out_row, out_head = _heads("out", out, dev, dtype, shape)
     lse = _empty(side, (n, h), torch.float32, dev) if return_lse else None
     if seqs is None:
         nseq, tab = (n // max_q_len if max_q_len > 0 else 0), 0
@@ -262,9 +282,12 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
     if key_mask is not None:
         mask = _plain("key_mask", key_mask, dev, _MASKS, (k_rows,))
     g = (0, 0, 0) if gate is None else _heads("gate", gate, dev, dtype, shape)
-    a = _ATTN.pack(dev, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
-                   d ** -0.5 if scale is None else scale, n, tab, *_heads("q", q, dev, dtype, shape), *g, out_p, out_row,
-                   out_head, mask, 0 if lse is None else lse.data_ptr())
+    try:
+        a = _ATTN.pack(dev, _dtype_code[dtype], h, kv_heads, d, nseq, max_q_len, max_k_len,
+                       d ** -0.5 if scale is None else scale, n, tab, *_heads("q", q, dev, dtype, shape), *g, out_p,
+                       out_row, out_head, mask, 0 if lse is None else lse.data_ptr())
+    except (struct.error, OverflowError) as e:
+        raise IrodoriError(22, f"max_q_len, max_k_len or scale is out of range: {e}") from None
     status = call(a, *context, handle)
     if status:
         _check(status)
@@ -293,11 +316,11 @@ def cross_attention(q, k, v, seqs, max_q_len: int, max_k_len: int, key_mask=None
     matters."""
     _first("q", q)
     _first("k", k)
-    n = k.shape[0]
-    shape = (n, k.shape[1], q.shape[2])
+    n, kv_heads, _ = k.shape
+    shape = (n, kv_heads, q.shape[2])
     dev = q.get_device()
     context = (_ROWS.pack(*_heads("k", k, dev, q.dtype, shape)), _ROWS.pack(*_heads("v", v, dev, q.dtype, shape)), n)
-    return _attention(lib().irt_cross_attention, q, shape[1], n, seqs, max_q_len, max_k_len, key_mask, gate, scale,
+    return _attention(lib().irt_cross_attention, q, kv_heads, n, seqs, max_q_len, max_k_len, key_mask, gate, scale,
                       out, return_lse, stream, context, (k, v))
 
 
@@ -310,6 +333,8 @@ def kv4_attention(q, cache: Kv4Cache, seqs, max_q_len: int, max_k_len: int, k_se
     those of ``cross_attention``, the cache's rows in the place of ``k``, ``v``."""
     _first("q", q)
     dev = q.get_device()
+    if not isinstance(cache, Kv4Cache):
+        raise IrodoriError(22, "cache must be a Kv4Cache")
     if cache.device != dev:
         raise IrodoriError(22, f"the cache must be on cuda:{dev}, got cuda:{cache.device}")
     shape = (q.shape[0], cache.kv_heads, q.shape[2])

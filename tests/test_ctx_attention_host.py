@@ -177,3 +177,67 @@ def test_python_calls_refuse_host_tensors(pkg, ops):
         assert ei.value.kind == "Shape"
     with pytest.raises(pkg.IrodoriError):
         pkg.attention_table([1], [1], [1, 2])
+
+
+def test_what_is_written_must_lie_apart(pkg, ops):
+    """lse, the mask and the cache's buffers against what a call writes; columns of one tensor are apart."""
+    L = pkg.lib()
+    byref = ctypes.byref
+
+    def refusal(rc):
+        got, text = status(pkg, rc)
+        assert got == "InvalidArgument", (got, text)
+        return text
+
+    k, v = Rows(*K), Rows(*V)
+    for kw, msg in ((dict(lse=0x20000000), "out overlaps lse"), (dict(lse=0x10000000), "lse overlaps q"),
+                    (dict(lse=0x30000000), "lse overlaps k"), (dict(key_mask=0x20000004), "out overlaps key_mask"),
+                    (dict(seqs=0x20000010), "out overlaps seqs"), (dict(lse=0x60000002), "aligned to 4"),
+                    (dict(seqs=0x60000002), "aligned to 4")):
+        assert msg in refusal(L.irt_cross_attention(byref(attn_args(ops, **kw)), byref(k), byref(v), 10, None))
+    a = attn_args(ops, out=Rows(0x51000000, 512, 128))
+    assert "out overlaps k_scales" in refusal(L.irt_kv4_attention(byref(a), byref(cache_struct(ops)), None, None, None))
+    # 10 rows x 2 heads x 64 bytes of codes: 1280 bytes
+    for kw, msg in ((dict(v_codes=0x50000000 + 1264), "k_codes overlaps the cache's v_codes"),
+                    (dict(k_scales=0x50000000), "k_codes overlaps the cache's k_scales"),
+                    (dict(v_scales=0x30000000), "k overlaps the cache's v_scales"),
+                    (dict(k_codes=0x40000000), "v overlaps the cache's k_codes")):
+        c = cache_struct(ops, **kw)
+        assert msg in refusal(L.irt_kv4_append(0, 0, byref(c), 0, 5, byref(k), byref(v), 5, None, None))
+    c = cache_struct(ops)
+    assert "source index overlaps" in refusal(
+        L.irt_kv4_append(0, 0, byref(c), 0, 5, byref(k), byref(v), 5, 0x50000000, None))
+    assert "k overlaps v" in refusal(L.irt_kv4_read(0, 0, byref(c), 0, 5, byref(k), byref(k), None))
+    # columns of one tensor pass the check that a shared column fails (the call then stops at its lse)
+    wide = [Rows(0x10000000 + 2 * 256 * i, 768, 128) for i in range(3)]
+    for q, out, msg in ((0, 1, "lse overlaps k"), (1, 0, "lse overlaps k"), (2, 0, "lse overlaps k"),
+                        (1, 1, "out overlaps q")):
+        a = attn_args(ops, heads=2, kv_heads=2, q=wide[q], out=wide[out], lse=0x30000000)
+        assert refusal(L.irt_cross_attention(byref(a), byref(k), byref(v), 10, None)) == msg
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -2.4e38])
+def test_a_scale_that_the_kernels_cannot_hold(pkg, ops, scale):
+    a, k, v = attn_args(ops, scale=scale), Rows(*K), Rows(*V)
+    got, text = status(pkg, pkg.lib().irt_cross_attention(ctypes.byref(a), ctypes.byref(k), ctypes.byref(v), 10, None))
+    assert got == "InvalidArgument" and "scale" in text
+
+
+def test_python_ranges_that_c_integers_would_wrap(pkg, ops):
+    c = pkg.Kv4Cache.__new__(pkg.Kv4Cache)
+    c.rows = 10
+    for start, n in ((2 ** 64, 1), (0, 2 ** 64), (-1, 1), (11, 0), (3, 8), (-(2 ** 64), 2)):
+        with pytest.raises(pkg.IrodoriError) as ei:
+            ops._row_range(c, start, n)
+        assert ei.value.kind == "Shape" and "outside the cache" in str(ei.value)
+    ops._row_range(c, 10, 0)
+    with pytest.raises(pkg.IrodoriError):
+        ops._row_range(None, 0, 0)
+    for lens in (([2 ** 29, 2 ** 29], [1, 1]), ([1], [2 ** 31]), ([1, 1], [2 ** 29, 2 ** 29])):
+        with pytest.raises(pkg.IrodoriError) as ei:
+            pkg.attention_table(*lens)
+        assert ei.value.kind == "Shape" and "2^30" in str(ei.value)
+    for starts in ([2 ** 31], [-1]):
+        with pytest.raises(pkg.IrodoriError) as ei:
+            pkg.attention_table([1], [1], starts)
+        assert ei.value.kind == "Shape"

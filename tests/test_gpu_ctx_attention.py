@@ -565,3 +565,99 @@ def test_kv4_values_at_the_ends_of_the_range(pkg, dev, ql, size):
     out = pkg.kv4_attention(q, c, device_table([(0, ql, 2, 1)], dev), ql, 1)
     pkg.attention_check(0)
     assert torch.equal(out, v[2].expand(ql, h, hd))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("ql", [2, 70])
+def test_out_in_a_column_of_the_packed_projections(pkg, dev, dtype, ql):
+    """q, gate and out as columns of one tensor: only out's column changes."""
+    g = gen(dev, 91)
+    h, hd, n = 4, 64, 3 * ql
+    wide = torch.randn(n, 3, h, hd, device=dev, generator=g).to(dtype)
+    k, v = torch.randn(2, 300, h, hd, device=dev, generator=g).to(dtype).unbind(0)
+    seqs, _, _ = table([ql] * 3, [100, 1, 199])
+    before = wide.clone()
+    _, lse = pkg.cross_attention(wide[:, 0], k, v, device_table(seqs, dev), ql, 199, gate=wide[:, 2], out=wide[:, 1],
+                                 return_lse=True)
+    check(wide[:, 1], lse, reference(before[:, 0], k, v, seqs, 1 / math.sqrt(hd), gate=before[:, 2]))
+    assert torch.equal(wide[:, 0], before[:, 0]) and torch.equal(wide[:, 2], before[:, 2])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("ql", [1, 50])
+def test_tensors_without_rows(pkg, dev, dtype, ql):
+    h, hd = 4, 64
+    q, none = torch.randn(2 * ql, h, hd, device=dev).to(dtype), torch.empty(0, h, hd, device=dev, dtype=dtype)
+    empty, tab = pkg.Kv4Cache(0, h, hd), pkg.attention_table([ql, ql], [0, 0])
+    pkg.kv4_append(empty, none, none)
+    assert pkg.kv4_read(empty)[0].shape == (0, h, hd)
+    for seqs, mk in ((tab, 0), (tab, 70), (None, 0)):
+        for out, lse in (pkg.cross_attention(q, none, none, seqs, ql, mk, return_lse=True),
+                         pkg.kv4_attention(q, empty, seqs, ql, mk, return_lse=True)):
+            assert (out == 0).all() and (lse == -math.inf).all()
+    ks, vs = torch.randn(2, 2 * ql, h, hd, device=dev).to(dtype).unbind(0)
+    out, lse = pkg.kv4_attention(q, empty, tab, ql, 0, k_self=ks, v_self=vs, return_lse=True)
+    check(out, lse, reference(q, none, none, tab.tolist(), 1 / math.sqrt(hd), ks=ks, vs=vs))
+    k = torch.randn(5, h, hd, device=dev).to(dtype)
+    for seqs in (pkg.attention_table([], []), pkg.attention_table([0, 0], [2, 3])):
+        out, lse = pkg.cross_attention(none, k, k, seqs, 3, 3, return_lse=True)
+        assert out.shape == (0, h, hd) and lse.shape == (0, h)
+
+
+def test_python_arguments_out_of_range(pkg, dev):
+    q = torch.zeros(2, 4, 64, device=dev)
+    tab = pkg.attention_table([2], [2])
+    for kw in (dict(max_q_len=2 ** 40), dict(max_k_len=-2 ** 40), dict(scale=1e39), dict(scale=math.inf), dict(v=None),
+               dict(v=q.cpu().numpy()), dict(gate=[1.0]), dict(out="q")):
+        args = dict(q=q, k=q, v=q, seqs=tab, max_q_len=2, max_k_len=2) | kw
+        with pytest.raises(pkg.IrodoriError):
+            pkg.cross_attention(**args)
+    c = pkg.Kv4Cache(4, 4, 64)
+    for call in (lambda: pkg.kv4_append(c, q, q, row_start=2 ** 64), lambda: pkg.kv4_append(c, q, q, row_start=3),
+                 lambda: pkg.kv4_read(c, row_start=2 ** 64, rows=1), lambda: pkg.kv4_read(c, rows=5),
+                 lambda: pkg.kv4_append(c, q, None), lambda: pkg.kv4_attention(q, None, tab, 2, 2)):
+        with pytest.raises(pkg.IrodoriError):
+            call()
+    assert (pkg.kv4_read(c)[0] == 0).all()
+
+
+FIRST = """
+import importlib.util, sys, torch
+spec = importlib.util.spec_from_file_location("irodori_b200", sys.argv[1], submodule_search_locations=[sys.argv[2]])
+pkg = importlib.util.module_from_spec(spec); sys.modules["irodori_b200"] = pkg; spec.loader.exec_module(pkg)
+kind = sys.argv[3]
+dtype = torch.float32 if kind == "f32" else torch.bfloat16
+n = 1 if kind == "few" else 40
+torch.manual_seed(1)
+q, k = torch.randn(n, 4, 128, device="cuda").to(dtype), torch.randn(90, 4, 128, device="cuda").to(dtype)
+tab, cache, out = pkg.attention_table([n], [90]), pkg.Kv4Cache(90, 4, 128), torch.zeros_like(q)
+def step():
+    pkg.kv4_append(cache, k, k)
+    pkg.cross_attention(q, k, k, tab, n, 90, out=out)
+    got = pkg.kv4_attention(q, cache, tab, n, 90)
+    kk, _ = pkg.kv4_read(cache, dtype=dtype)
+    return out, got, kk
+torch.cuda.synchronize()
+gr = torch.cuda.CUDAGraph()
+with torch.cuda.graph(gr):
+    captured = step()
+gr.replay()
+torch.cuda.synchronize()
+captured = [x.clone() for x in captured]
+for a, b in zip(captured, step()):
+    assert torch.equal(a, b) and a.abs().sum() > 0
+pkg.attention_check(0)
+print("same")
+"""
+
+
+@pytest.mark.parametrize("kind", ["few", "bf16", "f32"])
+def test_the_first_calls_of_a_process_may_be_captured(pkg, dev, kind):
+    import pathlib
+    import subprocess
+    import sys
+
+    init = pathlib.Path(pkg.__file__)
+    r = subprocess.run([sys.executable, "-c", FIRST, str(init), str(init.parent), kind], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
