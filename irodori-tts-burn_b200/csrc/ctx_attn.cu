@@ -9,12 +9,20 @@
 // (maximum, sum, output) triples are merged in a fixed order: results do not
 // depend on timing, and no workspace is needed.
 #include <algorithm>
+#include <type_traits>
 
 #include "ctx_attn.cuh"
+#include "tc_common.cuh"
 
 namespace irt {
 
 namespace {
+
+using tcx::ex2;
+using tcx::f2_add;
+using tcx::f2_fma;
+using tcx::f2_pack;
+using tcx::f2_unpack;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -22,17 +30,40 @@ constexpr int ROW_WARPS = 8;
 
 struct RowArgs {
   CtxAttnParams p;
-  int lanes;  // lanes that share a key: a power of two >= head_dim / 8
+  int lanes;  // lanes that share a key: a power of two >= head_dim / (8 VC)
   int split;  // CTAs of a cluster over the keys of one row block
   int q_vec, k_vec, v_vec, ks_vec, vs_vec, out_vec;
+  int wide;  // a lane's two chunks of codes are one load
 };
 
+// Eight values as packed pairs.
+__device__ __forceinline__ void pairs(const float (&x)[8], uint64_t (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = f2_pack(__float_as_uint(x[2 * i]), __float_as_uint(x[2 * i + 1]));
+}
+// Eight codes u as pairs of f32 u - 8, exact: a code under the exponent of 2^23
+// is 2^23 + u.
+__device__ __forceinline__ void code_pairs(uint32_t w, uint64_t (&r)[4]) {
+  const uint64_t off = f2_pack(0xcb000008u, 0xcb000008u);  // -(2^23 + 8)
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r[i] = f2_add(f2_pack(((w >> (8 * i)) & 0xfu) | 0x4b000000u, ((w >> (8 * i + 4)) & 0xfu) | 0x4b000000u), off);
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float bf_value(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+
 // R packed query rows (query x grouped head) of one KV head per CTA.  A key is
-// held by `lanes` lanes, eight values each; a warp works on 32 / lanes keys at
-// a time, U of them in flight per lane group, each group with its own running
-// maximum.
-template <bool BF, bool CTX4, int R, int U>
-__global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __grid_constant__ RowArgs a) {
+// held by `lanes` lanes, VC chunks of eight values each; a warp works on
+// 32 / lanes keys at a time, U of them in flight per lane group, each group
+// with its own running maximum.  4-bit context: a lane's chunks are side by
+// side within a group of 32, whose scale goes to the score and to the weight;
+// the codes of the next keys are read meanwhile.
+template <bool BF, bool CTX4, int R, int U, int VC>
+__global__ void __launch_bounds__(32 * ROW_WARPS, 2) ctx_attn_rows_kernel(const __grid_constant__ RowArgs a) {
   const CtxAttnParams& p = a.p;
   irt_attn_seq sd;
   if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
@@ -48,80 +79,155 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int LK = a.lanes, sub = lane / LK, o = lane % LK, per = 32 / LK;
-  const bool on = 8 * o < hd;
+  auto at = [&](int c) { return 8 * (CTX4 ? o * VC + c : o + LK * c); };  // first value of a chunk
   const float qscale = p.scale * LOG2E;
-  float q[R][8], acc[R][8], m[R], l[R];
+  uint64_t q[R][VC][4], acc[R][VC][4];
+  float m[R], l[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int pr = row0 + r;
-    const bool ok = on && pr < sd.q_len * G;
-    if (ok)
-      load8<BF>(p.q.data, (sd.q_start + pr / G) * p.q.row_stride + (hk * G + pr % G) * p.q.head_stride + 8 * o, a.q_vec,
-                q[r]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (!ok) q[r][j] = 0.f;
-      acc[r][j] = 0.f;
+    for (int c = 0; c < VC; ++c) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      if (at(c) < hd && pr < sd.q_len * G)
+        load8<BF>(p.q.data, (sd.q_start + pr / G) * p.q.row_stride + (hk * G + pr % G) * p.q.head_stride + at(c), a.q_vec,
+                  x);
+      pairs(x, q[r][c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[r][c][i] = 0;
     }
     m[r] = -INFINITY;
     l[r] = 0.f;
   }
-  const int n_self = p.ks.data ? sd.q_len : 0;
-  const int nk = n_self + sd.k_len;
-  const int chunk = per * U;
-  for (int c0 = (rank * ROW_WARPS + warp) * chunk; c0 < nk; c0 += split * ROW_WARPS * chunk) {
-    float k[U][8], v[U][8];
-    bool ok[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = c0 + u * per + sub;
-      const long row = j < n_self ? (long)sd.q_start + j : (long)sd.k_start + (j - n_self);
-      ok[u] = j < nk && (j < n_self || !p.mask || p.mask[row]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) k[u][i] = v[u][i] = 0.f;
-      if (ok[u] && on) {
-        if (j < n_self) {
-          load8<BF>(p.ks.data, row * p.ks.row_stride + hk * p.ks.head_stride + 8 * o, a.ks_vec, k[u]);
-          load8<BF>(p.vs.data, row * p.vs.row_stride + hk * p.vs.head_stride + 8 * o, a.vs_vec, v[u]);
-        } else if (CTX4) {
-          const long cr = (long)hk * p.k_rows + row;
-          const int g = kv4_groups(hd);
-          kv4_unpack8(*reinterpret_cast<const uint32_t*>(p.kc + cr * (hd / 2) + 4 * o),
-                      reinterpret_cast<const uint16_t*>(p.kscale)[cr * g + o / 4], k[u]);
-          kv4_unpack8(*reinterpret_cast<const uint32_t*>(p.vc + cr * (hd / 2) + 4 * o),
-                      reinterpret_cast<const uint16_t*>(p.vscale)[cr * g + o / 4], v[u]);
-        } else {
-          load8<BF>(p.k.data, row * p.k.row_stride + hk * p.k.head_stride + 8 * o, a.k_vec, k[u]);
-          load8<BF>(p.v.data, row * p.v.row_stride + hk * p.v.head_stride + 8 * o, a.v_vec, v[u]);
-        }
-      }
-    }
+
+  // U keys of each lane group: scores times ks, weights times vs
+  auto step = [&](const uint64_t (&k)[U][VC][4], const float (&ks)[U], const uint64_t (&v)[U][VC][4],
+                  const float (&vs)[U], const bool (&ok)[U], auto scaled) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float s[U];
       float mx = m[r];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float d = 0.f;
+        uint64_t d2 = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d = fmaf(q[r][i], k[u][i], d);
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d2 = f2_fma(q[r][c][i], k[u][c][i], d2);
+        float d, d1;
+        f2_unpack(d2, d, d1);
+        d += d1;
+        if (scaled) d *= ks[u];
         for (int w = LK / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
         s[u] = ok[u] ? d * qscale : -INFINITY;
         mx = fmaxf(mx, s[u]);
       }
       const float base = mx == -INFINITY ? 0.f : mx;  // NaN scores stay NaN in p and the sum
-      const float corr = exp2f(m[r] - base);
-      m[r] = mx;
-      l[r] *= corr;
+      if (__any_sync(0xffffffffu, mx > m[r])) {
+        const float corr = ex2(m[r] - base);
+        m[r] = mx;
+        l[r] *= corr;
+        const uint64_t c2 = f2_pack(__float_as_uint(corr), __float_as_uint(corr));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[r][i] *= corr;
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[r][c][i] = f2_mul(acc[r][c][i], c2);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float e = exp2f(s[u] - base);
+        const float e = ex2(s[u] - base), f = scaled ? e * vs[u] : e;
         l[r] += e;
+        const uint64_t f2 = f2_pack(__float_as_uint(f), __float_as_uint(f));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(e, v[u][i], acc[r][i]);
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[r][c][i] = f2_fma(f2, v[u][c][i], acc[r][c][i]);
       }
+    }
+  };
+  const int chunk = per * U, first = (rank * ROW_WARPS + warp) * chunk + sub, stride = split * ROW_WARPS * chunk;
+  const float one[U] = {};
+  // native rows: the own ones (keys [0, q_len), unmasked), or the context
+  auto native = [&](const irt_rows& kr, const irt_rows& vr, int k_vec, int v_vec, long start, int n, const uint8_t* mask) {
+    for (int j0 = first; j0 - sub < n; j0 += stride) {
+      uint64_t k[U][VC][4], v[U][VC][4];
+      bool ok[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * per;
+        const long row = start + j;
+        ok[u] = j < n && (!mask || mask[row]);
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          float x[8], y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+          if (ok[u] && at(c) < hd) {
+            load8<BF>(kr.data, row * kr.row_stride + hk * kr.head_stride + at(c), k_vec, x);
+            load8<BF>(vr.data, row * vr.row_stride + hk * vr.head_stride + at(c), v_vec, y);
+          }
+          pairs(x, k[u][c]);
+          pairs(y, v[u][c]);
+        }
+      }
+      step(k, one, v, one, ok, std::false_type{});
+    }
+  };
+  if (p.ks.data) native(p.ks, p.vs, a.ks_vec, a.vs_vec, sd.q_start, sd.q_len, nullptr);
+  if constexpr (!CTX4) {
+    native(p.k, p.v, a.k_vec, a.v_vec, sd.k_start, sd.k_len, p.mask);
+  } else {
+    const int groups = kv4_groups(hd);
+    struct {
+      uint32_t k[U][VC], v[U][VC];
+      uint16_t ks[U], vs[U];
+      bool ok[U];
+    } next;
+    auto words = [&](const uint8_t* codes, bool in, uint32_t (&w)[VC]) {
+#pragma unroll
+      for (int c = 0; c < VC; ++c) w[c] = 0;
+      if (!in) return;
+      if (VC == 2 && a.wide) {
+        const uint2 x = *reinterpret_cast<const uint2*>(codes);
+        w[0] = x.x; w[1 % VC] = x.y;
+      } else {
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+          if (at(c) < hd) w[c] = *reinterpret_cast<const uint32_t*>(codes + 4 * c);
+      }
+    };
+    auto fetch = [&](int j0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + u * per;
+        const long row = (long)sd.k_start + j, cr = (long)hk * p.k_rows + row;
+        next.ok[u] = j < sd.k_len && (!p.mask || p.mask[row]);
+        const bool in = next.ok[u] && at(0) < hd;
+        words(p.kc + cr * (hd / 2) + at(0) / 2, in, next.k[u]);
+        words(p.vc + cr * (hd / 2) + at(0) / 2, in, next.v[u]);
+        next.ks[u] = in ? reinterpret_cast<const uint16_t*>(p.kscale)[cr * groups + at(0) / KV4_GROUP] : 0;
+        next.vs[u] = in ? reinterpret_cast<const uint16_t*>(p.vscale)[cr * groups + at(0) / KV4_GROUP] : 0;
+      }
+    };
+    if (first - sub < sd.k_len) fetch(first);
+    for (int j0 = first; j0 - sub < sd.k_len; j0 += stride) {
+      const auto cur = next;
+      if (j0 - sub + stride < sd.k_len) fetch(j0 + stride);
+      uint64_t k[U][VC][4], v[U][VC][4];
+      float ks[U], vs[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        ks[u] = bf_value(cur.ks[u]);
+        vs[u] = bf_value(cur.vs[u]);
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          code_pairs(cur.k[u][c], k[u][c]);
+          code_pairs(cur.v[u][c], v[u][c]);
+        }
+      }
+      step(k, ks, v, vs, cur.ok, std::true_type{});
     }
   }
 
@@ -130,15 +236,24 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
   for (int r = 0; r < R; ++r) {
     float mw = m[r];
     for (int w = LK; w < 32; w <<= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, w));
-    const float f = exp2f(m[r] - (mw == -INFINITY ? 0.f : mw));
+    const float f = ex2(m[r] - (mw == -INFINITY ? 0.f : mw));
     float lw = l[r] * f;
     for (int w = LK; w < 32; w <<= 1) lw += __shfl_xor_sync(0xffffffffu, lw, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float x = acc[r][i] * f;
-      for (int w = LK; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-      if (sub == 0 && on) part[(warp * R + r) * hd + 8 * o + i] = x;
-    }
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x, y;
+        f2_unpack(acc[r][c][i], x, y);
+        x *= f;
+        y *= f;
+        for (int w = LK; w < 32; w <<= 1) {
+          x += __shfl_xor_sync(0xffffffffu, x, w);
+          y += __shfl_xor_sync(0xffffffffu, y, w);
+        }
+        if (sub == 0 && at(c) < hd)
+          *reinterpret_cast<float2*>(part + (warp * R + r) * hd + at(c) + 2 * i) = make_float2(x, y);
+      }
     if (lane == 0) {
       pm[warp * R + r] = mw;
       pl[warp * R + r] = lw;
@@ -147,29 +262,31 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) ctx_attn_rows_kernel(const __g
   merge_partials<BF, R, ROW_WARPS>(p, sd, split, rank, hk, row0, sm, a.out_vec);
 }
 
-template <bool BF, bool CTX4, int R, int U>
+template <bool BF, bool CTX4, int R, int U, int VC>
 void launch_rows(const CtxAttnParams& p, cudaStream_t s) {
   RowArgs a{};
   a.p = p;
   a.lanes = 1;
-  while (a.lanes < p.hd / 8) a.lanes *= 2;
+  while (a.lanes * VC < p.hd / 8) a.lanes *= 2;
   a.q_vec = rows_vec(p.q, BF);
   a.k_vec = rows_vec(p.k, BF);
   a.v_vec = rows_vec(p.v, BF);
   a.ks_vec = rows_vec(p.ks, BF);
   a.vs_vec = rows_vec(p.vs, BF);
   a.out_vec = rows_vec(p.out, BF) && (!p.gate.data || rows_vec(p.gate, BF));
+  a.wide = p.hd % 16 == 0;
   const long blocks = ((long)p.max_q * p.G + R - 1) / R;
   const long ctas = blocks * p.Hkv * p.nseq;
   const long keys = (long)p.max_k + (p.ks.data ? p.max_q : 0);
   // Keys are split over a cluster while there are fewer than two CTAs per SM
-  // and every CTA keeps at least two chunks per warp.
+  // and every warp keeps a chunk (one query over 200 / 576 f32 rows 7.2 / 9.2
+  // us, 8.6 / 9.4 with two chunks, 7.6 / 9.4 with half a one).
   const int sms = device_sms();
   const long least = 2L * ROW_WARPS * U * (32 / a.lanes);
   a.split = 1;
-  while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 2L * sms && keys >= 2L * a.split * least) a.split *= 2;
+  while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 2L * sms && keys >= a.split * least) a.split *= 2;
   const size_t smem = (size_t)merge_floats(R, ROW_WARPS, p.hd) * sizeof(float);
-  auto kernel = ctx_attn_rows_kernel<BF, CTX4, R, U>;  // smem <= 37.3 KB (R = 4, head_dim 256)
+  auto kernel = ctx_attn_rows_kernel<BF, CTX4, R, U, VC>;  // smem <= 37.3 KB (R = 4, head_dim 256)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * a.split), p.Hkv, p.nseq);
   cfg.blockDim = dim3(32 * ROW_WARPS);
@@ -184,15 +301,23 @@ void launch_rows(const CtxAttnParams& p, cudaStream_t s) {
   IRT_CHECK_LAUNCH();
 }
 
+// Rows, keys in flight and chunks as measured, all with two CTAs an SM: 16
+// streams of 16 heads of 128 over 8192 f32 rows with 1 / 2 / 4 queries 324 / 392
+// / 611 us (reading them 328 us), without the split of U and VC by R 557 / 896 /
+// 1066; 4-bit rows 202 / 264 / 590 us (reading them 46 us: bound by unpacking
+// and multiplying in f32), one utterance of 576 9.4 / 11.6 / 13.9.  Twice the
+// chunks a lane took 175 / 243 / 531, but 11.0 / 14.5 / 27.4 there.
 template <bool BF>
 void rows_path(const CtxAttnParams& p, cudaStream_t s) {
-  const bool one = (long)p.max_q * p.G == 1;
+  const long rows = (long)p.max_q * p.G;
   if (p.kc) {
-    if (one) launch_rows<BF, true, 1, 4>(p, s);
-    else launch_rows<BF, true, 4, 2>(p, s);
+    if (rows == 1) launch_rows<BF, true, 1, 2, 2>(p, s);
+    else if (rows == 2) launch_rows<BF, true, 2, 1, 2>(p, s);
+    else launch_rows<BF, true, 4, 1, 1>(p, s);
   } else {
-    if (one) launch_rows<BF, false, 1, 4>(p, s);
-    else launch_rows<BF, false, 4, 2>(p, s);
+    if (rows == 1) launch_rows<BF, false, 1, 3, 1>(p, s);
+    else if (rows == 2) launch_rows<BF, false, 2, 3, 1>(p, s);
+    else launch_rows<BF, false, 4, 2, 1>(p, s);
   }
 }
 

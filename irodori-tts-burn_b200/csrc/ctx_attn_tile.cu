@@ -6,9 +6,13 @@
 // One CTA = 64 (32) packed query rows (query x grouped head) of one KV head, in
 // tiles of 64 keys; 256 threads as 16 x 16, each with 4 x 4 (2 x 4) scores (rows
 // r + 16 i, keys c + 16 j) and 4 x HDT / 16 outputs, so both products run from
-// registers at 16 multiply-adds for each 16-byte shared-memory load, as packed
-// f32 pairs along the head dimension (half the instructions of scalar ones).
-// Bound by the FP32 pipe.  Query rows are scaled by scale log2(e) on the way
+// registers at 8 multiply-adds a thread for each 16-byte shared-memory load, as
+// packed f32 pairs along the head dimension (half the instructions of scalar
+// ones).  Bound by the FP32 pipe (61 %) and shared-memory passes (73 %): two
+// sequences of 750 queries over 576 rows 223 us, with own rows and a 4-bit
+// context 524 us, 31 to 33 TFLOP/s.  8 x 4 scores a thread halve the passes and
+// the warps: 241 us.  f32 halves on the tensor cores are out: their
+// accumulators truncate, and scores need the error of f32 sums.  Query rows are scaled by scale log2(e) on the way
 // in.  K of the next tile is loaded during softmax and P V, V during the next
 // scores.  Shared rows of Q, K, V are f32, their 16-byte chunks XOR-swizzled by
 // the row against bank conflicts.
@@ -416,8 +420,10 @@ void launch_hd(const CtxAttnParams& p, cudaStream_t s) {
 }  // namespace
 
 bool ctx_attention_tile(const CtxAttnParams& p, cudaStream_t s) {
-  // Up to 8 rows the row kernel reads the keys once or twice and has no idle threads.
-  if (p.hd > 128 || (long)p.max_q * p.G <= 8) return false;
+  // Fewer rows are the row kernel's: 16 streams over 8192 f32 rows, 8 / 12 packed
+  // rows 1176 / 1765 us there and 1530 us here; 4-bit rows, 8 / 12 / 16 packed
+  // rows 1172 / 1757 / 2340 us there and 1935 us here.
+  if (p.hd > 128 || (long)p.max_q * p.G <= (p.kc ? 12 : 8)) return false;
   if (p.bf16_io) {
     if (p.kc) launch_hd<true, true>(p, s);
     else launch_hd<true, false>(p, s);
