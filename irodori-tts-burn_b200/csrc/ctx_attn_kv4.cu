@@ -1,11 +1,12 @@
 // Attention of few query rows over a 4-bit context cache (bf16, head_dim 64 or
 // 128, up to 16 packed query rows a KV head): the newest frames of a stream
-// against its context.
+// against its context.  More rows than 16 are faster on tcgen05, which unpacks
+// a tile once for up to 128 of them.
 //
 // Bound by reading the cache, 4.5 bits a value, and nearly as much by taking
 // the codes apart: 7 integer instructions for 8 codes, 65 % of that pipe at
-// 4.66 TB/s (0.71 of the copy peak; 16 streams over 20000 to 32768 rows in
-// 217 us).  Codes go into mma.sync.m16n8k16 as integers
+// 4.95 TB/s (0.75 of the copy peak; 16 streams over 20000 to 32768 rows in
+// 205 us; one frame over 576 rows 6.5 us).  Codes go into mma.sync.m16n8k16 as integers
 // and the scales, constant over 32 values of a key, are applied to the sums:
 //   score(q, j)  = sum_G sK[j][G] * (sum_{d in G} q_d c_jd)
 //   out(q, d)    = sum_j (p_qj sV[j][G(d)]) c_jd

@@ -24,6 +24,16 @@
 // Few query tiles: the key tiles of one query tile are shared by a cluster of
 // 2, 4 or 8 CTAs, which merge their (m, l, O) through distributed shared
 // memory in rank order.  No workspace, no atomics.
+//
+// Many queries: bound by the latency of a CTA's chain (load, scores, softmax,
+// product, rows out), of which an SM runs two: 256 of its 512 TMEM columns
+// each, for two score tiles and O.  About 7.4 us a CTA and 0.8 us a key tile:
+// 64 x 16 heads, 768 queries over 64 / 640 / 1280 keys 171 / 320 / 541 us, the
+// last at 0.95 PFLOP/s; 64 utterances of 50 to 750 frames over 141 to 632 rows
+// 164 us.  4-bit context with own rows 387 us, there also bound by the issue of
+// instructions of the code warps.  One query: bound by reading K and V, 6.1
+// TB/s over 5000 to 8192 rows.  Fewer keys a tile would leave the tensor pipe
+// waiting for softmax; 128 would need both halves of TMEM for one CTA.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -277,7 +287,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       // the swizzle.  The codes of a tile are read while the one before it is
       // written.  One small copy of the code: unrolled over tiles it outgrew
       // the instruction cache next to the softmax (64 utterances 523 us
-      // against 429 us).
+      // against 429 us before the other steps).
       constexpr int W = HDT / 16;   // words of eight codes per key and lane
       constexpr int NG = HDT / 64;  // groups of 32
       const bool is_v = warp >= 8;

@@ -137,7 +137,9 @@ __device__ __forceinline__ float amax8(const Raw<BF>& r) {
 // Two lanes hold a group, sixteen values each: one shuffle joins its maximum.
 // A CTA covers 64 rows of one head (NG groups a row), whose codes and scales
 // are contiguous in the cache; a thread's loads are in flight together.  Bound
-// by the issue of instructions for bf16 (2 bytes a value in, 4.5 bits out).
+// by the issue of instructions for bf16 (2 bytes a value in, 4.5 bits out;
+// about 17 instructions a value, 3.4 issued of 4 a clock): K and V of 25,600
+// rows of 16 heads of 128 in 66 us, 4.1 TB/s; f32 88 us, 5.4 TB/s; 576 rows 8 us.
 template <bool BF, int NG>
 __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __grid_constant__ Kv4Args a) {
   constexpr int HALVES = 2 * NG, N = KV4_TILE * HALVES / KV4_APPEND_THREADS;  // half groups of a row, missing ones included
@@ -197,6 +199,9 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __
   }
 }
 
+// A thread has one word of codes of several rows in flight and writes 16 (32)
+// bytes for each.  Bound by memory: 25,600 rows as above in 49 us, 5.5 TB/s;
+// f32 102 us, 4.7 TB/s.
 template <bool BF, int NG>
 __global__ void __launch_bounds__(KV4_READ_THREADS) kv4_read_kernel(const __grid_constant__ Kv4Args a) {
   constexpr int OCTS = 4 * NG, N = KV4_TILE * OCTS / KV4_READ_THREADS;
