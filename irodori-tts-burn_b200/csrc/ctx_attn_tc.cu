@@ -27,10 +27,10 @@
 //
 // Many queries: bound by the latency of a CTA's chain (load, scores, softmax,
 // product, rows out), of which an SM runs two: 256 of its 512 TMEM columns
-// each, for two score tiles and O.  About 7.4 us a CTA and 0.8 us a key tile:
-// 64 x 16 heads, 768 queries over 64 / 640 / 1280 keys 171 / 320 / 541 us, the
-// last at 0.95 PFLOP/s; 64 utterances of 50 to 750 frames over 141 to 632 rows
-// 164 us.  4-bit context with own rows 387 us, there also bound by the issue of
+// each, for two score tiles and O.  About 6.5 us a CTA and 0.9 us a key tile:
+// 64 x 16 heads, 768 queries over 64 / 640 / 1280 keys 139 / 317 / 546 us, the
+// last at 0.94 PFLOP/s; 64 utterances of 50 to 750 frames over 141 to 632 rows
+// 159 us.  4-bit context with own rows 339 us, there also bound by the issue of
 // instructions of the code warps.  One query: bound by reading K and V, 6.1
 // TB/s over 5000 to 8192 rows.  Fewer keys a tile would leave the tensor pipe
 // waiting for softmax; 128 would need both halves of TMEM for one CTA.
@@ -75,6 +75,7 @@ struct TcArgs {
   int log_gp; // heads packed into a query tile, a power of two
   int split;  // CTAs of the cluster
   int tma_out;  // a warp's 32 rows are a box of the output's map
+  int heads;    // head groups of the listed grid (see list_tiles), or 0
 };
 
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t acc) {
@@ -119,6 +120,53 @@ __device__ __forceinline__ void st_shared8_zero(uint32_t addr) {
   asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(addr), "r"(0) : "memory");
 }
 
+// Listed grids (4-bit context): ragged sequences of several query tiles are
+// numbered through, tile after tile, so that no CTA starts for a tile that its
+// sequence does not have.  The 20 warps of two CTAs fill the register file, and
+// an empty CTA held up the next one for about 7 us: 16 / 64 / 250 utterances of
+// 50 to 750 frames 113 / 382 / 1466 us, listed 100 / 339 / 1400 us.  The native
+// kernel leaves room, and looking for the tile costs what the empty CTAs do: 49
+// / 162 / 605 us, listed 48 / 161 / 691.
+// Tiles to start, QT packed rows (`group` heads a query) each: at least as many
+// as there are, since query ranges do not overlap.  0: the grid is [tiles of
+// max_q, head groups, sequences], because it is no larger, or there are too
+// many sequences to look through.
+constexpr int MAX_LISTED = 256;
+inline long list_tiles(const CtxAttnParams& p, int group, int QT) {
+  const long per = ((long)p.max_q * group + QT - 1) / QT, most = p.q_rows * group / QT + p.nseq;
+  return p.seqs && p.nseq <= MAX_LISTED && per > 1 && most < per * p.nseq ? most : 0;
+}
+// Sequence of listed tile `tile` and the tile's number in it, or -1 (the same
+// in every thread).  Called by whole warps.
+__device__ __forceinline__ int listed_tile(const CtxAttnParams& p, int tile, int group, int QT, irt_attn_seq& sd) {
+  const int lane = threadIdx.x % 32;
+  auto entry = [&](int n, irt_attn_seq& e) {
+    return n < p.nseq && ctx_attn_seq(p, n, e) ? (e.q_len * group + QT - 1) / QT : 0;
+  };
+  irt_attn_seq e, next{};
+  int t_next = entry(lane, next), before = 0;
+  for (int c = 0; c < p.nseq; c += 32) {
+    e = next;
+    const int t = t_next;
+    t_next = entry(c + 32 + lane, next);
+    int sum = t;
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, sum, w);
+      if (lane >= w) sum += o;
+    }
+    const uint32_t behind = __ballot_sync(0xffffffffu, before + sum > tile);
+    if (behind) {
+      const int f = __ffs(behind) - 1;
+      sd = {__shfl_sync(0xffffffffu, e.q_start, f), __shfl_sync(0xffffffffu, e.q_len, f),
+            __shfl_sync(0xffffffffu, e.k_start, f), __shfl_sync(0xffffffffu, e.k_len, f)};
+      return tile - before - __shfl_sync(0xffffffffu, sum - t, f);
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return -1;
+}
+
 template <int HDT, bool CTX4>
 __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     ctx_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKS,
@@ -137,11 +185,20 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   pdl_trigger();
   const CtxAttnParams& p = a.p;
   irt_attn_seq sd;
-  if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
   const int split = a.split, rank = blockIdx.x % split, lg = a.log_gp, gmask = (1 << lg) - 1;
-  const int q0 = (blockIdx.x / split) * (QT >> lg);  // first query of the tile
-  if (q0 >= sd.q_len) return;                       // the whole cluster
-  const int head0 = blockIdx.y << lg, hk = head0 / p.G;
+  int q0, head0;  // first query and first head of the tile
+  if (CTX4 && a.heads) {
+    const int tile = blockIdx.x / a.heads;
+    head0 = (blockIdx.x - tile * a.heads) << lg;
+    q0 = listed_tile(p, tile, 1 << lg, QT, sd) * (QT >> lg);
+    if (q0 < 0) return;
+  } else {
+    if (!ctx_attn_seq(p, blockIdx.z, sd)) return;
+    q0 = (blockIdx.x / split) * (QT >> lg);
+    if (q0 >= sd.q_len) return;  // the whole cluster
+    head0 = blockIdx.y << lg;
+  }
+  const int hk = head0 / p.G;
   const int rows = min(QT, (sd.q_len - q0) << lg);  // packed query rows of the tile
   const int n_self = p.ks.data ? (sd.q_len + KT - 1) / KT : 0;
   const int n_all = n_self + (sd.k_len + KT - 1) / KT;
@@ -696,11 +753,13 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
       a.split = n;
     }
   }
+  const long listed = CTX4 && a.split == 1 ? list_tiles(p, gp, QT) : 0;
+  if (listed && listed * (p.H / gp) < (1L << 31)) a.heads = p.H / gp;
   auto kernel = ctx_attn_tc_kernel<HDT, CTX4>;
   static std::atomic<uint64_t> told{0};
   allow_smem(kernel, C::SMEM, told);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(qtiles * a.split), p.H / gp, p.nseq);
+  cfg.gridDim = a.heads ? dim3((unsigned)(listed * a.heads)) : dim3((unsigned)(qtiles * a.split), p.H / gp, p.nseq);
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;

@@ -661,3 +661,37 @@ def test_the_first_calls_of_a_process_may_be_captured(pkg, dev, kind):
     r = subprocess.run([sys.executable, "-c", FIRST, str(init), str(init.parent), kind], capture_output=True, text=True,
                        timeout=300)
     assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("own_rows", [False, True])
+@pytest.mark.parametrize("n", [2, 32, 33, 70, 256, 257])
+def test_many_ragged_sequences(pkg, dev, four_bit, own_rows, n):
+    """Ragged batches whose sequences have none to four query tiles, with gaps between them, in another order than
+    their rows, and entries that are skipped at both ends and inside."""
+    if own_rows and not four_bit:
+        pytest.skip("cross attention has no own rows")
+    g = gen(dev, 95 + n)
+    h, hkv, hd, mq, mk = 4, 2, 64, 200, 60
+    r = torch.Generator().manual_seed(n)
+    ql = torch.randint(0, mq + 1, (n,), generator=r) * (torch.rand(n, generator=r) < 0.8)
+    kl = torch.randint(0, mk + 1, (n,), generator=r)
+    ql[n // 2], kl[n // 2] = mq, mk
+    seqs, nq, nk = table(ql.tolist(), kl.tolist(), 3, 1)
+    seqs = [seqs[i] for i in torch.randperm(n, generator=r).tolist()]
+    bad = [(0, mq + 1, 0, 1), (nq - 5, 6, 0, 1), (-1, 5, 0, 1), (0, 5, nk - 1, 2), (0, 5, 0, mk + 1), (0, -1, 0, 1)]
+    given = list(seqs)
+    for i in (0, len(given) // 2, len(given)):  # the batch stays within n + 3 entries
+        given.insert(i, bad[(n + i) % len(bad)])
+    q = torch.randn(nq, h, hd, device=dev, generator=g).to(BF)
+    fill, own = torch.full_like(q, 5.0), {}
+    if own_rows:
+        own["k_self"], own["v_self"] = torch.randn(2, nq, hkv, hd, device=dev, generator=g).to(BF).unbind(0)
+    if four_bit:
+        cache, k, v = make_cache(pkg, nk, hkv, hd, g, dev)
+        out, lse = pkg.kv4_attention(q, cache, device_table(given, dev), mq, mk, out=fill, return_lse=True, **own)
+    else:
+        k, v = torch.randn(2, nk, hkv, hd, device=dev, generator=g).to(BF).unbind(0)
+        out, lse = pkg.cross_attention(q, k, v, device_table(given, dev), mq, mk, out=fill, return_lse=True)
+    check(out, lse, reference(q, k, v, seqs, 1 / math.sqrt(hd), ks=own.get("k_self"), vs=own.get("v_self")), 5.0)
+    pkg.attention_check(0)
