@@ -116,9 +116,6 @@ __device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&v)[4]) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void st_shared8_zero(uint32_t addr) {
-  asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(addr), "r"(0) : "memory");
-}
 
 // Listed grids (4-bit context): ragged sequences of several query tiles are
 // numbered through, tile after tile, so that no CTA starts for a tile that its
@@ -476,11 +473,11 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         mx *= a.scale_log2;
         if (partial && (!CTX4 || own)) {  // V rows that do not count: zeros
           mbar_wait(V_FULL(j % NKV), (j / NKV) & 1);
-          for (int key = warp; key < KT; key += sm_warps)
-            if (!((key < 32 ? on0 >> key : on1 >> (key - 32)) & 1)) {
-              if (HDT == 128) st_shared8_zero(sV(j % NKV) + (lane >> 4) * C::HALF + key * 128 + (lane & 15) * 8);
-              else if (lane < 16) st_shared8_zero(sV(j % NKV) + key * 128 + lane * 8);
-            }
+          constexpr int CH = HDT / 8, KW = 32 / CH;  // 16-byte chunks of a row, rows of a warp at a time
+          const uint32_t at = sV(j % NKV) + (lane % CH >> 3) * C::HALF + (lane & 7) * 16;
+#pragma unroll 4
+          for (int key = warp * KW + lane / CH; key < KT; key += sm_warps * KW)
+            if (!((key < 32 ? on0 >> key : on1 >> (key - 32)) & 1)) st_shared16(at + key * 128, make_uint4(0, 0, 0, 0));
           fence_proxy_async();
         }
         float corr = 1.f;
