@@ -56,6 +56,9 @@ constexpr float LN2 = 0.6931471805599453f;
 template <int HDT, bool CTX4>
 struct Cfg {
   static constexpr int CODE_WARPS = CTX4 ? 4 : 0, THREADS = 192 + 32 * CODE_WARPS;
+  // The native kernel's 6 warps stay within 128 registers: with more, two CTAs
+  // fill the register file and a CTA's successor starts late (64 utterances 188
+  // us at 149 registers against 159).
   static constexpr uint32_t Q_HALF = QT * 128, Q_BYTES = Q_HALF * (HDT / 64);  // 64-column halves
   static constexpr uint32_t HALF = KT * 128, TILE = HALF * (HDT / 64);
   static constexpr uint32_t OFF_K = Q_BYTES, OFF_V = OFF_K + NKV * TILE, OFF_BAR = OFF_V + NKV * TILE;
