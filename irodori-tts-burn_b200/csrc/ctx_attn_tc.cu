@@ -732,7 +732,6 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
   if (p.k.data && p.k_rows > 0 &&
       (!rows_map(k, p.k, p.k_rows, p.Hkv, p.hd, 1, KT) || !rows_map(v, p.v, p.k_rows, p.Hkv, p.hd, 1, KT)))
     return false;
-  a.tma_out = gp <= 32 && rows_map(o, p.out, p.q_rows, p.H, p.hd, gp, 32 / gp);
   const int sms = device_sms();
   const long qtiles = ((long)p.max_q * gp + QT - 1) / QT;
   const long ctas = qtiles * (p.H / gp) * p.nseq;
@@ -753,6 +752,8 @@ bool launch(const CtxAttnParams& p, cudaStream_t s) {
       a.split = n;
     }
   }
+  a.tma_out = a.split == 1 && (long)p.max_q * gp >= 32 && gp <= 32 &&
+              rows_map(o, p.out, p.q_rows, p.H, p.hd, gp, 32 / gp);
   const long listed = CTX4 && a.split == 1 ? list_tiles(p, gp, QT) : 0;
   if (listed && listed * (p.H / gp) < (1L << 31)) a.heads = p.H / gp;
   auto kernel = ctx_attn_tc_kernel<HDT, CTX4>;

@@ -2,15 +2,23 @@
 //
 // A group of 32 values of one row of one KV head is s * c, c in [-7, 7], s of
 // 5 significant bits: s = min{t : 7 t >= max|x|}.  c = x / s rounded half away
-// from zero.  Both are decided by comparisons that are exact in f32: 7 t and
-// the borders (c + 1/2) s have at most 9 significant bits, so neither result
+// from zero.  Both are exact: 7 t and the borders (c + 1/2) s have at most 9
+// significant bits, so comparisons with them in f32 decide, and neither result
 // depends on how a quotient was rounded.  c s has at most 8 significant bits:
 // it is a bf16 number.
 #include "ctx_attn.cuh"
+#include "tc_common.cuh"
 
 namespace irt {
 
 namespace {
+
+using tcx::f2_add;
+using tcx::f2_fma;
+using tcx::f2_pack;
+using tcx::f2_unpack;
+
+__device__ __forceinline__ uint64_t f2_both(float x) { return f2_pack(__float_as_uint(x), __float_as_uint(x)); }
 
 constexpr float KV4_MIN_MAX = 7.88860905e-31f;  // 2^-100: smaller groups hold zeros
 constexpr float MAGIC = 12582912.f;              // 1.5 * 2^23: adding it rounds to a whole number
@@ -46,6 +54,28 @@ __device__ __forceinline__ float kv4_code(float x, float s, float half, float in
 __device__ __forceinline__ uint32_t kv4_pack(const float (&c)[8]) {
   const float lo = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + (MAGIC + 34952.f);  // 0x8888
   const float hi = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + (MAGIC + 34952.f);
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
+}
+
+// Eight bf16 values x as codes of scale s, inv a little above 1 / s (one part in
+// 2^20).  x and the borders (c + 1/2) s have at most 8 and 9 significant bits,
+// so x is on a border or at least one part in 2^9 away from it: inv takes the
+// former outwards and the latter nowhere.  Values i and i + 4 are a packed pair.
+__device__ __forceinline__ uint32_t kv4_codes_bf16(uint4 v, float inv) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const uint64_t inv2 = f2_both(inv), magic = f2_both(MAGIC), back = f2_both(-MAGIC), sixteen = f2_both(16.f);
+  uint64_t c[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    c[2 * i] = f2_pack(w[i] << 16, w[i + 2] << 16);
+    c[2 * i + 1] = f2_pack(w[i] & 0xffff0000u, w[i + 2] & 0xffff0000u);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = f2_add(f2_fma(c[i], inv2, magic), back);
+  const uint64_t word = f2_add(f2_fma(f2_fma(f2_fma(c[3], sixteen, c[2]), sixteen, c[1]), sixteen, c[0]),
+                               f2_both(MAGIC + 34952.f));  // 0x8888
+  float lo, hi;
+  f2_unpack(word, lo, hi);
   return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x5410);
 }
 
@@ -137,9 +167,9 @@ __device__ __forceinline__ float amax8(const Raw<BF>& r) {
 // Two lanes hold a group, sixteen values each: one shuffle joins its maximum.
 // A CTA covers 64 rows of one head (NG groups a row), whose codes and scales
 // are contiguous in the cache; a thread's loads are in flight together.  Bound
-// by the issue of instructions for bf16 (2 bytes a value in, 4.5 bits out;
-// about 17 instructions a value, 3.4 issued of 4 a clock): K and V of 25,600
-// rows of 16 heads of 128 in 66 us, 4.1 TB/s; f32 88 us, 5.4 TB/s; 576 rows 8 us.
+// by memory and, for bf16, the issue of instructions (2 bytes a value in, 4.5
+// bits out): K and V of 25,600 rows of 16 heads of 128 in 54 us, 5.0 TB/s (66 us
+// with the f32 values' exact remainders); f32 90 us, 5.3 TB/s; 576 rows 8 us.
 template <bool BF, int NG>
 __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __grid_constant__ Kv4Args a) {
   constexpr int HALVES = 2 * NG, N = KV4_TILE * HALVES / KV4_APPEND_THREADS;  // half groups of a row, missing ones included
@@ -176,7 +206,8 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __
       m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
       float s = kv4_scale(m), inv;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-      inv *= 0.9999996f;  // one part in 2.5e6 below, more than rcp.approx is off
+      // more than rcp.approx is off: one part in 2^20 above, or in 2.5e6 below
+      inv *= BF ? 1.00000095f : 0.9999996f;
       float hs = 0.5f * s;
       if (s == 0.f) {  // the values are too small: codes 0
         inv = 0.f;
@@ -187,11 +218,17 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __
       const int row = e / HALVES;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float x[8];
-        expand<BF>(raw[i][u], x);
+        uint32_t w;
+        if constexpr (BF) {
+          w = kv4_codes_bf16(raw[i][u].v[0], inv);
+        } else {
+          float x[8];
+          expand<BF>(raw[i][u], x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = kv4_code(x[j], s, hs, inv);
-        const uint32_t w = bad ? 0x99999999u : kv4_pack(x);
+          for (int j = 0; j < 8; ++j) x[j] = kv4_code(x[j], s, hs, inv);
+          w = kv4_pack(x);
+        }
+        if (bad) w = 0x99999999u;
         if (in[i][u]) *reinterpret_cast<uint32_t*>(codes + row * (a.hd / 2) + half * 8 + 4 * u) = w;
       }
       if (in[i][0] && !(half & 1)) scales[row * NG + half / 2] = __float2bfloat16_rn(s);

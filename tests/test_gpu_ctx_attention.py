@@ -401,6 +401,27 @@ def test_kv4_cache_holds_its_definition(pkg, dev, dtype, hd):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("exponent", [-99, 0, 124])
+def test_every_bf16_value_against_every_maximum(pkg, dev, dtype, exponent):
+    """All 128 largest magnitudes of a binade with all bf16 values of the six binades up to it: every border between
+    codes that a bf16 value can lie on or next to."""
+    sig = torch.arange(128, device=dev, dtype=torch.float64) / 128 + 1
+    vals = torch.cat([sig * 2.0 ** (exponent - i) for i in range(6)])
+    vals = torch.cat([vals, -vals, torch.zeros(31 - 2 * len(vals) % 31, device=dev, dtype=torch.float64)]).reshape(-1, 31)
+    x = torch.empty(128, len(vals), 32, device=dev, dtype=torch.float64)
+    x[:, :, 1:] = vals
+    top = (sig * 2.0 ** exponent)[:, None, None]
+    x = torch.where(x.abs() <= top, x, torch.zeros_like(x))
+    x[:, :, 0] = top[:, :, 0]
+    x = x.to(dtype)
+    assert torch.equal(x.double().abs().amax(-1, keepdim=True), top.expand(-1, len(vals), 1))
+    c = pkg.Kv4Cache(128, len(vals), 32)
+    pkg.kv4_append(c, x, -x)
+    k, v = pkg.kv4_read(c, dtype=F32)
+    assert torch.equal(k.double(), quantised(x)) and torch.equal(v.double(), quantised(-x))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_kv4_append_gathers_and_leaves_the_rest(pkg, dev, dtype):
     g = gen(dev, 2)
     h, hd = 5, 96
