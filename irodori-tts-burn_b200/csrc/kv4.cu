@@ -123,23 +123,11 @@ __device__ __forceinline__ void load_raw(const Kv4Side& sd, long off, bool in, R
     }
   }
 }
-template <bool BF>
-__device__ __forceinline__ void expand(const Raw<BF>& r, float (&x)[8]) {
-  const uint32_t a[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
-  if constexpr (BF) {
+// Eight f32 values.
+__device__ __forceinline__ void expand(const Raw<false>& r, float (&x)[8]) {
+  const uint32_t w[8] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w, r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(a[i] << 16);
-      x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
-    }
-  } else {
-    const uint32_t b[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = __uint_as_float(a[i]);
-      x[4 + i] = __uint_as_float(b[i]);
-    }
-  }
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
 }
 
 // Largest magnitude of eight values; NaN if one is NaN.
@@ -157,7 +145,7 @@ __device__ __forceinline__ float amax8(const Raw<BF>& r) {
     return max_nan(__bfloat162float(t.x), __bfloat162float(t.y));
   } else {
     float x[8], m = 0.f;
-    expand<BF>(r, x);
+    expand(r, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(x[j]));
     return m;
@@ -223,7 +211,7 @@ __global__ void __launch_bounds__(KV4_APPEND_THREADS) kv4_append_kernel(const __
           w = kv4_codes_bf16(raw[i][u].v[0], inv);
         } else {
           float x[8];
-          expand<BF>(raw[i][u], x);
+          expand(raw[i][u], x);
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = kv4_code(x[j], s, hs, inv);
           w = kv4_pack(x);
