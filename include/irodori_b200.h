@@ -281,7 +281,8 @@ typedef struct irt_rows {
 
 /* One sequence: queries [q_start, q_start + q_len) attend to the context rows
  * [k_start, k_start + k_len).  Context ranges may overlap (guidance variants
- * of one utterance read sub-ranges of the same rows); query ranges must not. */
+ * of one utterance read sub-ranges of the same rows); query ranges must not:
+ * of rows that two sequences share, some may be written by neither. */
 typedef struct irt_attn_seq {
   int32_t q_start, q_len, k_start, k_len;
 } irt_attn_seq;

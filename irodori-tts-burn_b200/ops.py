@@ -304,7 +304,9 @@ def cross_attention(q, k, v, seqs, max_q_len: int, max_k_len: int, key_mask=None
 
     ``seqs`` is an ``attention_table`` (or None: equal sequences of
     ``max_q_len`` query and ``max_k_len`` context rows, in order); ``max_q_len``
-    and ``max_k_len`` bound its lengths.  Query head h reads KV head
+    and ``max_k_len`` bound its lengths.  A table of your own may place
+    sequences anywhere and let them share context rows, but not query rows
+    (which of those are written is not defined).  Query head h reads KV head
     h // (heads // kv_heads).  ``key_mask`` uint8 / bool [k_rows]: non-zero =
     attend.  ``gate``, shaped like ``q``, is multiplied into the output.
     ``scale`` defaults to 1 / sqrt(head_dim).
