@@ -134,10 +134,9 @@ def _empty_like(side, t):
 
 def _keep(side, *tensors):
     """Keeps the allocator from handing out these tensors' memory before an explicit stream is done with them."""
-    if side is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(side)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(side)
 
 
 def attention_table(q_lens, k_lens, k_starts=None, device=0):
@@ -231,8 +230,11 @@ def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=
         idx = _plain("src_rows", src_rows, cache.device, _INT32, (n,))
     _row_range(cache, row_start, n)
     handle, side = _stream(stream, cache.device)
-    _check(lib().irt_kv4_append(cache.device, _dtype_code[k.dtype], cache._c, row_start, n, kr, vr, n_src, idx, handle))
-    _keep(side, k, v, src_rows, *cache.buffers)
+    status = lib().irt_kv4_append(cache.device, _dtype_code[k.dtype], cache._c, row_start, n, kr, vr, n_src, idx, handle)
+    if status:
+        _check(status)
+    if side is not None:
+        _keep(side, k, v, src_rows, *cache.buffers)
 
 
 def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=None):
@@ -249,11 +251,13 @@ def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=
     shape = (n, cache.kv_heads, cache.head_dim)
     k = _empty(side, shape, dtype, cache.device)
     v = _empty_like(side, k)
-    row = cache.kv_heads * cache.head_dim
-    _check(lib().irt_kv4_read(cache.device, _dtype_code[dtype], cache._c, row_start, n,
-                              _ROWS.pack(k.data_ptr(), row, cache.head_dim),
-                              _ROWS.pack(v.data_ptr(), row, cache.head_dim), handle))
-    _keep(side, *cache.buffers)
+    row, head, _ = k.stride()
+    status = lib().irt_kv4_read(cache.device, _dtype_code[dtype], cache._c, row_start, n,
+                                _ROWS.pack(k.data_ptr(), row, head), _ROWS.pack(v.data_ptr(), row, head), handle)
+    if status:
+        _check(status)
+    if side is not None:
+        _keep(side, *cache.buffers)
     return k, v
 
 
