@@ -30,7 +30,7 @@
 // each, for two score tiles and O.  About 6.5 us a CTA and 0.9 us a key tile:
 // 64 x 16 heads, 768 queries over 64 / 640 / 1280 keys 139 / 317 / 546 us, the
 // last at 0.94 PFLOP/s; 64 utterances of 50 to 750 frames over 141 to 632 rows
-// 159 us.  4-bit context with own rows 339 us, there also bound by the issue of
+// 157 us.  4-bit context with own rows 337 us, there also bound by the issue of
 // instructions of the code warps.  One query: bound by reading K and V, 6.1
 // TB/s over 5000 to 8192 rows.  Fewer keys a tile would leave the tensor pipe
 // waiting for softmax; 128 would need both halves of TMEM for one CTA.
