@@ -1,7 +1,9 @@
 // Attention of few query rows over a 4-bit context cache (bf16, head_dim 64 or
 // 128, up to 16 packed query rows a KV head): the newest frames of a stream
-// against its context.  More rows than 16 are faster on tcgen05, which unpacks
-// a tile once for up to 128 of them.
+// against its context.  tcgen05 unpacks a tile once for up to 128 rows: with 8 /
+// 16 / 24 rows, 16 streams over 20000 rows take 184 / 309 / 508 us here and 456
+// us there, over 576 rows 14 / 25 / 35 and 22 us, one stream over 576 rows 9 / 9
+// / 11 and 12 us.
 //
 // Bound by reading the cache, 4.5 bits a value, and nearly as much by taking
 // the codes apart: 7 integer instructions for 8 codes, 65 % of that pipe at
@@ -30,6 +32,7 @@
 // (no CTA barrier in the loop); warps and the CTAs of a cluster share the keys
 // and join their states at the end.
 #include <algorithm>
+#include <cmath>
 
 #include "ctx_attn.cuh"
 #include "tc_common.cuh"
@@ -472,12 +475,30 @@ void launch(void (*kernel)(Kv4RowArgs), const CtxAttnParams& p, cudaStream_t s) 
   const int sms = device_sms();
   const long blocks = ((long)p.max_q * p.G + R - 1) / R;
   const long ctas = blocks * p.Hkv * p.nseq;
-  // Keys are split over a cluster up to four times the two CTAs an SM holds,
-  // which evens out ragged sequences (16 streams x 16 heads of 20000 to 32768
-  // rows: 221 / 217 / 231 us at 2 / 4 / 8), while every warp keeps a tile (one
-  // frame over 576 rows: 9.1 / 8.2 / 6.8 / 7.4 us at 1 / 2 / 4 / 8).
-  a.split = 1;
-  while (a.split < MAX_SPLIT && ctas * a.split * 2 <= 8L * sms && p.max_k >= (long)a.split * WARPS * KEYS) a.split *= 2;
+  // Keys are shared by a cluster where that pays.  Microseconds, of a CTA that
+  // starts with the launch 6.8, of one that waits for its place what the work
+  // beside it leaves of them; `key` for a key of one head, twice that where two
+  // CTAs share an SM, in as many rounds of CTAs as it takes (the last one, if not
+  // full, counts the less the more there are); of the longest sequences what they
+  // are longer than the mean (the rows of the cache over the sequences); and the
+  // merge.  head_dim 128, 1 / 2 / 4 / 8 CTAs, 16 heads of 1 stream over
+  // 8192 rows 35.5 / 21.4 / 13.8 / 13.8 us; of 4 streams over 2000 13.0 / 10.3 /
+  // 10.5 / 15.5; of 16 over 576 11.2 / 16.3 / 26.5 / 49.4, over 20000 to 32768 215
+  // / 209 / 207 / 224.
+  const float key = 3.6e-3f * (HD == 64 ? 0.65f : 1.f) * (R == 8 ? 1.25f : 1.f);
+  const float places = 2.f * sms, longest = (float)p.max_k, mean = std::min(longest, (float)p.k_rows / p.nseq);
+  float best = 0.f;
+  for (int n = 1; n <= MAX_SPLIT && (n == 1 || p.max_k > (n / 2) * KEYS * WARPS / 2); n *= 2) {
+    const float rounds = ctas * n / places, share = ctas * n > sms ? 2.f : 1.f, one = mean / n * key;
+    const float late = std::max(0.f, rounds - 1.f) / (1.f + one * 2.f / 40.f);
+    const float all = std::max(1.f, rounds + 0.5f * (std::ceil(rounds) - rounds) / rounds) * one * share +
+                      (longest - mean) / n * key;
+    const float t = 6.8f * (1.f + late) + std::max(all, longest / n * key * share) + (n > 1 ? 0.8f + 0.15f * n : 0.f);
+    if (n == 1 || t < best) {
+      best = t;
+      a.split = n;
+    }
+  }
   static std::atomic<uint64_t> told{0};
   allow_smem(kernel, smem, told);
   cudaLaunchConfig_t cfg = {};
