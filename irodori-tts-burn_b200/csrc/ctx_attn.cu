@@ -424,6 +424,7 @@ void kv4_check_rows(const irt_kv4_cache& c, int dtype, long row_start, long n, c
   if (written && overlap(sk, sv)) throw arg_error("k overlaps v");
   Span buf[4];
   kv4_spans(c, buf);
+  if (reinterpret_cast<uintptr_t>(idx) % 4) throw arg_error("the source index must be aligned to 4 bytes");
   const Span si = span_of(idx, 4 * n);
   for (int i = 0; i < 4; ++i) {
     const std::string name = std::string("the cache's ") + KV4_NAMES[i];
