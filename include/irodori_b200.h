@@ -325,7 +325,9 @@ IRT_API int irt_cross_attention(const irt_attn_args* a, const irt_rows* k, const
  * tensor cores multiply it without a further rounding.
  * Codes c + 8 are packed two a byte, the even index in the low half; scales
  * are bf16.  Each KV head's rows are contiguous.  The buffers are the
- * caller's, aligned to 16 bytes.
+ * caller's, aligned to 16 bytes.  A caller that fills them may use any bf16
+ * scale: f32 calls read c s exactly, bf16 calls may round it to bf16 where it
+ * has more than 8 significant bits.
  */
 typedef struct irt_kv4_cache {
   int64_t rows;
@@ -344,7 +346,7 @@ IRT_API int irt_kv4_append(int device, int dtype, const irt_kv4_cache* cache, in
                            const irt_rows* k, const irt_rows* v, int64_t src_rows, const int32_t* src_index,
                            void* stream);
 /* The values that cache rows [row_start, row_start + n) hold, into rows 0..n
- * of k and v.  Exact in bf16 and f32. */
+ * of k and v.  Exact in f32; in bf16 too for the scales that append writes. */
 IRT_API int irt_kv4_read(int device, int dtype, const irt_kv4_cache* cache, int64_t row_start, int64_t n,
                          const irt_rows* k, const irt_rows* v, void* stream);
 /* Attention over [own rows | context rows of the cache].  k_self, v_self

@@ -73,9 +73,10 @@ inline bool rows_vec(const irt_rows& r, int bf16_io) {
 }
 
 // Eight codes u -> eight bf16 values (u - 8) s, in order.  Under the exponent
-// of 16 a code is the bf16 number 16 + u; (16 + u) s - 24 s is exact in one
-// fused step, since 24 s has at most 7 significant bits.  n2 = -24 s, twice.
-// BIG: 24 s is beyond bf16's range; (16 + u - 24) s in two exact steps.
+// of 16 a code is the bf16 number 16 + u; for a scale of 5 significant bits
+// (16 + u) s - 24 s is exact in one fused step, since 24 s has at most 7.  n2 =
+// -24 s, twice.  BIG: 24 s is not a bf16 number; (16 + u - 24) s in two steps,
+// the second one rounded where s has more than 5 bits.
 template <bool BIG>
 __device__ __forceinline__ uint4 kv4_bf16x8(uint32_t w, __nv_bfloat162 s2, __nv_bfloat162 n2) {
   const uint32_t lo = ((w << 3) & 0x78787878u) | 0x80808080u;                        // codes 0 2 4 6, low bytes
@@ -92,17 +93,12 @@ __device__ __forceinline__ uint4 kv4_bf16x8(uint32_t w, __nv_bfloat162 s2, __nv_
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// Eight codes (one word) of a 4-bit group with scale s, bf16 bits `sb`.
+// Eight codes (one word) of a 4-bit group with scale s, bf16 bits `sb`: exact
+// in f32 for every s.  A code u under the exponent of 2^23 is 2^23 + u.
 __device__ __forceinline__ void kv4_unpack8(uint32_t w, uint16_t sb, float (&x)[8]) {
-  const uint32_t s = (uint32_t)sb << 16 | sb;
-  const __nv_bfloat162 s2 = *reinterpret_cast<const __nv_bfloat162*>(&s);
-  const uint4 v = kv4_bf16x8<true>(w, s2, s2);
-  const uint32_t p[4] = {v.x, v.y, v.z, v.w};
+  const float s = __uint_as_float((uint32_t)sb << 16);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(p[i] << 16);
-    x[2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 8; ++i) x[i] = (__uint_as_float((w >> (4 * i) & 0xfu) | 0x4b000000u) - 8388616.f) * s;
 }
 
 // SMs of the current device, looked up once per device.

@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
               const uint32_t w[4] = {cur.w[e][g].x, cur.w[e][g].y, cur.w[e][g].z, cur.w[e][g].w};
               const int c0 = part * W + 4 * g;  // 16-byte chunk of the row
               const uint32_t at = row + (c0 >> 3) * C::HALF;
-              if (cur.s[e][g] < 0x7d00) {  // 2^123
+              // below 2^123 and of 5 significant bits, as append writes it; a caller's own may be any bf16 number
+              if (cur.s[e][g] < 0x7d00 && (cur.s[e][g] & 7) == 0) {
 #pragma unroll
                 for (int o = 0; o < 4; ++o)
                   st_shared16(at + ((((c0 + o) & 7) ^ (lane & 7)) << 4), kv4_bf16x8<false>(w[o], s2, n2));

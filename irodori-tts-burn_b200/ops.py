@@ -192,7 +192,11 @@ class Kv4Cache:
     @classmethod
     def from_buffers(cls, k_codes, k_scales, v_codes, v_scales) -> "Kv4Cache":
         """A cache over tensors of the caller: codes uint8 [kv_heads, rows,
-        head_dim / 2], scales bfloat16 [kv_heads, rows, ceil(head_dim / 32)]."""
+        head_dim / 2] (c + 8, the even index in the low half), scales bfloat16
+        [kv_heads, rows, ceil(head_dim / 32)].  ``kv4_append`` writes scales of
+        5 significant bits, whose values c s are bf16 numbers.  Scales of your
+        own may be any bf16 number: float32 calls read c s exactly, bfloat16
+        calls may round it to bfloat16."""
         self = cls.__new__(cls)
         self._set(k_codes, k_scales, v_codes, v_scales)
         return self
@@ -240,7 +244,8 @@ def kv4_append(cache: Kv4Cache, k, v, row_start: int = 0, src_rows=None, stream=
 def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=None):
     """The values that cache rows [row_start, row_start + rows) hold, as
     (k, v) [rows, kv_heads, head_dim] of ``dtype`` (bfloat16, the default, or
-    float32; exact in both)."""
+    float32; exact in both for scales of 5 significant bits, in float32 for
+    any)."""
     torch = _t()
     dtype = torch.bfloat16 if dtype is None else dtype
     if dtype not in _dtype_code:
