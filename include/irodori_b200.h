@@ -271,8 +271,10 @@ IRT_API int irt_codec_decode_noalloc(irt_codec* c, const float* latent, int32_t 
  * Rows of heads: element (row, head, d) of a tensor is at
  * data[row * row_stride + head * head_stride + d], strides in elements.
  * Types: irt_precision (IRT_PREC_BF16: bf16, IRT_PREC_F32: float) for every
- * tensor of a call; scores, softmax and sums are f32 in both.  Query head h
- * reads KV head h / (heads / kv_heads).  head_dim is a multiple of 8, 8..256.
+ * tensor of a call; scores, softmax and sums are f32 in both.  Weights are at
+ * most 1 before the normalisation: sums of values stay finite where the
+ * values' magnitudes, summed over the keys, do.  Query head h reads KV head
+ * h / (heads / kv_heads).  head_dim is a multiple of 8, 8..256.
  */
 typedef struct irt_rows {
   void* data;

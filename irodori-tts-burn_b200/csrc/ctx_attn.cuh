@@ -173,8 +173,9 @@ constexpr __host__ __device__ int merge_floats(int R, int W, int hd) { return (W
 // sm: part [W][R][hd], then pm [W][R] (base-2 maxima) and pl [W][R] (sums),
 // written by the warps; the rest is used here.  16-byte aligned.  Called by
 // every thread of every CTA of the cluster.  vec: rows of out and gate can be
-// accessed four values at a time.
-template <bool BF, int R, int W>
+// accessed four values at a time.  HEADROOM: how far (log2) the m_w lie above
+// the maxima; the log of the sum moves it over, so that it loses nothing to it.
+template <bool BF, int R, int W, int HEADROOM = 0>
 __device__ __forceinline__ void merge_partials(const CtxAttnParams& p, const irt_attn_seq& sd, int split, int rank,
                                                int hk, int row0, float* sm, bool vec) {
   namespace cg = cooperative_groups;
@@ -256,7 +257,9 @@ __device__ __forceinline__ void merge_partials(const CtxAttnParams& p, const irt
       x.x *= g.x; x.y *= g.y; x.z *= g.z; x.w *= g.w;
     }
     store4<BF>(p.out.data, row * p.out.row_stride + head * p.out.head_stride + d, vec, x);
-    if (p.lse && d == 0) p.lse[row * p.H + head] = lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
+    if (p.lse && d == 0)
+      p.lse[row * p.H + head] =
+          lt == 0.f ? -INFINITY : fmaf(mt - HEADROOM, LN2, logf(lt * (float)(1 << HEADROOM)));
   }
   if (split > 1) cluster.sync();  // the others may still read this CTA's part
 }

@@ -46,7 +46,9 @@ using tcx::pack_bf16x2;
 using tcx::smem_u32;
 
 constexpr int WARPS = 8, STAGES = 3, KEYS = 32, SUB = KEYS / 16;
-constexpr float RESCALE_LOG2 = 8.f;  // raise the running maximum only beyond 2^8 growth
+// m starts 2^8 above a row's maximum and is raised only when a score passes it:
+// weights are at most 1, and weights times scales no larger than the scales.
+constexpr int HEADROOM_LOG2 = 8;
 
 template <int NGR>
 struct Ring {
@@ -356,15 +358,16 @@ __global__ void __launch_bounds__(32 * WARPS, 2) ctx_attn_kv4_rows_kernel(const 
 #pragma unroll
       for (int i = 1; i < 2 * SUB; ++i) mx[n] = fmaxf(mx[n], sc[i / 2][i % 2][n]);
       mx[n] *= a.scale_log2;
-      raise |= mx[n] > m[n] + RESCALE_LOG2 || (m[n] == -INFINITY && mx[n] > -INFINITY);
+      raise |= mx[n] > m[n];
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        float mn = fmaxf(mx[n], m[n]);
+        float mn = mx[n];
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
-        const float corr = m[n] == -INFINITY ? 0.f : ex2(m[n] - mn);
+        mn = mn > m[n] ? mn + HEADROOM_LOG2 : m[n];
+        const float corr = m[n] == mn ? 1.f : ex2(m[n] - mn);
         m[n] = mn;
         l[n] *= corr;
 #pragma unroll
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(32 * WARPS, 2) ctx_attn_kv4_rows_kernel(const 
           *reinterpret_cast<float2*>(dst + 32 * G + 2 * mt) = make_float2(o[G][mt][k], o[G][mt][2 + k]);
     }
   }
-  merge_partials<true, R, WARPS>(p, sd, split, rank, hk, row0, part, a.out_vec);
+  merge_partials<true, R, WARPS, HEADROOM_LOG2>(p, sd, split, rank, hk, row0, part, a.out_vec);
 }
 
 template <int NGR, int R>

@@ -7,9 +7,10 @@
 // rows.  Warps:
 //   0..3  softmax: thread = query row.  Per tile: scores from TMEM, masked
 //         keys to -inf, P = exp2(s - m) as packed bf16 over the first half of
-//         the score buffer (the A operand of P V).  m is raised, and O rescaled,
-//         only when a row's maximum grows by more than 2^8.  Warps without a
-//         query row take no part.
+//         the score buffer (the A operand of P V).  m starts 2^8 above a row's
+//         maximum and is raised, and O rescaled, only when a score passes it, so
+//         weights are at most 1 and O no larger than the values' sum.  Warps
+//         without a query row take no part.
 //   4     TMA: Q once, K and V of native tiles (2-stage rings, K two tiles
 //         ahead of V).
 //   5     tcgen05.mma issue: S_j = Q K_j^T, O += P_j V_j.
@@ -50,7 +51,7 @@ namespace {
 using namespace tcx;
 
 constexpr int QT = 128, KT = 64, NKV = 2;
-constexpr float RESCALE_LOG2 = 8.f;
+constexpr float HEADROOM_LOG2 = 8.f;  // of m above the maximum when it is raised
 constexpr float LN2 = 0.6931471805599453f;
 
 template <int HDT, bool CTX4>
@@ -118,6 +119,11 @@ __device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&v)[4]) {
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                : "r"(addr)
                : "memory");
+}
+
+// m log 2 + log l, the headroom moved from one to the other: their sum loses nothing to it.
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return fmaf(m - HEADROOM_LOG2, LN2, logf(l * exp2f(HEADROOM_LOG2)));
 }
 
 // Listed grids (4-bit context): ragged sequences of several query tiles are
@@ -485,10 +491,11 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
           fence_proxy_async();
         }
         float corr = 1.f;
-        const bool raise = mx > m_run + RESCALE_LOG2 || (m_run == -INFINITY && mx > -INFINITY);
+        const bool raise = mx > m_run;
         if (raise) {
-          corr = m_run == -INFINITY ? 0.f : ex2(m_run - mx);
-          m_run = mx;
+          const float m_new = mx + HEADROOM_LOG2;
+          corr = ex2(m_run - m_new);
+          m_run = m_new;
         }
         const float nbase = m_run == -INFINITY ? 0.f : -m_run;
         // P_{j-1} V_{j-1} must be done before O is read; the phase in flight
@@ -593,7 +600,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       }
       if (qrow < rows && p.lse)
         p.lse[((long)sd.q_start + q0 + (qrow >> lg)) * p.H + head0 + (qrow & gmask)] =
-            l_run == 0.f ? -INFINITY : fmaf(m_run, LN2, logf(l_run));
+            l_run == 0.f ? -INFINITY : lse_of(m_run, l_run);
       constexpr int LPR = HDT / 8;  // lanes of a row
       const int chunk = lane % LPR;
       if (!boxes && 8 * chunk < p.hd) {
@@ -664,7 +671,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         if (c < split) wt[i * MAX_SPLIT + c] = m[c] * inv;
       if (p.lse)
         p.lse[((long)sd.q_start + q0 + (r >> lg)) * p.H + head0 + (r & gmask)] =
-            lt == 0.f ? -INFINITY : fmaf(mt, LN2, logf(lt));
+            lt == 0.f ? -INFINITY : lse_of(mt, lt);
     }
     __syncthreads();
     const int per_row = p.hd / 4;
