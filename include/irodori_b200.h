@@ -173,7 +173,8 @@ IRT_API int irt_engine_set_sampling(irt_engine* e, const irt_sampler_params* p);
  * bytes, projected and quantised a layer at a time; for batches whose context
  * rows bound the utterances in flight.  The context's values are rounded
  * (relative error about 0.1 each), the latents change accordingly.  Takes
- * effect with the next irt_engine_sample. */
+ * effect with the next irt_engine_sample, which gives the memory of the other
+ * mode's cache back. */
 typedef enum irt_ctx_cache { IRT_CTX_CACHE_NATIVE = 0, IRT_CTX_CACHE_4BIT = 1 } irt_ctx_cache;
 IRT_API int irt_engine_set_context_cache(irt_engine* e, int mode);
 /* with_default_sampling() (src/inference.rs:158-164). */

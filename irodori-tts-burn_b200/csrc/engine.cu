@@ -536,11 +536,7 @@ void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, i
     cudaError_t e = cudaGraphInstantiate(&ge, g, 0);
     cudaGraphDestroy(g);
     IRT_CUDA(e);
-    if (graphs.size() > 64) {  // bound the cache
-      for (auto& kv : graphs) cudaGraphExecDestroy(kv.second);
-      graphs.clear();
-      graph_kernels.clear();
-    }
+    if (graphs.size() > 64) drop_graphs();  // bound the cache
     graph_seen.erase(key);
     it = graphs.emplace(key, ge).first;
     // kernels recorded in the graph (captured launches are not executed)
@@ -549,6 +545,12 @@ void Engine::forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, i
   }
   IRT_CUDA(cudaGraphLaunch(it->second, s));
   launch_counter().fetch_add(graph_kernels[key]);
+}
+
+void Engine::drop_graphs() {
+  for (auto& kv : graphs) cudaGraphExecDestroy(kv.second);
+  graphs.clear();
+  graph_kernels.clear();
 }
 
 size_t Engine::cache4_layer_bytes(long rows) const {
@@ -908,6 +910,13 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
   const int nctx = base[B];
   const size_t lstride_el = (size_t)nctx * D;
   const bool kv4 = ctx_cache == IRT_CTX_CACHE_4BIT;
+  if (ctx_cache != ctx_cache_held) {  // the buffers of the other mode, and the graphs that read them, go
+    ws.cache_k.release();
+    ws.cache_v.release();
+    ws.cache4.release();
+    drop_graphs();
+    ctx_cache_held = ctx_cache;
+  }
   if (nctx > 0) {
     const int lp = kv4 ? 1 : L;  // layers that cache_k / cache_v hold
     ws.cache_k.ensure((size_t)lp * lstride_el * esz());

@@ -48,6 +48,7 @@ struct Engine {
   // bits (kv4.cu), projected and quantised one layer at a time, so that no
   // full-precision copy of the cache exists.
   int ctx_cache = IRT_CTX_CACHE_NATIVE;
+  int ctx_cache_held = IRT_CTX_CACHE_NATIVE;  // mode that the workspaces' cache buffers were made for
 
   // dimensions
   int D = 0, L = 0, H = 0, hd = 0, P = 0, F = 0, Fp = 0, R = 0, Temb = 0;
@@ -115,6 +116,7 @@ struct Engine {
   std::map<std::vector<uintptr_t>, cudaGraphExec_t> graphs;
   std::map<std::vector<uintptr_t>, int> graph_seen;
   std::map<std::vector<uintptr_t>, long long> graph_kernels;
+  void drop_graphs();
   DevBuf ada_cur;  // adaLN parameters of the current step, read by the graph
   void forward_step(int M, const SeqDesc* d_seqs, int nseq, int max_len, int max_ctx, int t_index, int nrows_ctx,
                     cudaStream_t s);
