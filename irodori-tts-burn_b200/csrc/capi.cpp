@@ -252,8 +252,9 @@ int irt_cross_attention(const irt_attn_args* a, const irt_rows* k, const irt_row
     need(a, "args");
     need(k, "k");
     need(v, "v");
-    const irt::CtxAttnParams p = irt::ctx_attn_params(*a, nullptr, k, v, k_rows, nullptr, nullptr);
+    irt::CtxAttnParams p = irt::ctx_attn_params(*a, nullptr, k, v, k_rows, nullptr, nullptr);
     irt::DeviceGuard dg(a->device);
+    p.expired = irt::ctx_attn_status();
     irt::ctx_attention(p, reinterpret_cast<cudaStream_t>(stream));
   });
 }
@@ -263,8 +264,9 @@ int irt_kv4_attention(const irt_attn_args* a, const irt_kv4_cache* cache, const 
   return guard([&] {
     need(a, "args");
     need(cache, "cache");
-    const irt::CtxAttnParams p = irt::ctx_attn_params(*a, cache, nullptr, nullptr, cache->rows, k_self, v_self);
+    irt::CtxAttnParams p = irt::ctx_attn_params(*a, cache, nullptr, nullptr, cache->rows, k_self, v_self);
     irt::DeviceGuard dg(a->device);
+    p.expired = irt::ctx_attn_status();
     irt::ctx_attention(p, reinterpret_cast<cudaStream_t>(stream));
   });
 }

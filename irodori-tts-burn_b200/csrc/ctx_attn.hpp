@@ -30,6 +30,10 @@ struct CtxAttnParams {
   const bf16 *kscale, *vscale;
   const uint8_t* mask;       // [k_rows] or null
   float* lse;                // [q_rows, H] or null
+  // Device memory that a bounded wait sets to 1 when it runs out; once it is
+  // set, every wait that reports here gives up at once.  The operators have one
+  // word per device (ctx_attn_status), an engine has its own.
+  int* expired;
 };
 
 // Range of sequence n; false when its table entry reaches outside the tensors
@@ -54,8 +58,12 @@ bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s);
 bool ctx_attention_kv4_rows(const CtxAttnParams& p, cudaStream_t s);
 // Many query rows in f32 arithmetic, head_dim <= 128 (ctx_attn_tile.cu); false as above.
 bool ctx_attention_tile(const CtxAttnParams& p, cudaStream_t s);
-// Bounded-wait flag of the tcgen05 kernels on the current device (0 = ok).
+// The operators' word for expired waits on the current device; reading clears it.
+int* ctx_attn_status();
 int read_and_clear_ctx_attn_error();
+// Test hook: `waits` bounded waits of the kernels on a barrier that nothing
+// arrives on, with a limit of limit_ns each, reported to `expired`.
+void ctx_attn_watchdog_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns, int* expired);
 
 // cache rows [row_start, row_start + n) from source rows idx[i] (or i); see
 // irt_kv4_append / irt_kv4_read.

@@ -101,6 +101,26 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
       : "memory");
 }
 
+// Bounded wait as tcx::mbar_wait, reported to `status` in the place of the
+// file's own flag.
+__device__ __forceinline__ void wait_or_report(uint32_t bar, uint32_t parity, int* status) {
+  if (mbar_try_wait(bar, parity)) return;
+  volatile int* flag = status;
+  if (*flag) return;
+  const uint64_t limit = *reinterpret_cast<volatile unsigned long long*>(&g_wait_limit_ns);
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (mbar_try_wait(bar, parity)) return;
+    if (*flag) return;
+    if (globaltimer() - t0 > limit) {
+      atomicExch(status, 1);
+      return;
+    }
+  }
+}
+
 // Box of a (d, head, row) tensor.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
@@ -223,6 +243,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   auto P_FULL = [&](int b) { return bar(5 + 4 * NKV + b); };
   const uint32_t G_FULL = bar(7 + 4 * NKV);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 4 * NKV);
+  auto bar_wait = [&](uint32_t b, uint32_t parity) { wait_or_report(b, parity, p.expired); };
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sm_warps = (rows + 31) / 32;  // softmax warps that have a query row
@@ -241,7 +262,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
 
   // K (V) rows of local tile j, by the TMA thread
   auto load = [&](int j, uint32_t full, uint32_t empty, uint32_t dst, const CUtensorMap* self, const CUtensorMap* ctx) {
-    mbar_wait(empty, ((j / NKV) & 1) ^ 1);
+    bar_wait(empty, ((j / NKV) & 1) ^ 1);
     const bool own = t0 + j < n_self;
     if (CTX4 && !own) {  // the code warps fill this one
       mbar_arrive(full);
@@ -300,7 +321,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
           load_v(j + 1);
         }
         if (split == 1 && p.gate.data) {  // the gate takes Q's place once the last scores are done
-          mbar_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1);
+          bar_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1);
           mbar_expect_tx(G_FULL, C::Q_BYTES);
 #pragma unroll
           for (int h = 0; h < HDT / 64; ++h)
@@ -310,11 +331,11 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     } else if (warp == 5) {
       // ---------------- MMA ----------------
       if (lane == 0) {
-        mbar_wait(Q_FULL, 0);
+        bar_wait(Q_FULL, 0);
         tc_fence_after();
         auto issue_s = [&](int j) {
           const int r = j % NKV, b = j & 1;
-          mbar_wait(K_FULL(r), (j / NKV) & 1);
+          bar_wait(K_FULL(r), (j / NKV) & 1);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < HDT / 16; ++kk) {
@@ -329,8 +350,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         if (nt > 1) issue_s(1);
         for (int j = 0; j < nt; ++j) {
           const int s = j & 1, r = j % NKV;
-          mbar_wait(V_FULL(r), (j / NKV) & 1);
-          mbar_wait(P_FULL(s), (j >> 1) & 1);
+          bar_wait(V_FULL(r), (j / NKV) & 1);
+          bar_wait(P_FULL(s), (j >> 1) & 1);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < KT / 16; ++kk) {
@@ -385,7 +406,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         const Codes cur = next;
         if (j + 1 < nt) fetch(j + 1);
         const int r = j % NKV;
-        mbar_wait(is_v ? V_EMPTY(r) : K_EMPTY(r), ((j / NKV) & 1) ^ 1);
+        bar_wait(is_v ? V_EMPTY(r) : K_EMPTY(r), ((j / NKV) & 1) ^ 1);
         if (t0 + j >= n_self) {
           const uint32_t dst = is_v ? sV(r) : sK(r);
 #pragma unroll
@@ -446,7 +467,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         }
         fetch_mask(j + 1);
         const bool partial = (on0 & on1) != 0xffffffffu;
-        mbar_wait(S_FULL(b), (j >> 1) & 1);
+        bar_wait(S_FULL(b), (j >> 1) & 1);
         tc_fence_after();
         // Scores in halves of 32 columns.  One register copy of a tile's scores
         // (native context), or two readings of them: 96 registers a thread
@@ -482,7 +503,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         }
         mx *= a.scale_log2;
         if (partial && (!CTX4 || own)) {  // V rows that do not count: zeros
-          mbar_wait(V_FULL(j % NKV), (j / NKV) & 1);
+          bar_wait(V_FULL(j % NKV), (j / NKV) & 1);
           constexpr int CH = HDT / 8, KW = 32 / CH;  // 16-byte chunks of a row, rows of a warp at a time
           const uint32_t at = sV(j % NKV) + (lane % CH >> 3) * C::HALF + (lane & 7) * 16;
 #pragma unroll 4
@@ -501,7 +522,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         // P_{j-1} V_{j-1} must be done before O is read; the phase in flight
         // is j - 1 or already j
         if (__any_sync(0xffffffffu, raise) && j > 0) {
-          mbar_wait(O_DONE, (j - 1) & 1);
+          bar_wait(O_DONE, (j - 1) & 1);
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < HDT / 32; ++c) {
@@ -539,7 +560,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(P_FULL(b));
       }
-      mbar_wait(O_FINAL, 0);
+      bar_wait(O_FINAL, 0);
       tc_fence_after();
     }
   }
@@ -556,7 +577,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       const bool gated = p.gate.data && nt > 0;
-      if (gated) mbar_wait(G_FULL, 0);
+      if (gated) bar_wait(G_FULL, 0);
 #pragma unroll 1
       for (int c = 0; c < HDT; c += 32) {
         uint32_t r[32], g[4][4];
@@ -799,6 +820,41 @@ bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s) {
   return p.hd > 64 ? launch<128, false>(p, s) : launch<64, false>(p, s);
 }
 
+int* ctx_attn_status() {
+  static std::atomic<int*> known[64];
+  int dev = 0;
+  IRT_CUDA(cudaGetDevice(&dev));
+  int* p = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (!p) {
+    IRT_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_watchdog));
+    if (dev < 64) known[dev].store(p, std::memory_order_relaxed);
+  }
+  return p;
+}
+
 int read_and_clear_ctx_attn_error() { return read_and_clear_flag(); }
+
+namespace {
+__global__ void wait_probe_kernel(int waits, int* expired, unsigned long long* elapsed_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar), 1);
+    const uint64_t t0 = globaltimer();
+    for (int i = 0; i < waits; ++i) wait_or_report(smem_u32(&bar), 0, expired);  // phase 0 never completes
+    *elapsed_ns = globaltimer() - t0;
+  }
+}
+}  // namespace
+
+void ctx_attn_watchdog_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns, int* expired) {
+  DevBuf d(sizeof(*elapsed_ns));
+  IRT_CUDA(set_wait_limit_ns(limit_ns));
+  wait_probe_kernel<<<1, 32>>>(waits, expired, d.as<unsigned long long>());
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  IRT_CUDA(set_wait_limit_ns(DEFAULT_WAIT_LIMIT_NS));
+  IRT_CUDA(e);
+  IRT_CUDA(cudaMemcpy(elapsed_ns, d.p, sizeof(*elapsed_ns), cudaMemcpyDeviceToHost));
+}
 
 }  // namespace irt

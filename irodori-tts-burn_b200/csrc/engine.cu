@@ -636,6 +636,7 @@ void Engine::dit_forward(int M, const SeqDesc* d_seqs, int nseq, int max_len, in
       cp.vc = c4.v_codes;
       cp.kscale = reinterpret_cast<const bf16*>(c4.k_scales);
       cp.vscale = reinterpret_cast<const bf16*>(c4.v_scales);
+      cp.expired = ctx_expired.as<int>();
       ctx_attention(cp, s);
     } else {
       attention(ap, bf, s);
@@ -910,6 +911,20 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
   const int nctx = base[B];
   const size_t lstride_el = (size_t)nctx * D;
   const bool kv4 = ctx_cache == IRT_CTX_CACHE_4BIT;
+  if (kv4 && !ctx_expired.p) {
+    ctx_expired.alloc(sizeof(int));
+    IRT_CUDA(cudaMemsetAsync(ctx_expired.p, 0, sizeof(int), s));
+  }
+  struct AtRest {  // a call that fails leaves no expired wait for the next one
+    const DevBuf& word;
+    cudaStream_t s;
+    bool clear;
+    ~AtRest() {
+      if (!clear || !word.p) return;
+      cudaMemsetAsync(word.p, 0, sizeof(int), s);
+      cudaStreamSynchronize(s);
+    }
+  } at_rest{ctx_expired, s, kv4};
   if (ctx_cache != ctx_cache_held) {  // the buffers of the other mode, and the graphs that read them, go
     ws.cache_k.release();
     ws.cache_v.release();
@@ -1277,9 +1292,15 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
   } else {
     IRT_CUDA(cudaMemcpyAsync(out, xs, nel * 4, okind, s));
   }
+  int ctx_late = 0;
+  if (kv4) IRT_CUDA(cudaMemcpyAsync(&ctx_late, ctx_expired.p, sizeof(int), cudaMemcpyDeviceToHost, s));
   IRT_CUDA(cudaStreamSynchronize(s));
-  if (read_and_clear_kernel_error() | read_and_clear_attn_error() | read_and_clear_ctx_attn_error())
+  if (read_and_clear_kernel_error() | read_and_clear_attn_error())
     throw Error(IRT_E_CUDA, "a GEMM pipeline wait timed out (device watchdog); results are invalid");
+  if (ctx_late)
+    throw Error(IRT_E_CUDA,
+                "a wait of the attention over the 4-bit context cache timed out (device watchdog); results are invalid");
+  at_rest.clear = false;
   last_launches = launch_counter().load() - launches0;
 }
 

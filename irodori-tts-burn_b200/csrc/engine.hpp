@@ -48,6 +48,9 @@ struct Engine {
   // bits (kv4.cu), projected and quantised one layer at a time, so that no
   // full-precision copy of the cache exists.
   int ctx_cache = IRT_CTX_CACHE_NATIVE;
+  // where the attention over that cache reports a wait that has run out (zero at
+  // rest; the stand-alone operators have their own)
+  DevBuf ctx_expired;
   int ctx_cache_held = IRT_CTX_CACHE_NATIVE;  // mode that the workspaces' cache buffers were made for
 
   // dimensions

@@ -6,6 +6,7 @@
 
 #include "codec.hpp"
 #include "common.hpp"
+#include "ctx_attn.hpp"
 #include "engine.hpp"
 #include "kernels.hpp"
 #include "lora.hpp"
@@ -258,6 +259,12 @@ IRTT_API int irtt_watchdog_probe(int which, unsigned long long limit_ns, int wai
     else if (which == 2) irt::conv_watchdog_probe(limit_ns, waits, elapsed_ns);
     else throw irt::Error(IRT_E_INVALID_ARG, "which must be 0, 1 or 2");
   });
+}
+
+// The same with the waits of the attention operators, reported to their word on
+// the current device.
+IRTT_API int irtt_attention_wait_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns) {
+  return guard([&] { irt::ctx_attn_watchdog_probe(limit_ns, waits, elapsed_ns, irt::ctx_attn_status()); });
 }
 
 // Reads and clears the watchdog flag of one translation unit (0 GEMM,
