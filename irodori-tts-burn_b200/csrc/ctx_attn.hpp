@@ -31,8 +31,9 @@ struct CtxAttnParams {
   const uint8_t* mask;       // [k_rows] or null
   float* lse;                // [q_rows, H] or null
   // Device memory that a bounded wait sets to 1 when it runs out; once it is
-  // set, every wait that reports here gives up at once.  The operators have one
-  // word per device (ctx_attn_status), an engine has its own.
+  // set, every wait that reports here gives up at once and later launches load
+  // nothing: what they write means nothing.  The operators have one word per device (ctx_attn_status),
+  // an engine has its own.
   int* expired;
 };
 

@@ -102,23 +102,30 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
 }
 
 // Bounded wait as tcx::mbar_wait, reported to `status` in the place of the
-// file's own flag.
-__device__ __forceinline__ void wait_or_report(uint32_t bar, uint32_t parity, int* status) {
-  if (mbar_try_wait(bar, parity)) return;
+// file's own flag; false where it gives up.
+__device__ __forceinline__ bool wait_or_report(uint32_t bar, uint32_t parity, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
   volatile int* flag = status;
-  if (*flag) return;
+  if (*flag) return false;
   const uint64_t limit = *reinterpret_cast<volatile unsigned long long*>(&g_wait_limit_ns);
   const uint64_t t0 = globaltimer();
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 256; ++i)
-      if (mbar_try_wait(bar, parity)) return;
-    if (*flag) return;
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*flag) return false;
     if (globaltimer() - t0 > limit) {
       atomicExch(status, 1);
-      return;
+      return false;
     }
   }
+}
+// Before a CTA with a late wait leaves: what it started (loads, products) may
+// still be on its way and must not reach the shared memory of the CTA that
+// takes its place.  A millisecond is a thousand times what a load takes.
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = globaltimer();
+  for (int i = 0; i < 10000 && globaltimer() - t0 < 1000000; ++i) __nanosleep(200);
 }
 
 // Box of a (d, head, row) tensor.
@@ -210,6 +217,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   pdl_wait();
   pdl_trigger();
   const CtxAttnParams& p = a.p;
+  // read by the TMA thread: after an expired wait nothing is loaded
+  const bool go = threadIdx.x != 128 || *reinterpret_cast<volatile int*>(p.expired) == 0;
   irt_attn_seq sd;
   const int split = a.split, rank = blockIdx.x % split, lg = a.log_gp, gmask = (1 << lg) - 1;
   int q0, head0;  // first query and first head of the tile
@@ -243,7 +252,15 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   auto P_FULL = [&](int b) { return bar(5 + 4 * NKV + b); };
   const uint32_t G_FULL = bar(7 + 4 * NKV);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 4 * NKV);
-  auto bar_wait = [&](uint32_t b, uint32_t parity) { wait_or_report(b, parity, p.expired); };
+  auto bar_wait = [&](uint32_t b, uint32_t parity) { return wait_or_report(b, parity, p.expired); };
+  // Waits of the threads that start loads and products, and those for the last
+  // of them.  The others leave it at that: next to them these cost 2 %.
+  __shared__ volatile int late;
+  auto own_wait = [&](uint32_t b, uint32_t parity) {
+    if (bar_wait(b, parity)) return true;
+    late = 1;
+    return false;
+  };
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sm_warps = (rows + 31) / 32;  // softmax warps that have a query row
@@ -262,7 +279,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
 
   // K (V) rows of local tile j, by the TMA thread
   auto load = [&](int j, uint32_t full, uint32_t empty, uint32_t dst, const CUtensorMap* self, const CUtensorMap* ctx) {
-    bar_wait(empty, ((j / NKV) & 1) ^ 1);
+    if (!own_wait(empty, ((j / NKV) & 1) ^ 1)) return;
     const bool own = t0 + j < n_self;
     if (CTX4 && !own) {  // the code warps fill this one
       mbar_arrive(full);
@@ -295,7 +312,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     }
     mbar_fence_init();
     fence_proxy_async();
-    if (nt > 0) {
+    late = 0;
+    if (nt > 0 && go) {
       mbar_expect_tx(Q_FULL, C::Q_BYTES);
 #pragma unroll
       for (int h = 0; h < HDT / 64; ++h) tma_load_3d(sQ + h * C::Q_HALF, &tmQ, Q_FULL, 64 * h, head0, sd.q_start + q0);
@@ -315,13 +333,13 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   if (nt > 0) {
     if (warp == 4) {
       // ---------------- TMA ----------------
-      if (lane == 0) {
+      if (lane == 0 && go) {
         for (int j = 0; j + 1 < nt; ++j) {  // K two tiles ahead of V, as the products are issued
           if (j + 2 < nt) load_k(j + 2);
           load_v(j + 1);
         }
-        if (split == 1 && p.gate.data) {  // the gate takes Q's place once the last scores are done
-          bar_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1);
+        // the gate takes Q's place once the last scores are done
+        if (split == 1 && p.gate.data && own_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1)) {
           mbar_expect_tx(G_FULL, C::Q_BYTES);
 #pragma unroll
           for (int h = 0; h < HDT / 64; ++h)
@@ -331,11 +349,11 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     } else if (warp == 5) {
       // ---------------- MMA ----------------
       if (lane == 0) {
-        bar_wait(Q_FULL, 0);
+        own_wait(Q_FULL, 0);
         tc_fence_after();
         auto issue_s = [&](int j) {
           const int r = j % NKV, b = j & 1;
-          bar_wait(K_FULL(r), (j / NKV) & 1);
+          own_wait(K_FULL(r), (j / NKV) & 1);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < HDT / 16; ++kk) {
@@ -350,8 +368,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         if (nt > 1) issue_s(1);
         for (int j = 0; j < nt; ++j) {
           const int s = j & 1, r = j % NKV;
-          bar_wait(V_FULL(r), (j / NKV) & 1);
-          bar_wait(P_FULL(s), (j >> 1) & 1);
+          own_wait(V_FULL(r), (j / NKV) & 1);
+          own_wait(P_FULL(s), (j >> 1) & 1);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < KT / 16; ++kk) {
@@ -560,7 +578,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(P_FULL(b));
       }
-      bar_wait(O_FINAL, 0);
+      own_wait(O_FINAL, 0);
       tc_fence_after();
     }
   }
@@ -577,7 +595,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       const bool gated = p.gate.data && nt > 0;
-      if (gated) bar_wait(G_FULL, 0);
+      if (gated) own_wait(G_FULL, 0);
 #pragma unroll 1
       for (int c = 0; c < HDT; c += 32) {
         uint32_t r[32], g[4][4];
@@ -725,6 +743,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
 
   tc_fence_before();
   __syncthreads();
+  if (late) settle();
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TM_COLS);

@@ -267,6 +267,29 @@ IRTT_API int irtt_attention_wait_probe(unsigned long long limit_ns, int waits, u
   return guard([&] { irt::ctx_attn_watchdog_probe(limit_ns, waits, elapsed_ns, irt::ctx_attn_status()); });
 }
 
+// Three sample() calls of a fresh engine with the 4-bit context cache, a wait
+// that reports to the engine running out before the second one; their statuses,
+// the second one's message and the outputs of the first and the last.
+IRTT_API int irtt_sample_after_expired_wait(const char* ckpt, int precision, const irt_sampler_params* sp,
+                                            const irt_request* rq, unsigned long long limit_ns, int* statuses,
+                                            float* first, float* last) {
+  return guard([&] {
+    irt::Engine e(0, ckpt, precision);
+    irt::validate_sampler_params(*sp);
+    e.params = *sp;
+    e.has_params = true;
+    e.ctx_cache = IRT_CTX_CACHE_4BIT;
+    std::string message;
+    for (int i = 0; i < 3; ++i) {
+      unsigned long long ns = 0;
+      if (i == 1) irt::ctx_attn_watchdog_probe(limit_ns, 1, &ns, e.ctx_expired.as<int>());
+      statuses[i] = guard([&] { e.sample(*rq, i == 0 ? first : last, IRT_MEM_HOST, nullptr); });
+      if (i == 1) message = g_err;
+    }
+    g_err = message;
+  });
+}
+
 // Reads and clears the watchdog flag of one translation unit (0 GEMM,
 // 1 attention, 2 conv); returns the flag's value or -1 on a bad index.
 IRTT_API int irtt_watchdog_read_and_clear(int which) {
