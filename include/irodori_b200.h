@@ -266,7 +266,8 @@ IRT_API int irt_codec_decode_noalloc(irt_codec* c, const float* latent, int32_t 
  * is device memory of GPU `device`; the work is queued on `stream` (a
  * cudaStream_t, NULL = that GPU's legacy default stream) and the call returns
  * without waiting for it, so it can be captured into a CUDA graph; and no
- * state is kept, so calls from several threads and streams are independent.
+ * state is kept, so calls from several threads and streams are independent
+ * (but for an expired wait, see irt_attention_check).
  * The current device of the calling thread is left as it was.
  *
  * Rows of heads: element (row, head, d) of a tensor is at
@@ -358,9 +359,12 @@ IRT_API int irt_kv4_read(int device, int dtype, const irt_kv4_cache* cache, int6
  * the cache alone. */
 IRT_API int irt_kv4_attention(const irt_attn_args* a, const irt_kv4_cache* cache, const irt_rows* k_self,
                               const irt_rows* v_self, void* stream);
-/* Waits for GPU `device` and reports whether a bounded wait inside one of the
- * attention operators' kernels has expired since the last check (IRT_E_CUDA:
- * outputs since then are invalid). */
+/* Waits for GPU `device` and reports whether a bounded wait (4 s) inside one of
+ * the attention operators' kernels has expired since the last check (IRT_E_CUDA:
+ * outputs since then are invalid).  From the expiry to this report
+ * irt_cross_attention and irt_kv4_attention answer IRT_E_CUDA on that GPU, and
+ * calls already queued or captured give up at once.  An engine's own waits are
+ * reported by irt_engine_sample and do not count here. */
 IRT_API int irt_attention_check(int device);
 
 #ifdef __cplusplus

@@ -254,7 +254,7 @@ int irt_cross_attention(const irt_attn_args* a, const irt_rows* k, const irt_row
     need(v, "v");
     irt::CtxAttnParams p = irt::ctx_attn_params(*a, nullptr, k, v, k_rows, nullptr, nullptr);
     irt::DeviceGuard dg(a->device);
-    p.expired = irt::ctx_attn_status();
+    irt::ctx_attn_report(p, a->device);
     irt::ctx_attention(p, reinterpret_cast<cudaStream_t>(stream));
   });
 }
@@ -266,7 +266,7 @@ int irt_kv4_attention(const irt_attn_args* a, const irt_kv4_cache* cache, const 
     need(cache, "cache");
     irt::CtxAttnParams p = irt::ctx_attn_params(*a, cache, nullptr, nullptr, cache->rows, k_self, v_self);
     irt::DeviceGuard dg(a->device);
-    p.expired = irt::ctx_attn_status();
+    irt::ctx_attn_report(p, a->device);
     irt::ctx_attention(p, reinterpret_cast<cudaStream_t>(stream));
   });
 }
@@ -302,7 +302,7 @@ int irt_attention_check(int device) {
   return guard([&] {
     irt::DeviceGuard dg(device);
     IRT_CUDA(cudaDeviceSynchronize());
-    if (irt::read_and_clear_ctx_attn_error())
+    if (irt::read_and_clear_ctx_attn_error(device))
       throw irt::Error(IRT_E_CUDA, "a bounded wait inside an attention operator expired: its outputs are invalid");
   });
 }

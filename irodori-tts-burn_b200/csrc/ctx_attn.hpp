@@ -35,6 +35,7 @@ struct CtxAttnParams {
   // nothing: what they write means nothing.  The operators have one word per device (ctx_attn_status),
   // an engine has its own.
   int* expired;
+  int* expired_host;         // a word in mapped host memory that is set with it, or null
 };
 
 // Range of sequence n; false when its table entry reaches outside the tensors
@@ -59,12 +60,20 @@ bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s);
 bool ctx_attention_kv4_rows(const CtxAttnParams& p, cudaStream_t s);
 // Many query rows in f32 arithmetic, head_dim <= 128 (ctx_attn_tile.cu); false as above.
 bool ctx_attention_tile(const CtxAttnParams& p, cudaStream_t s);
-// The operators' word for expired waits on the current device; reading clears it.
-int* ctx_attn_status();
-int read_and_clear_ctx_attn_error();
+// Where waits of the operators on device `dev`, the current one, report: `device` as
+// CtxAttnParams::expired, `host` as expired_host.  The host's word lets a call
+// see an expired wait without waiting for the GPU; reading clears both.
+struct CtxAttnStatus {
+  int *device, *host;
+};
+CtxAttnStatus ctx_attn_status(int dev);
+// Sets p's words to the operators'; throws while an expired wait is unreported.
+void ctx_attn_report(CtxAttnParams& p, int dev);
+int read_and_clear_ctx_attn_error(int dev);
 // Test hook: `waits` bounded waits of the kernels on a barrier that nothing
 // arrives on, with a limit of limit_ns each, reported to `expired`.
-void ctx_attn_watchdog_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns, int* expired);
+void ctx_attn_watchdog_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns,
+                             const CtxAttnStatus& report);
 
 // cache rows [row_start, row_start + n) from source rows idx[i] (or i); see
 // irt_kv4_append / irt_kv4_read.

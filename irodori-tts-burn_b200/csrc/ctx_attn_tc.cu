@@ -38,6 +38,8 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cstring>
+#include <mutex>
 
 #include "ctx_attn.cuh"
 #include "tc_common.cuh"
@@ -103,7 +105,7 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
 
 // Bounded wait as tcx::mbar_wait, reported to `status` in the place of the
 // file's own flag; false where it gives up.
-__device__ __forceinline__ bool wait_or_report(uint32_t bar, uint32_t parity, int* status) {
+__device__ __forceinline__ bool wait_or_report(uint32_t bar, uint32_t parity, int* status, int* host) {
   if (mbar_try_wait(bar, parity)) return true;
   volatile int* flag = status;
   if (*flag) return false;
@@ -116,6 +118,7 @@ __device__ __forceinline__ bool wait_or_report(uint32_t bar, uint32_t parity, in
     if (*flag) return false;
     if (globaltimer() - t0 > limit) {
       atomicExch(status, 1);
+      if (host) *reinterpret_cast<volatile int*>(host) = 1;
       return false;
     }
   }
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   auto P_FULL = [&](int b) { return bar(5 + 4 * NKV + b); };
   const uint32_t G_FULL = bar(7 + 4 * NKV);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 4 * NKV);
-  auto bar_wait = [&](uint32_t b, uint32_t parity) { return wait_or_report(b, parity, p.expired); };
+  auto bar_wait = [&](uint32_t b, uint32_t parity) { return wait_or_report(b, parity, p.expired, p.expired_host); };
   // Waits of the threads that start loads and products, and those for the last
   // of them.  The others leave it at that: next to them these cost 2 %.
   __shared__ volatile int late;
@@ -839,36 +842,70 @@ bool ctx_attention_tc(const CtxAttnParams& p, cudaStream_t s) {
   return p.hd > 64 ? launch<128, false>(p, s) : launch<64, false>(p, s);
 }
 
-int* ctx_attn_status() {
-  static std::atomic<int*> known[64];
-  int dev = 0;
-  IRT_CUDA(cudaGetDevice(&dev));
-  int* p = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
+CtxAttnStatus ctx_attn_status(int dev) {
+  constexpr int MAX_DEVICES = 64;
+  static std::atomic<int*> known[MAX_DEVICES];
+  static std::atomic<int*> words{nullptr};
+  static std::mutex mu;
+  if (dev >= MAX_DEVICES) throw unsupported("more than 64 devices");
+  int* w = words.load(std::memory_order_acquire);
+  if (!w) {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!(w = words.load(std::memory_order_acquire))) {
+      // the first call of a process may be captured into a graph; this allocation is no part of it
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      IRT_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+      const cudaError_t e =
+          cudaHostAlloc(reinterpret_cast<void**>(&w), MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      IRT_CUDA(e);
+      std::memset(w, 0, MAX_DEVICES * sizeof(int));
+      words.store(w, std::memory_order_release);
+    }
+  }
+  int* p = known[dev].load(std::memory_order_relaxed);
   if (!p) {
     IRT_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_watchdog));
-    if (dev < 64) known[dev].store(p, std::memory_order_relaxed);
+    known[dev].store(p, std::memory_order_relaxed);
   }
-  return p;
+  return {p, w + dev};
 }
 
-int read_and_clear_ctx_attn_error() { return read_and_clear_flag(); }
+void ctx_attn_report(CtxAttnParams& p, int dev) {
+  const CtxAttnStatus st = ctx_attn_status(dev);
+  if (*reinterpret_cast<volatile int*>(st.host))
+    throw Error(IRT_E_CUDA,
+                "a bounded wait inside an earlier attention operator expired: its outputs are invalid "
+                "(irt_attention_check reports it and lets calls through again)");
+  p.expired = st.device;
+  p.expired_host = st.host;
+}
+
+int read_and_clear_ctx_attn_error(int dev) {
+  const CtxAttnStatus st = ctx_attn_status(dev);
+  const int v = read_and_clear_flag();
+  *reinterpret_cast<volatile int*>(st.host) = 0;
+  return v;
+}
 
 namespace {
-__global__ void wait_probe_kernel(int waits, int* expired, unsigned long long* elapsed_ns) {
+__global__ void wait_probe_kernel(int waits, CtxAttnStatus report, unsigned long long* elapsed_ns) {
   __shared__ __align__(8) uint64_t bar;
   if (threadIdx.x == 0) {
     mbar_init(smem_u32(&bar), 1);
     const uint64_t t0 = globaltimer();
-    for (int i = 0; i < waits; ++i) wait_or_report(smem_u32(&bar), 0, expired);  // phase 0 never completes
+    for (int i = 0; i < waits; ++i)
+      wait_or_report(smem_u32(&bar), 0, report.device, report.host);  // phase 0 never completes
     *elapsed_ns = globaltimer() - t0;
   }
 }
 }  // namespace
 
-void ctx_attn_watchdog_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns, int* expired) {
+void ctx_attn_watchdog_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns,
+                             const CtxAttnStatus& report) {
   DevBuf d(sizeof(*elapsed_ns));
   IRT_CUDA(set_wait_limit_ns(limit_ns));
-  wait_probe_kernel<<<1, 32>>>(waits, expired, d.as<unsigned long long>());
+  wait_probe_kernel<<<1, 32>>>(waits, report, d.as<unsigned long long>());
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   IRT_CUDA(set_wait_limit_ns(DEFAULT_WAIT_LIMIT_NS));

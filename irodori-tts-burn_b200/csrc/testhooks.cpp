@@ -262,9 +262,9 @@ IRTT_API int irtt_watchdog_probe(int which, unsigned long long limit_ns, int wai
 }
 
 // The same with the waits of the attention operators, reported to their word on
-// the current device.
+// device 0.
 IRTT_API int irtt_attention_wait_probe(unsigned long long limit_ns, int waits, unsigned long long* elapsed_ns) {
-  return guard([&] { irt::ctx_attn_watchdog_probe(limit_ns, waits, elapsed_ns, irt::ctx_attn_status()); });
+  return guard([&] { irt::ctx_attn_watchdog_probe(limit_ns, waits, elapsed_ns, irt::ctx_attn_status(0)); });
 }
 
 // Three sample() calls of a fresh engine with the 4-bit context cache, a wait
@@ -282,7 +282,7 @@ IRTT_API int irtt_sample_after_expired_wait(const char* ckpt, int precision, con
     std::string message;
     for (int i = 0; i < 3; ++i) {
       unsigned long long ns = 0;
-      if (i == 1) irt::ctx_attn_watchdog_probe(limit_ns, 1, &ns, e.ctx_expired.as<int>());
+      if (i == 1) irt::ctx_attn_watchdog_probe(limit_ns, 1, &ns, {e.ctx_expired.as<int>(), nullptr});
       statuses[i] = guard([&] { e.sample(*rq, i == 0 ? first : last, IRT_MEM_HOST, nullptr); });
       if (i == 1) message = g_err;
     }

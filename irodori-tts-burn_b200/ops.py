@@ -358,5 +358,6 @@ def kv4_attention(q, cache: Kv4Cache, seqs, max_q_len: int, max_k_len: int, k_se
 
 def attention_check(device: int = 0) -> None:
     """Waits for the GPU and raises if a bounded wait inside an attention
-    operator's kernel has expired since the last check."""
+    operator's kernel has expired since the last check; until then the attention
+    calls on that GPU raise too."""
     _check(lib().irt_attention_check(device))

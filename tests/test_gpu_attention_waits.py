@@ -135,3 +135,42 @@ def test_the_engine_reports_its_own(pkg, dev, synth, ckpt_dir, probe):  # noqa: 
     assert list(statuses) == [0, 20, 0] and "4-bit context cache" in message
     assert np.isfinite(first).all() and np.linalg.norm(last - first) <= 2e-2 * np.linalg.norm(first)
     pkg.attention_check(0)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_calls_after_an_expired_wait(pkg, dev, probe, four_bit):  # noqa: F811
+    """No call returns success with outputs that mean nothing: they are refused, without a wait for the GPU and inside
+    a capture too, until the check has reported the wait."""
+    h, hd, nk, ql = 2, 128, 90, 20
+    q = torch.randn(ql, h, hd, device=dev).to(torch.bfloat16)
+    k, v = torch.randn(2, nk, h, hd, device=dev).to(torch.bfloat16).unbind(0)
+    tab, cache, out = pkg.attention_table([ql], [nk]), pkg.Kv4Cache(nk, h, hd), torch.full_like(q, 3.0)
+
+    def call():
+        if four_bit:
+            return pkg.kv4_attention(q, cache, tab, ql, nk, out=out)
+        return pkg.cross_attention(q, k, v, tab, ql, nk, out=out)
+
+    pkg.kv4_append(cache, k, v)
+    want = call().clone()
+    expire(probe)
+    out.fill_(3.0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(2):
+            with pytest.raises(pkg.IrodoriError) as ei:
+                call()
+            assert ei.value.kind == "Cuda" and "irt_attention_check" in str(ei.value)
+        again = q * 1  # the capture goes on
+    with pytest.raises(pkg.IrodoriError):
+        call()
+    pkg.kv4_append(cache, k, v)  # no waits inside: not refused
+    pkg.kv4_read(cache)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, q) and (out == 3).all()
+    with pytest.raises(pkg.IrodoriError) as ei:
+        pkg.attention_check(0)
+    assert ei.value.kind == "Cuda" and "bounded wait" in str(ei.value)
+    assert torch.equal(call(), want)
+    pkg.attention_check(0)
