@@ -16,8 +16,10 @@ Unlike ``InferenceEngine.sample`` the calls queue their work and return: with
 ``stream=None`` on torch's current stream of the tensors' GPU (whichever GPU is
 current), so they order like torch's own operators and can be captured into a
 CUDA graph.  On an explicit ``stream`` the caller orders the work before and
-after; the tensors' memory is kept until that stream is done with it.  They are forward only; a tensor that requires a gradient is
-refused while gradients are recorded.
+after; the tensors' memory is kept until that stream is done with it.  They are
+forward only: a tensor that requires a gradient is refused while gradients are
+recorded, one with a forward-mode tangent too, and so is torch.jit.trace, which
+would record a call's allocations and not its kernel.
 """
 
 from __future__ import annotations
@@ -46,26 +48,43 @@ SIGNATURES = {
 GROUP = 32  # values that share a scale in the 4-bit cache
 
 _torch = None
+_forward_ad = None
 _dtype_code = None  # torch dtype -> irt_precision
 _INT32 = _MASKS = None
 
 
 def _t():
     """torch, imported at the first call (the package itself does not need it)."""
-    global _torch, _dtype_code, _INT32, _MASKS
+    global _torch, _forward_ad, _dtype_code, _INT32, _MASKS
     if _torch is None:
         import torch
-        _torch = torch
+        import torch.autograd.forward_ad
+        _torch, _forward_ad = torch, torch.autograd.forward_ad
         _INT32, _MASKS = (torch.int32,), (torch.uint8, torch.bool)
         _dtype_code = {torch.bfloat16: PREC["bf16"], torch.float32: PREC["f32"]}
     return _torch
+
+
+def _no_gradient(name, t):
+    if t.requires_grad and _torch.is_grad_enabled():
+        raise IrodoriError(4, f"Unsupported mode: {name} requires a gradient; the operators are forward only "
+                              "(call them under torch.no_grad())")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise IrodoriError(4, f"Unsupported mode: {name} has a forward-mode tangent, which the operators would lose "
+                              "(pass its primal)")
+
+
+def _no_tracing():
+    if _torch._C._is_tracing():
+        raise IrodoriError(4, "Unsupported mode: torch.jit.trace records torch's own operators only")
 
 
 def _heads(name, t, device, dtype, shape):
     """(address, row stride, head stride) of a [rows, heads, head_dim] tensor (any strides, the last one 1)."""
     if not isinstance(t, _torch.Tensor):
         raise IrodoriError(22, f"{name} must be a torch CUDA tensor")
-    if t.dtype is dtype and t.get_device() == device and t.shape == shape and not t.requires_grad:
+    if t.dtype is dtype and t.get_device() == device and t.shape == shape and not t.requires_grad and \
+            _forward_ad._current_level < 0:
         row, head, one = t.stride()
         if one == 1:
             return t.data_ptr(), row, head
@@ -75,9 +94,7 @@ def _heads(name, t, device, dtype, shape):
         raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
     if t.get_device() != device:
         raise IrodoriError(22, f"{name} must be on cuda:{device}, got {t.device}")
-    if t.requires_grad and _torch.is_grad_enabled():
-        raise IrodoriError(4, f"Unsupported mode: {name} requires a gradient; the operators are forward only "
-                              "(call them under torch.no_grad())")
+    _no_gradient(name, t)
     if t.stride(2) != 1 and t.numel():
         raise IrodoriError(22, f"{name}: the values of a head must be contiguous")
     return t.data_ptr(), t.stride(0), t.stride(1)
@@ -85,6 +102,7 @@ def _heads(name, t, device, dtype, shape):
 
 def _first(name, t):
     torch = _t()
+    _no_tracing()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise IrodoriError(22, f"{name} must be a torch CUDA tensor")
     if t.dim() != 3:
@@ -97,7 +115,7 @@ def _first(name, t):
 def _plain(name, t, device, dtypes, shape):
     """Address of a contiguous helper tensor (table, mask, index, cache buffer)."""
     if isinstance(t, _torch.Tensor) and t.dtype in dtypes and t.get_device() == device and t.shape == shape and \
-            t.is_contiguous():
+            t.is_contiguous() and not t.requires_grad and _forward_ad._current_level < 0:
         return t.data_ptr()
     if not isinstance(t, _torch.Tensor) or t.get_device() != device:
         raise IrodoriError(22, f"{name} must be a tensor on cuda:{device}")
@@ -105,7 +123,10 @@ def _plain(name, t, device, dtypes, shape):
         raise IrodoriError(9, f"{name} must be {dtypes[0]}, got {t.dtype}")
     if t.shape != shape:
         raise IrodoriError(2, f"Shape mismatch: {name} must be {list(shape)}, got {list(t.shape)}")
-    raise IrodoriError(22, f"{name} must be contiguous")
+    if not t.is_contiguous():
+        raise IrodoriError(22, f"{name} must be contiguous")
+    _no_gradient(name, t)
+    return t.data_ptr()
 
 
 def _stream(stream, device):
@@ -247,6 +268,7 @@ def kv4_read(cache: Kv4Cache, row_start: int = 0, rows=None, dtype=None, stream=
     float32; exact in both for scales of 5 significant bits, in float32 for
     any)."""
     torch = _t()
+    _no_tracing()
     dtype = torch.bfloat16 if dtype is None else dtype
     if dtype not in _dtype_code:
         raise IrodoriError(9, f"dtype must be bfloat16 or float32, got {dtype}")
