@@ -9,6 +9,7 @@
 // (maximum, sum, output) triples are merged in a fixed order: results do not
 // depend on timing, and no workspace is needed.
 #include <algorithm>
+#include <numeric>
 #include <type_traits>
 
 #include "ctx_attn.cuh"
@@ -328,27 +329,43 @@ constexpr long MAX_ROWS = (1L << 30) - 1;
 
 Error arg_error(const std::string& m) { return Error(IRT_E_INVALID_ARG, m); }
 
-// First and one-past-last byte of a tensor; for rows of heads also the bytes
-// from one row to the next and those that a row spans.
+// First and one-past-last byte of a tensor.  For rows of heads also the windows
+// that its bytes repeat in: every byte is in [lo + i period, + extent) for some
+// i, with the step that rows and heads share, that of the rows, and that of the
+// heads as the period (0: no such window).
 struct Span {
-  uintptr_t lo, hi, period, extent;
+  uintptr_t lo, hi;
+  struct {
+    uintptr_t period, extent;
+  } win[3];
 };
 Span span_of(const irt_rows& r, long rows, int heads, int hd, int esz) {
   const uintptr_t lo = reinterpret_cast<uintptr_t>(r.data);
-  if (!r.data || rows <= 0) return {lo, lo, 0, 0};
-  const uintptr_t extent = (uintptr_t)((heads - 1) * r.head_stride + hd) * esz, period = (uintptr_t)r.row_stride * esz;
-  return {lo, lo + (rows - 1) * period + extent, period, extent};
+  if (!r.data || rows <= 0) return {lo, lo, {}};
+  // a stride that nothing steps by says nothing
+  const long row = rows > 1 ? r.row_stride : 0, head = heads > 1 ? r.head_stride : 0;
+  const uintptr_t in_row = (heads - 1) * head + hd, in_head = (rows - 1) * row + hd;
+  Span s{lo, lo + ((rows - 1) * row + in_row) * esz, {}};
+  s.win[0] = {(uintptr_t)std::gcd(row, head) * esz, (uintptr_t)hd * esz};
+  s.win[1] = {(uintptr_t)row * esz, in_row * esz};
+  s.win[2] = {(uintptr_t)head * esz, in_head * esz};
+  return s;
 }
 Span span_of(const void* data, long bytes) {
   const uintptr_t lo = reinterpret_cast<uintptr_t>(data);
-  return {lo, data ? lo + bytes : lo, 0, 0};
+  return {lo, data ? lo + bytes : lo, {}};
 }
 bool overlap(const Span& a, const Span& b) {
-  if (a.lo >= b.hi || b.lo >= a.hi) return false;
-  if (a.period == 0 || a.period != b.period) return true;
-  // columns of one tensor: rows of both in the same period, side by side
-  const uintptr_t d = b.lo >= a.lo ? (b.lo - a.lo) % a.period : (a.period - (a.lo - b.lo) % a.period) % a.period;
-  return d < a.extent || d + b.extent > a.period;
+  if (a.lo == a.hi || b.lo == b.hi || a.lo >= b.hi || b.lo >= a.hi) return false;
+  // inside one tensor: apart where windows of the same period lie side by side
+  for (const auto& x : a.win)
+    for (const auto& y : b.win) {
+      const uintptr_t p = x.period;
+      if (p == 0 || p != y.period) continue;
+      const uintptr_t d = b.lo >= a.lo ? (b.lo - a.lo) % p : (p - (a.lo - b.lo) % p) % p;
+      if (d >= x.extent && d + y.extent <= p) return false;
+    }
+  return true;
 }
 
 void check_rows(const char* name, const irt_rows& r, long rows, int heads, int esz) {
