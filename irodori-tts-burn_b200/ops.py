@@ -294,7 +294,8 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
     n, h, d = shape = q.shape
     dev, dtype = q.get_device(), q.dtype
     handle, side = _stream(stream, dev)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty_like(side, q)
         out_row, out_head, _ = out.stride()
         out_p = out.data_ptr()
@@ -322,6 +323,8 @@ def _attention(call, q, kv_heads, k_rows, seqs, max_q_len, max_k_len, key_mask, 
     status = call(a, *context, handle)
     if status:
         _check(status)
+    if given:
+        torch.autograd.graph.increment_version(out)  # autograd's record of in-place writes
     if side is not None:
         _keep(side, q, seqs, key_mask, gate, out, *keep)
     return (out, lse) if return_lse else out
