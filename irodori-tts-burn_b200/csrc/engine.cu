@@ -940,15 +940,12 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
     to_device(ws.rowmap_t, map_t.data(), map_t.size(), IRT_MEM_HOST, s);
     if (aux_in) to_device(ws.rowmap_a, map_a.data(), map_a.size(), IRT_MEM_HOST, s);
     const int nl = !skv_cfg ? 0 : pr.speaker_kv_max_layers < 0 ? L : std::min(pr.speaker_kv_max_layers, L);
-    int nscaled = 0;  // rows of the scaled speaker copies (SpeakerKvConfig, src/rf/kv_scaling.rs:10-60)
+    std::vector<int> scaled;  // rows of the scaled speaker copies (SpeakerKvConfig, src/rf/kv_scaling.rs:10-60)
     if (skv_cfg) {
       to_device(ws.rowmap_as, map_as.data(), map_as.size(), IRT_MEM_HOST, s);
-      std::vector<int> rows;
       for (int b = 0; b < B; ++b)
-        for (int i = 0; i < sc[b]; ++i) rows.push_back(base[b] + i);
-      to_device(ws.rows, rows.data(), rows.size(), IRT_MEM_HOST, s);
-      nscaled = (int)rows.size();
-      IRT_CUDA(cudaStreamSynchronize(s));
+        for (int i = 0; i < sc[b]; ++i) scaled.push_back(base[b] + i);
+      to_device(ws.rows, scaled.data(), scaled.size(), IRT_MEM_HOST, s);
     }
     // K and V of layers [l0, l0 + n) into cache_k / cache_v from layer 0 on
     auto project = [&](int l0, int n) {
@@ -975,8 +972,8 @@ void Engine::sample(const irt_request& rq, float* out, int out_memory, cudaStrea
       for (int l = l0; l < std::min(nl, l0 + n); ++l) {
         uint8_t* kl = ws.cache_k.as<uint8_t>() + (size_t)(l - l0) * lstride_el * esz();
         uint8_t* vl = ws.cache_v.as<uint8_t>() + (size_t)(l - l0) * lstride_el * esz();
-        scale_rows_bf16_or_f32(kl, bf, D, ws.rows.as<int>(), nscaled, pr.speaker_kv_scale, s);
-        scale_rows_bf16_or_f32(vl, bf, D, ws.rows.as<int>(), nscaled, pr.speaker_kv_scale, s);
+        scale_rows_bf16_or_f32(kl, bf, D, ws.rows.as<int>(), (int)scaled.size(), pr.speaker_kv_scale, s);
+        scale_rows_bf16_or_f32(vl, bf, D, ws.rows.as<int>(), (int)scaled.size(), pr.speaker_kv_scale, s);
       }
     };
     if (!kv4) {
