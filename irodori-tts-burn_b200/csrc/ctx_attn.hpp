@@ -35,7 +35,7 @@ struct CtxAttnParams {
   // nothing: what they write means nothing.  The operators have one word per device (ctx_attn_status),
   // an engine has its own.
   int* expired;
-  int* expired_host;         // a word in mapped host memory that is set with it, or null
+  int* expired_host;         // a word in mapped host memory that a CTA with such a wait sets, or null
 };
 
 // Range of sequence n; false when its table entry reaches outside the tensors

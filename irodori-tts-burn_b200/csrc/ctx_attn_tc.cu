@@ -104,29 +104,32 @@ __device__ __forceinline__ void tmem_st_cols(uint32_t taddr, const uint32_t (&r)
 }
 
 // Bounded wait as tcx::mbar_wait, reported to `status` in the place of the
-// file's own flag; false where it gives up.
-__device__ __forceinline__ bool wait_or_report(uint32_t bar, uint32_t parity, int* status, int* host) {
-  if (mbar_try_wait(bar, parity)) return true;
+// file's own flag.
+__device__ __forceinline__ void wait_or_report(uint32_t bar, uint32_t parity, int* status) {
+  if (mbar_try_wait(bar, parity)) return;
   volatile int* flag = status;
-  if (*flag) return false;
+  if (*flag) return;
   const uint64_t limit = *reinterpret_cast<volatile unsigned long long*>(&g_wait_limit_ns);
   const uint64_t t0 = globaltimer();
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 256; ++i)
-      if (mbar_try_wait(bar, parity)) return true;
-    if (*flag) return false;
+      if (mbar_try_wait(bar, parity)) return;
+    if (*flag) return;
     if (globaltimer() - t0 > limit) {
       atomicExch(status, 1);
-      if (host) *reinterpret_cast<volatile int*>(host) = 1;
-      return false;
+      return;
     }
   }
 }
-// Before a CTA with a late wait leaves: what it started (loads, products) may
-// still be on its way and must not reach the shared memory of the CTA that
-// takes its place.  A millisecond is a thousand times what a load takes.
-__device__ __forceinline__ void settle() {
+// For a CTA with an expired wait, before it leaves: tells the host, and stays.
+// What it started (loads, products) may still be on its way and must not reach
+// the shared memory of the CTA that takes its place; a millisecond is a
+// thousand times what a load takes.  Not inlined, and looked for where the
+// chain does not wait: next to the softmax a few instructions more in every
+// wait cost the 4-bit kernel 5 %.
+__device__ __noinline__ void settle(int* host) {
+  if (host) *reinterpret_cast<volatile int*>(host) = 1;
   const uint64_t t0 = globaltimer();
   for (int i = 0; i < 10000 && globaltimer() - t0 < 1000000; ++i) __nanosleep(200);
 }
@@ -255,15 +258,7 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
   auto P_FULL = [&](int b) { return bar(5 + 4 * NKV + b); };
   const uint32_t G_FULL = bar(7 + 4 * NKV);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8 + 4 * NKV);
-  auto bar_wait = [&](uint32_t b, uint32_t parity) { return wait_or_report(b, parity, p.expired, p.expired_host); };
-  // Waits of the threads that start loads and products, and those for the last
-  // of them.  The others leave it at that: next to them these cost 2 %.
-  __shared__ volatile int late;
-  auto own_wait = [&](uint32_t b, uint32_t parity) {
-    if (bar_wait(b, parity)) return true;
-    late = 1;
-    return false;
-  };
+  auto bar_wait = [&](uint32_t b, uint32_t parity) { wait_or_report(b, parity, p.expired); };
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sm_warps = (rows + 31) / 32;  // softmax warps that have a query row
@@ -282,7 +277,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
 
   // K (V) rows of local tile j, by the TMA thread
   auto load = [&](int j, uint32_t full, uint32_t empty, uint32_t dst, const CUtensorMap* self, const CUtensorMap* ctx) {
-    if (!own_wait(empty, ((j / NKV) & 1) ^ 1)) return;
+    bar_wait(empty, ((j / NKV) & 1) ^ 1);
+    if (!mbar_try_wait(empty, ((j / NKV) & 1) ^ 1)) return;  // gave up: nothing more is started
     const bool own = t0 + j < n_self;
     if (CTX4 && !own) {  // the code warps fill this one
       mbar_arrive(full);
@@ -315,7 +311,6 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     }
     mbar_fence_init();
     fence_proxy_async();
-    late = 0;
     if (nt > 0 && go) {
       mbar_expect_tx(Q_FULL, C::Q_BYTES);
 #pragma unroll
@@ -342,7 +337,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
           load_v(j + 1);
         }
         // the gate takes Q's place once the last scores are done
-        if (split == 1 && p.gate.data && own_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1)) {
+        if (split == 1 && p.gate.data) {
+          bar_wait(K_EMPTY((nt - 1) % NKV), ((nt - 1) / NKV) & 1);
           mbar_expect_tx(G_FULL, C::Q_BYTES);
 #pragma unroll
           for (int h = 0; h < HDT / 64; ++h)
@@ -352,11 +348,11 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
     } else if (warp == 5) {
       // ---------------- MMA ----------------
       if (lane == 0) {
-        own_wait(Q_FULL, 0);
+        bar_wait(Q_FULL, 0);
         tc_fence_after();
         auto issue_s = [&](int j) {
           const int r = j % NKV, b = j & 1;
-          own_wait(K_FULL(r), (j / NKV) & 1);
+          bar_wait(K_FULL(r), (j / NKV) & 1);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < HDT / 16; ++kk) {
@@ -371,8 +367,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         if (nt > 1) issue_s(1);
         for (int j = 0; j < nt; ++j) {
           const int s = j & 1, r = j % NKV;
-          own_wait(V_FULL(r), (j / NKV) & 1);
-          own_wait(P_FULL(s), (j >> 1) & 1);
+          bar_wait(V_FULL(r), (j / NKV) & 1);
+          bar_wait(P_FULL(s), (j >> 1) & 1);
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < KT / 16; ++kk) {
@@ -384,6 +380,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
           if (j + 2 < nt) issue_s(j + 2);  // overwrites S_j / P_j after P_j V_j in the tensor pipe's order
         }
         umma_commit(O_FINAL);
+        // a wait has given up before (read while the last rows are written)
+        if (*reinterpret_cast<volatile int*>(p.expired)) settle(p.expired_host);
       }
     } else if (CTX4 && warp >= 6) {
       // ---------------- codes -> bf16 tiles ----------------
@@ -581,7 +579,8 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(P_FULL(b));
       }
-      own_wait(O_FINAL, 0);
+      bar_wait(O_FINAL, 0);
+      if (!__all_sync(0xffffffffu, mbar_try_wait(O_FINAL, 0))) settle(p.expired_host);
       tc_fence_after();
     }
   }
@@ -598,7 +597,10 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
       const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
       const bool gated = p.gate.data && nt > 0;
-      if (gated) own_wait(G_FULL, 0);
+      if (gated) {
+        bar_wait(G_FULL, 0);
+        if (!__all_sync(0xffffffffu, mbar_try_wait(G_FULL, 0))) settle(p.expired_host);
+      }
 #pragma unroll 1
       for (int c = 0; c < HDT; c += 32) {
         uint32_t r[32], g[4][4];
@@ -746,7 +748,6 @@ __global__ void __launch_bounds__(Cfg<HDT, CTX4>::THREADS, 2)
 
   tc_fence_before();
   __syncthreads();
-  if (late) settle();
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TM_COLS);
@@ -895,8 +896,9 @@ __global__ void wait_probe_kernel(int waits, CtxAttnStatus report, unsigned long
     mbar_init(smem_u32(&bar), 1);
     const uint64_t t0 = globaltimer();
     for (int i = 0; i < waits; ++i)
-      wait_or_report(smem_u32(&bar), 0, report.device, report.host);  // phase 0 never completes
+      wait_or_report(smem_u32(&bar), 0, report.device);  // phase 0 never completes
     *elapsed_ns = globaltimer() - t0;
+    if (*reinterpret_cast<volatile int*>(report.device)) settle(report.host);
   }
 }
 }  // namespace
