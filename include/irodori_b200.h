@@ -273,8 +273,10 @@ IRT_API int irt_codec_decode_noalloc(irt_codec* c, const float* latent, int32_t 
  * Rows of heads: element (row, head, d) of a tensor is at
  * data[row * row_stride + head * head_stride + d], strides in elements.
  * Types: irt_precision (IRT_PREC_BF16: bf16, IRT_PREC_F32: float) for every
- * tensor of a call; scores, softmax and sums are f32 in both.  Weights are at
- * most 1 before the normalisation: sums of values stay finite where the
+ * tensor of a call; scores, softmax and sums are f32 in both.  In bf16 calls
+ * the weights (over 4 bits with few queries: weight times scale) are rounded to
+ * bf16 before they meet the values, the sum of the weights is not.  Weights are
+ * at most 1 before the normalisation: sums of values stay finite where the
  * values' magnitudes, summed over the keys, do.  Query head h reads KV head
  * h / (heads / kv_heads).  head_dim is a multiple of 8, 8..256.
  */
@@ -356,7 +358,8 @@ IRT_API int irt_kv4_read(int device, int dtype, const irt_kv4_cache* cache, int6
 /* Attention over [own rows | context rows of the cache].  k_self, v_self
  * [q_rows, kv_heads, head_dim]: a sequence's queries also attend to the rows
  * of its own query range, unmasked, as in the model's joint attention; NULL:
- * the cache alone. */
+ * the cache alone.  Without them few bf16 queries are multiplied with the codes
+ * before the scales: their magnitudes must stay below 2^115. */
 IRT_API int irt_kv4_attention(const irt_attn_args* a, const irt_kv4_cache* cache, const irt_rows* k_self,
                               const irt_rows* v_self, void* stream);
 /* Waits for GPU `device` and reports whether a bounded wait (4 s) inside one of

@@ -29,12 +29,13 @@
 // Many queries: bound by the latency of a CTA's chain (load, scores, softmax,
 // product, rows out), of which an SM runs two: 256 of its 512 TMEM columns
 // each, for two score tiles and O.  About 6.5 us a CTA and 0.9 us a key tile:
-// 64 x 16 heads, 768 queries over 64 / 640 / 1280 keys 139 / 317 / 546 us, the
-// last at 0.94 PFLOP/s; 64 utterances of 50 to 750 frames over 141 to 632 rows
-// 157 us.  4-bit context with own rows 337 us, there also bound by the issue of
+// 64 x 16 heads, 768 queries over 64 / 640 / 1280 keys without a gate 130 / 303 /
+// 535 us, the last at 0.96 PFLOP/s; 64 utterances of 50 to 750 frames over 141 to 632 rows
+// 158 us.  4-bit context with own rows 338 us, there also bound by the issue of
 // instructions of the code warps.  One query: bound by reading K and V, 6.1
 // TB/s over 5000 to 8192 rows.  Fewer keys a tile would leave the tensor pipe
-// waiting for softmax; 128 would need both halves of TMEM for one CTA.
+// waiting for softmax.  All 512 columns for one CTA (128 keys a tile, or two
+// query tiles that share each K and V tile) have not been measured.
 #include <cooperative_groups.h>
 
 #include <algorithm>

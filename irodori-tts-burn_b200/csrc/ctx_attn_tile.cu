@@ -10,12 +10,13 @@
 // packed f32 pairs along the head dimension (half the instructions of scalar
 // ones).  Bound by the FP32 pipe (61 %) and shared-memory passes (73 %): two
 // sequences of 750 queries over 576 rows 223 us, with own rows and a 4-bit
-// context 524 us, 31 to 33 TFLOP/s.  8 x 4 scores a thread halve the passes and
-// the warps: 241 us.  f32 halves on the tensor cores are out: their
-// accumulators truncate, and scores need the error of f32 sums.  Query rows are scaled by scale log2(e) on the way
-// in.  K of the next tile is loaded during softmax and P V, V during the next
-// scores.  Shared rows of Q, K, V are f32, their 16-byte chunks XOR-swizzled by
-// the row against bank conflicts.
+// context 530 us, 31 to 33 TFLOP/s.  8 x 4 scores a thread halve the passes and
+// the warps: 241 us.  tf32 halves on the tensor cores with sums handed over in
+// chunks, as the f32 GEMM has them, have not been tried for these products.
+// Query rows are scaled by scale log2(e) on the way in.  K of the next tile is
+// loaded during softmax and P V, V during the next scores.  Shared rows of Q, K,
+// V are f32, their 16-byte chunks XOR-swizzled by the row against bank
+// conflicts.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -2,8 +2,10 @@
 attention to an encoder's states, and the context cache held in 4 bits.
 
 The engine's joint attention (src/model/attention.rs:403-418, :619-664) reads
-its latent frames and its text / speaker rows in one pass; these calls offer
-the same attention to programs that keep queries and context rows themselves.
+its latent frames and its text / speaker rows in one pass.  These calls are for
+programs that keep queries and context rows themselves: ``kv4_attention`` reads
+both as the engine does, from a 4-bit context; ``cross_attention`` reads a
+native context alone.
 
     table = attention_table(q_lens, k_lens, device=0)           # once per batch
     out = cross_attention(q, k, v, table, max(q_lens), max(k_lens))
